@@ -39,6 +39,7 @@ extern "C" {
 
 #define MEP_F32 0
 #define MEP_BF16 1
+#define MEP_E4M3 2 /* 8-bit floats with one fp32 scale a row (key/value caches only) */
 
 #define MEP_IPC_HANDLE_BYTES 64
 
@@ -293,6 +294,98 @@ int mep_dest_ranks_noalloc(int num_experts, int world, const int64_t* table,
                            const int64_t* n_rep, int rmax, int64_t* rr,
                            const int64_t* expert_ids, int64_t m, int64_t* dest_out,
                            void* stream);
+
+/*
+ * Decode-step operators. They take no context: tensors, sizes and strides (in
+ * elements) are all in the arguments, messages come from mep_last_error(NULL),
+ * and calls on different streams or threads share nothing but what their
+ * arguments share. `dtype` is the model dtype (MEP_F32 or MEP_BF16).
+ * Pointers start on 16-byte boundaries and the strides of q, k and v are
+ * multiples of 16 bytes. head_dim is a multiple of 16 up to 128; query head h
+ * reads key/value head h / (q_heads / kv_heads).
+ *
+ * A layer's cache is (batch, kv_heads, capacity, head_dim), contiguous, in the
+ * model dtype or in MEP_E4M3 (`cache_dtype`) with fp32 scales (batch,
+ * kv_heads, capacity). `col` is the cache column of the call's first token
+ * (token t: column col + t); with col_dev non-NULL it is read on the device
+ * from there instead (one int64), so that a captured graph can advance it.
+ * Columns outside [0, capacity) are then neither written nor read.
+ */
+
+/*
+ * Head norms, rotation and cache write of new tokens in one pass. q, k
+ * (optionally RMS-normalised over each head with weights q_norm / k_norm
+ * (head_dim,), NULL for none) are rotated by the tables' row positions[b][t]:
+ *   r[i] = y[i] cos[i] - y[i + D/2] sin[i]
+ *   r[i + D/2] = y[i + D/2] cos[i + D/2] + y[i] sin[i + D/2]
+ * in fp32, rounded once. q goes to q_out (batch, tokens, q_heads, head_dim),
+ * k and the unrotated v to the cache. A quantised row holds
+ * e4m3(x * (448 / a)) and the scale a / 448, a = max |x| (a < 2^-100: zeros).
+ * cos / sin: (table_rows, head_dim), fp32 or the model dtype (table_dtype).
+ * A position outside the tables gives NaN rows.
+ */
+int mep_norm_rope_store(int dtype, int cache_dtype, int64_t batch, int64_t tokens, int q_heads,
+                        int kv_heads, int head_dim, const void* q, int64_t q_sb, int64_t q_st,
+                        int64_t q_sh, const void* k, int64_t k_sb, int64_t k_st, int64_t k_sh,
+                        const void* v, int64_t v_sb, int64_t v_st, int64_t v_sh,
+                        const void* q_norm, const void* k_norm, float eps, const void* cos,
+                        const void* sin, int table_dtype, int64_t table_rows,
+                        const int64_t* positions, int64_t p_sb, int64_t p_st, void* q_out,
+                        void* k_cache, void* v_cache, float* k_scale, float* v_scale,
+                        int64_t capacity, int64_t col, const int64_t* col_dev, void* stream);
+
+/*
+ * Columns [start, start + columns) of a quantised layer in the model dtype:
+ * k_out, v_out (batch, kv_heads, columns, head_dim).
+ */
+int mep_kv_read(int dtype, int64_t batch, int kv_heads, int head_dim, const void* k_cache,
+                const void* v_cache, const float* k_scale, const float* v_scale, int64_t capacity,
+                int64_t start, int64_t columns, void* k_out, void* v_out, void* stream);
+
+/*
+ * Attention of `tokens` new tokens a row over the cache and, with prefix_cols
+ * > 0, a prefix all rows share (k_prefix, v_prefix: (kv_heads, prefix_cols,
+ * head_dim) in the model dtype), whose scores are computed for the whole
+ * batch at once. Query (b, t) sees the whole prefix and the own columns c with
+ * c <= col + t and (c < lengths[b] or c >= prompt_cols): the row's prompt in
+ * columns [0, lengths[b]) of the padded prompt_cols, and what was decoded
+ * behind them (lengths NULL: every c <= col + t). A query that sees nothing
+ * gets zeros. q: (batch, tokens, q_heads, head_dim) strided; out the same,
+ * contiguous. workspace: mep_cache_attention_workspace bytes, the caller's, in
+ * use until the call's work on `stream` is done.
+ */
+int mep_cache_attention(int dtype, int cache_dtype, int64_t batch, int64_t tokens, int q_heads,
+                        int kv_heads, int head_dim, const void* q, int64_t q_sb, int64_t q_st,
+                        int64_t q_sh, const void* k_cache, const void* v_cache,
+                        const float* k_scale, const float* v_scale, int64_t capacity,
+                        const int64_t* lengths, int64_t prompt_cols, int64_t col,
+                        const int64_t* col_dev, const void* k_prefix, const void* v_prefix,
+                        int64_t prefix_cols, float scale, void* out, void* workspace,
+                        int64_t workspace_bytes, void* stream);
+/* Workspace of such a call (host arithmetic only). col: as given to the call,
+ * or -1 when it is read on the device. */
+int mep_cache_attention_workspace(int dtype, int cache_dtype, int64_t batch, int64_t tokens,
+                                  int q_heads, int kv_heads, int head_dim, int64_t capacity,
+                                  int64_t col, int64_t prefix_cols, int64_t* bytes_out);
+
+/*
+ * Next token of each row of logits (rows, vocab), rows `stride` elements
+ * apart, from one uniform number each, u in [0, 1). Tokens are ordered by
+ * (logit descending, id ascending) and weighted w = exp((l - lmax) /
+ * temperature); kept are the ranks below top_k (0: all), of those the ranks
+ * whose preceding mass is below top_p times their mass (>= 1: all), of those
+ * w >= min_p. The token is the first id, ascending, whose running sum of kept
+ * weights exceeds u times their sum; logprobs (fp32, may be NULL) its log
+ * probability among the kept. The best token is always kept; temperature 0
+ * takes it (log probability 0). A row without a logit above -inf gives token
+ * -1 and log probability -inf; NaN logits count as -inf; +inf logits share
+ * the mass. temperature, top_k, top_p, min_p: (rows,) on the device, or NULL
+ * to use the *_all value for every row.
+ */
+int mep_sample(int dtype, const void* logits, int64_t rows, int64_t vocab, int64_t stride,
+               const float* u, const float* temperature, const int32_t* top_k, const float* top_p,
+               const float* min_p, float temperature_all, int32_t top_k_all, float top_p_all,
+               float min_p_all, int64_t* tokens, float* logprobs, void* stream);
 
 #ifdef __cplusplus
 }

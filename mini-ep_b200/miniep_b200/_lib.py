@@ -14,6 +14,7 @@ LIB_PATH = Path(__file__).resolve().parent / "libminiep_b200.so"
 MEP_OK = 0
 MEP_F32 = 0
 MEP_BF16 = 1
+MEP_E4M3 = 2
 IPC_HANDLE_BYTES = 64
 # step-timeline slots (MEP_TL_* of include/miniep_b200.h): name -> slot; a
 # stage name has its start at the slot and its end at slot + 1
@@ -56,6 +57,16 @@ SIGNATURES = {
     "mep_debug_wait": [_P, C.c_uint32, _I64, _P],
     "mep_barrier": [_P, _P],
     "mep_read_timeline": [_P, _P, _P],
+    "mep_norm_rope_store": [_I, _I, _I64, _I64, _I, _I, _I] + [_P, _I64, _I64, _I64] * 3 +
+                           [_P, _P, C.c_float, _P, _P, _I, _I64, _P, _I64, _I64, _P, _P, _P, _P,
+                            _P, _I64, _I64, _P, _P],
+    "mep_kv_read": [_I, _I64, _I, _I, _P, _P, _P, _P, _I64, _I64, _I64, _P, _P, _P],
+    "mep_cache_attention": [_I, _I, _I64, _I64, _I, _I, _I, _P, _I64, _I64, _I64, _P, _P, _P, _P,
+                            _I64, _P, _I64, _I64, _P, _P, _P, _I64, C.c_float, _P, _P, _I64, _P],
+    "mep_cache_attention_workspace": [_I, _I, _I64, _I64, _I, _I, _I, _I64, _I64, _I64,
+                                      C.POINTER(_I64)],
+    "mep_sample": [_I, _P, _I64, _I64, _I64, _P, _P, _P, _P, _P, C.c_float, C.c_int32, C.c_float,
+                   C.c_float, _P, _P, _P],
     "mep_dest_ranks_noalloc": [_I, _I, _P, _P, _I, _P, _P, _I64, _P, _P],
 }
 _RESTYPES = {"mep_last_error": C.c_char_p}

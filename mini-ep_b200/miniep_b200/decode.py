@@ -1,0 +1,371 @@
+"""The operators of a decode step around the expert-parallel layer, as CUDA
+kernels: writing new tokens into the key/value cache, attention over it, and
+sampling the next token.
+
+  * ``KVCache``: keys and values of a batch for every layer, in the model
+    dtype or quantised to e4m3 with one fp32 scale a row;
+  * ``norm_rope_store``: head norms, rotation and the cache write in one pass;
+  * ``cache_attention``: attention of new tokens over a row's cache and, with a
+    ``SharedPrefix``, over a prefix that all rows share;
+  * ``sample_tokens`` / ``Sampler``: temperature, top-k, top-p and min-p from
+    given uniform numbers.
+
+Tensors are CUDA tensors on one device, whichever is current; work goes to
+that device's current stream and nothing synchronises. The operators are for
+inference: a tensor that requires grad is refused while grad mode is on.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from dataclasses import dataclass
+from functools import lru_cache
+
+import torch
+
+from . import _lib
+from ._lib import MEPError, check
+
+_DTYPES = {torch.float32: _lib.MEP_F32, torch.bfloat16: _lib.MEP_BF16}
+_CACHE_DTYPES = {**_DTYPES, torch.float8_e4m3fn: _lib.MEP_E4M3}
+
+
+def _need(cond: bool, msg: str):
+    if not cond:
+        raise MEPError(msg)
+
+
+def _tensor(t, name: str, device, dtype=None):
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise MEPError(f"{name} must be a CUDA tensor")
+    if device is not None and t.device != device:
+        raise MEPError(f"{name} is on {t.device}, expected {device}")
+    if dtype is not None and t.dtype != dtype:
+        raise MEPError(f"{name} must be {dtype}, not {t.dtype}")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise MEPError(f"{name} requires grad: this operator has no backward pass")
+
+
+def _rows(t):
+    """`t` itself where the kernels' 16-byte accesses fit its strides, else a copy."""
+    unit = 16 // t.element_size()
+    st = t.stride()
+    if st[-1] == 1 and t.data_ptr() % 16 == 0 and not any(s % unit for s in st[:-1]):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _flat(t):
+    """Contiguous and on a 16-byte boundary."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+class _on:
+    """Calls into the library with the tensors' device current."""
+
+    def __init__(self, device):
+        self.index = device.index
+
+    def __enter__(self):
+        self.before = torch.cuda.current_device()
+        if self.before != self.index:
+            torch.cuda.set_device(self.index)
+        return torch.cuda.current_stream().cuda_stream
+
+    def __exit__(self, *exc):
+        if self.before != self.index:
+            torch.cuda.set_device(self.before)
+
+
+class KVCache:
+    """Keys and values (layers, batch, kv_heads, capacity, head_dim),
+    contiguous CUDA tensors the caller owns. In the model dtype, or quantised:
+    torch.float8_e4m3fn codes with fp32 scales (layers, batch, kv_heads,
+    capacity); `dtype` is then the model dtype that `read` answers in."""
+
+    def __init__(self, k, v, k_scale=None, v_scale=None, dtype=None):
+        _tensor(k, "k", None)
+        _tensor(v, "v", k.device, k.dtype)
+        _need(k.dtype in _CACHE_DTYPES, f"a cache is fp32, bf16 or e4m3, not {k.dtype}")
+        _need(k.dim() == 5 and k.shape == v.shape,
+              "k and v must both be (layers, batch, kv_heads, capacity, head_dim)")
+        self.quantized = k.dtype == torch.float8_e4m3fn
+        dtype = dtype or (torch.bfloat16 if self.quantized else k.dtype)
+        _need(dtype in _DTYPES, f"the model dtype is fp32 or bf16, not {dtype}")
+        _need(self.quantized or dtype == k.dtype,
+              f"a {k.dtype} cache cannot serve a {dtype} model")
+        _need((k_scale is not None) == self.quantized and (v_scale is not None) == self.quantized,
+              "k_scale and v_scale go with an e4m3 cache, and only with one")
+        parts = [k, v]
+        if self.quantized:
+            for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+                _tensor(t, name, k.device, torch.float32)
+                _need(t.shape == k.shape[:-1], f"{name} must be {tuple(k.shape[:-1])}")
+            parts += [k_scale, v_scale]
+        for t in parts:
+            _need(t.is_contiguous() and t.data_ptr() % 16 == 0,
+                  "cache tensors must be contiguous and start on a 16-byte boundary")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.dtype, self.device = dtype, k.device
+        self.layers, self.batch, self.kv_heads, self.capacity, self.head_dim = k.shape
+        self._code = _CACHE_DTYPES[k.dtype]
+        # every layer starts on a 16-byte boundary too: a row is a multiple of
+        # 16 bytes (head_dim is one of 16), and scales are read one at a time
+        step = [t[0].numel() * t.element_size() if self.layers else 0 for t in parts]
+        at = [t.data_ptr() for t in parts] + [None] * (4 - len(parts))
+        self._ptrs = [tuple(None if p is None else p + l * d
+                            for p, d in zip(at, step + [0] * (4 - len(parts))))
+                      for l in range(self.layers)]
+
+    @classmethod
+    def empty(cls, layers: int, batch: int, kv_heads: int, capacity: int, head_dim: int,
+              dtype=torch.bfloat16, quantized: bool = False, device="cuda") -> "KVCache":
+        """A zeroed cache of its own tensors."""
+        shape = (layers, batch, kv_heads, capacity, head_dim)
+        store = torch.float8_e4m3fn if quantized else dtype
+        k, v = (torch.zeros(shape, dtype=store, device=device) for _ in range(2))
+        ks = vs = None
+        if quantized:
+            ks, vs = (torch.zeros(shape[:-1], dtype=torch.float32, device=device) for _ in range(2))
+        return cls(k, v, ks, vs, dtype)
+
+    def layer(self, layer: int) -> tuple:
+        _need(0 <= layer < self.layers, f"layer {layer} outside [0, {self.layers})")
+        return self._ptrs[layer]
+
+    def read(self, layer: int, start: int, end: int):
+        """Columns [start, end) of one layer, (batch, kv_heads, end - start,
+        head_dim) each, in the model dtype: a view of a cache that holds it,
+        code * scale rounded once of a quantised one."""
+        kp, vp, ksp, vsp = self.layer(layer)
+        _need(0 <= start <= end <= self.capacity,
+              f"columns [{start}, {end}) outside the cache's {self.capacity}")
+        if not self.quantized:
+            return self.k[layer, :, :, start:end], self.v[layer, :, :, start:end]
+        shape = (2, self.batch, self.kv_heads, end - start, self.head_dim)
+        out = torch.empty(shape, dtype=self.dtype, device=self.device)
+        k, v = out[0], out[1]
+        with _on(self.device) as stream:
+            check(_lib.lib().mep_kv_read(_DTYPES[self.dtype], self.batch, self.kv_heads,
+                                         self.head_dim, kp, vp, ksp, vsp, self.capacity, start,
+                                         end - start, k.data_ptr(), v.data_ptr(), stream),
+                  None, "KVCache.read")
+        return k, v
+
+
+class SharedPrefix:
+    """Keys and values of a prefix all rows of a batch share: (layers,
+    kv_heads, columns, head_dim) each, rotated, in the model dtype."""
+
+    def __init__(self, k, v):
+        _tensor(k, "prefix k", None)
+        _tensor(v, "prefix v", k.device, k.dtype)
+        _need(k.dtype in _DTYPES, f"a prefix is fp32 or bf16, not {k.dtype}")
+        _need(k.dim() == 4 and k.shape == v.shape,
+              "prefix k and v must both be (layers, kv_heads, columns, head_dim)")
+        for t in (k, v):
+            _need(t.is_contiguous() and t.data_ptr() % 16 == 0,
+                  "prefix tensors must be contiguous and start on a 16-byte boundary")
+        self.k, self.v = k, v
+        self.layers, self.kv_heads, self.columns, self.head_dim = k.shape
+        step = k[0].numel() * k.element_size() if self.layers else 0
+        self._ptrs = [(k.data_ptr() + l * step, v.data_ptr() + l * step)
+                      for l in range(self.layers)]
+
+    @classmethod
+    def from_cache(cls, cache: KVCache, row: int, columns: int) -> "SharedPrefix":
+        """A copy of the first `columns` columns of one row, of every layer
+        (read back to the model dtype from a quantised cache)."""
+        _need(0 <= row < cache.batch, f"row {row} outside [0, {cache.batch})")
+        got = [cache.read(l, 0, columns) for l in range(cache.layers)]
+        return cls(torch.stack([k[row] for k, _ in got]).contiguous(),
+                   torch.stack([v[row] for _, v in got]).contiguous())
+
+
+def _column(col, device):
+    """(host column or -1, device pointer or None)."""
+    if isinstance(col, torch.Tensor):
+        _tensor(col, "col", device, torch.int64)
+        _need(col.numel() == 1, "col must hold one column")
+        return -1, col.data_ptr()
+    return int(col), None
+
+
+def _heads(q, cache: KVCache):
+    _tensor(q, "q", cache.device, cache.dtype)
+    _need(q.dim() == 4, "q must be (batch, tokens, heads, head_dim)")
+    B, T, Hq, D = q.shape
+    _need(B == cache.batch and D == cache.head_dim,
+          f"q {tuple(q.shape)} does not fit a cache of batch {cache.batch}, "
+          f"head_dim {cache.head_dim}")
+    return B, T, Hq, D
+
+
+def norm_rope_store(q, k, v, cos, sin, positions, cache: KVCache, layer: int, col, *,
+                    q_norm=None, k_norm=None, eps: float = 1e-6):
+    """Optional RMS norm of each q and k head, rotation, and the cache write of
+    new tokens, in one pass. q: (B, T, Hq, D); k, v: (B, T, Hk, D), any
+    strides; cos, sin: (rows, D) fp32 or model dtype; positions: (B, T) int64
+    (broadcast over B allowed). Token t's K (rotated) and V go to column
+    col + t of `cache`'s `layer`, quantised if the cache is; `col` is an int
+    or a one-element int64 device tensor (columns outside the cache are then
+    not written). Returns the rotated q, (B, T, Hq, D) contiguous."""
+    B, T, Hq, D = _heads(q, cache)
+    dev, dt = cache.device, cache.dtype
+    Hk = cache.kv_heads
+    for name, t in (("k", k), ("v", v)):
+        _tensor(t, name, dev, dt)
+        _need(t.shape == (B, T, Hk, D), f"{name} must be {(B, T, Hk, D)}, not {tuple(t.shape)}")
+    _tensor(cos, "cos", dev)
+    _tensor(sin, "sin", dev, cos.dtype)
+    _need(cos.dtype in (torch.float32, dt), f"cos and sin must be fp32 or {dt}")
+    _need(cos.dim() == 2 and cos.shape[1] == D and cos.shape == sin.shape,
+          f"cos and sin must both be (rows, {D})")
+    _tensor(positions, "positions", dev, torch.int64)
+    if positions.shape != (B, T):
+        _need(positions.dim() == 2 and positions.shape[0] == 1 and positions.shape[1] == T,
+              f"positions must be {(B, T)}, not {tuple(positions.shape)}")
+        positions = positions.expand(B, T)
+    for name, t in (("q_norm", q_norm), ("k_norm", k_norm)):
+        if t is not None:
+            _tensor(t, name, dev, dt)
+            _need(t.shape == (D,), f"{name} must be ({D},)")
+    host, devcol = _column(col, dev)
+    kp, vp, ksp, vsp = cache.layer(layer)
+    q, k, v, cos, sin = _rows(q), _rows(k), _rows(v), _flat(cos), _flat(sin)
+    q_norm = None if q_norm is None else _flat(q_norm)
+    k_norm = None if k_norm is None else _flat(k_norm)
+    out = torch.empty((B, T, Hq, D), dtype=dt, device=dev)
+    qs, ks, vs, ps = q.stride(), k.stride(), v.stride(), positions.stride()
+    with _on(dev) as stream:
+        check(_lib.lib().mep_norm_rope_store(
+            _DTYPES[dt], cache._code, B, T, Hq, Hk, D, q.data_ptr(), qs[0], qs[1], qs[2],
+            k.data_ptr(), ks[0], ks[1], ks[2], v.data_ptr(), vs[0], vs[1], vs[2],
+            None if q_norm is None else q_norm.data_ptr(),
+            None if k_norm is None else k_norm.data_ptr(), eps, cos.data_ptr(), sin.data_ptr(),
+            _DTYPES[cos.dtype], cos.shape[0], positions.data_ptr(), ps[0], ps[1], out.data_ptr(),
+            kp, vp, ksp, vsp, cache.capacity, host, devcol, stream), None, "norm_rope_store")
+    return out
+
+
+@lru_cache(maxsize=4096)
+def _attention_workspace(*sizes) -> int:
+    n = C.c_int64()
+    check(_lib.lib().mep_cache_attention_workspace(*sizes, C.byref(n)), None, "cache_attention")
+    return n.value
+
+
+def cache_attention(q, cache: KVCache, layer: int, col, scale: float, *, lengths=None,
+                    prompt_cols: int = 0, prefix: SharedPrefix | None = None):
+    """Attention of new tokens over `cache`'s `layer`: q (B, T, Hq, D) rotated,
+    any strides; query head h reads K/V head h // (Hq // Hk). Query t of row b
+    sees the own columns c <= col + t with c < lengths[b] or c >= prompt_cols
+    (`lengths` (B,) int64: the row's prompt inside the padded prompt columns;
+    None: every c <= col + t), and all of `prefix`. `col` is an int or a
+    one-element int64 device tensor. Returns (B, T, Hq, D) contiguous; zeros
+    for a query that sees nothing."""
+    B, T, Hq, D = _heads(q, cache)
+    dev, dt = cache.device, cache.dtype
+    if lengths is not None:
+        _tensor(lengths, "lengths", dev, torch.int64)
+        _need(lengths.shape == (B,), f"lengths must be ({B},), not {tuple(lengths.shape)}")
+        lengths = lengths.contiguous()
+    P, pk, pv = 0, None, None
+    if prefix is not None:
+        _need(prefix.k.device == dev and prefix.k.dtype == dt,
+              f"the prefix must be {dt} on {dev}")
+        _need(prefix.kv_heads == cache.kv_heads and prefix.head_dim == D,
+              "the prefix and the cache have different heads")
+        _need(0 <= layer < prefix.layers, f"layer {layer} outside the prefix's {prefix.layers}")
+        P, (pk, pv) = prefix.columns, prefix._ptrs[layer]
+    host, devcol = _column(col, dev)
+    kp, vp, ksp, vsp = cache.layer(layer)
+    q = _rows(q)
+    dc = _DTYPES[dt]
+    nbytes = _attention_workspace(dc, cache._code, B, T, Hq, cache.kv_heads, D, cache.capacity,
+                                  host, P)
+    out = torch.empty((B, T, Hq, D), dtype=dt, device=dev)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    qs = q.stride()
+    with _on(dev) as stream:
+        check(_lib.lib().mep_cache_attention(
+            dc, cache._code, B, T, Hq, cache.kv_heads, D, q.data_ptr(), qs[0], qs[1], qs[2], kp,
+            vp, ksp, vsp, cache.capacity, None if lengths is None else lengths.data_ptr(),
+            prompt_cols, host, devcol, pk, pv, P, scale, out.data_ptr(),
+            None if ws is None else ws.data_ptr(), nbytes, stream), None, "cache_attention")
+    return out
+
+
+def sample_tokens(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, *,
+                  return_logprobs: bool = False):
+    """Next token of each row of `logits` (B, V) from one uniform number each
+    (u: (B,) fp32 in [0, 1)): (B,) int64, and with `return_logprobs` the drawn
+    tokens' log probabilities among the kept ones (fp32). Tokens are ordered by
+    (logit descending, id ascending), w = exp((l - lmax) / temperature); kept
+    are the first top_k (0: all), of those the ones whose preceding mass is
+    below top_p of their mass, of those w >= min_p; the token is the first id,
+    ascending, whose running kept weight exceeds u times its sum. Temperature 0
+    takes the best token (lowest id). Each of temperature, top_p, min_p (fp32)
+    and top_k (int32) is a number or a (B,) device tensor. A row whose logits
+    are all -inf or NaN gives token -1."""
+    _tensor(logits, "logits", None)
+    dev = logits.device
+    _need(logits.dtype in _DTYPES, f"logits are fp32 or bf16, not {logits.dtype}")
+    _need(logits.dim() == 2 and logits.shape[1] > 0, "logits must be (rows, vocab)")
+    B, V = logits.shape
+    _tensor(u, "u", dev, torch.float32)
+    _need(u.shape == (B,), f"u must be ({B},), not {tuple(u.shape)}")
+    if logits.stride(1) != 1:
+        logits = logits.contiguous()
+    u = u.contiguous()
+    ptrs, nums, keep = [], [], []
+    for name, x, dt, num in (("temperature", temperature, torch.float32, float),
+                             ("top_k", top_k, torch.int32, int),
+                             ("top_p", top_p, torch.float32, float),
+                             ("min_p", min_p, torch.float32, float)):
+        if isinstance(x, torch.Tensor):
+            _tensor(x, name, dev, dt)
+            _need(x.shape == (B,), f"{name} must be a number or ({B},)")
+            x = x.contiguous()
+            keep.append(x)
+            ptrs.append(x.data_ptr())
+            nums.append(num(1))
+        else:
+            ptrs.append(None)
+            nums.append(min(num(x), 0x7fffffff) if dt == torch.int32 else num(x))
+    tokens = torch.empty(B, dtype=torch.int64, device=dev)
+    logprobs = torch.empty(B, dtype=torch.float32, device=dev) if return_logprobs else None
+    with _on(dev) as stream:
+        check(_lib.lib().mep_sample(_DTYPES[logits.dtype], logits.data_ptr(), B, V,
+                                    logits.stride(0), u.data_ptr(), *ptrs, *nums,
+                                    tokens.data_ptr(),
+                                    None if logprobs is None else logprobs.data_ptr(), stream),
+              None, "sample_tokens")
+    return (tokens, logprobs) if return_logprobs else tokens
+
+
+@dataclass
+class Sampler:
+    """Filters of `sample_tokens` with a source of its uniform numbers: a
+    generator on the logits' device, seeded with `seed` at the first draw. The
+    same seed gives the same sequence of draws."""
+    temperature: object = 1.0
+    top_k: object = 0
+    top_p: object = 1.0
+    min_p: object = 0.0
+    seed: int = 0
+
+    def __post_init__(self):
+        self._gen = None
+
+    def uniform(self, *shape, device):
+        """The next uniform numbers of the sequence."""
+        if self._gen is None or self._gen.device != torch.device(device):
+            self._gen = torch.Generator(device=device)
+            self._gen.manual_seed(self.seed)
+        return torch.rand(*shape, generator=self._gen, device=device)
+
+    def __call__(self, logits, u=None):
+        if u is None:
+            u = self.uniform(logits.shape[0], device=logits.device)
+        return sample_tokens(logits, u, self.temperature, self.top_k, self.top_p, self.min_p)

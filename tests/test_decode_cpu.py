@@ -1,0 +1,103 @@
+"""Decode-step operators without a GPU: what they refuse on the host, and the
+library's own argument checks (all made before any CUDA call)."""
+import ctypes as C
+
+import pytest
+import torch
+
+import miniep_b200 as M
+from miniep_b200 import MEPError, _lib, build
+
+
+@pytest.fixture(scope="module")
+def lib():
+    build.build()
+    return _lib.lib()
+
+
+def test_host_tensors_are_refused():
+    k = torch.zeros(1, 2, 2, 8, 64)
+    with pytest.raises(MEPError, match="CUDA"):
+        M.KVCache(k, k)
+    with pytest.raises(MEPError, match="CUDA"):
+        M.KVCache.empty(1, 2, 2, 8, 64, torch.float32, device="cpu")
+    with pytest.raises(MEPError, match="CUDA"):
+        M.SharedPrefix(k[0], k[0])
+    with pytest.raises(MEPError, match="CUDA"):
+        M.sample_tokens(torch.zeros(2, 5), torch.zeros(2))
+    with pytest.raises(MEPError, match="CUDA"):
+        M.sample_tokens([1.0], torch.zeros(2))
+
+
+def _heads(dtype=1, cache=1, B=2, T=1, Hq=4, Hk=2, D=64):
+    return [dtype, cache, B, T, Hq, Hk, D]
+
+
+BAD_HEADS = [(dict(dtype=2), b"dtype"), (dict(dtype=3), b"dtype"), (dict(cache=0), b"cache"),
+             (dict(B=-1), b"negative"), (dict(T=-1), b"negative"), (dict(Hq=3), b"multiple"),
+             (dict(Hk=0), b"multiple"), (dict(D=24), b"head_dim"), (dict(D=144), b"head_dim"),
+             (dict(D=0), b"head_dim"), (dict(B=1 << 20), b"batch")]
+
+
+@pytest.mark.parametrize("bad,word", BAD_HEADS, ids=str)
+def test_bad_heads(lib, bad, word):
+    n = C.c_int64()
+    assert lib.mep_cache_attention_workspace(*_heads(**bad), 8, 0, 0, C.byref(n)) == 1
+    assert word in lib.mep_last_error(None)
+    store = [None, 0, 0, 0] * 3 + [None, None, 1e-6, None, None, 0, 8, None, 0, 0] + [None] * 5
+    assert lib.mep_norm_rope_store(*_heads(**bad), *store, 8, 0, None, None) == 1
+    assert word in lib.mep_last_error(None)
+    attend = [None, 0, 0, 0, None, None, None, None, 8, None, 0, 0, None, None, None, 0, 1.0, None,
+              None, 0, None]
+    assert lib.mep_cache_attention(*_heads(**bad), *attend) == 1
+    assert word in lib.mep_last_error(None)
+
+
+def test_columns_and_null_tensors(lib):
+    store = [None, 0, 0, 0] * 3 + [None, None, 1e-6, None, None, 0, 8, None, 0, 0] + [None] * 5
+    for cap, col, word in ((8, 8, b"fit"), (8, -1, b"fit"), (-1, 0, b"capacity"), (8, 0, b"null")):
+        assert lib.mep_norm_rope_store(*_heads(), *store, cap, col, None, None) == 1
+        assert word in lib.mep_last_error(None)
+        attend = [None, 0, 0, 0, None, None, None, None, cap, None, 0, col, None, None, None, 0,
+                  1.0, None, None, 0, None]
+        assert lib.mep_cache_attention(*_heads(), *attend) == 1
+        assert (b"null" if cap == 8 and col == 0 else b"") in lib.mep_last_error(None)
+    for start, n in ((-1, 2), (0, 9), (8, 1), (3, -1)):
+        assert lib.mep_kv_read(1, 2, 2, 64, None, None, None, None, 8, start, n, None, None,
+                               None) == 1
+        assert b"columns" in lib.mep_last_error(None)
+    assert lib.mep_kv_read(1, 2, 2, 64, None, None, None, None, 8, 0, 0, None, None, None) == 0
+    assert lib.mep_kv_read(1, 2, 2, 64, None, None, None, None, 8, 0, 1, None, None, None) == 1
+
+
+def test_calls_without_rows_do_nothing(lib):
+    """No token, no row: fine, and no CUDA call (none would work here)."""
+    store = [None, 0, 0, 0] * 3 + [None, None, 1e-6, None, None, 0, 8, None, 0, 0] + [None] * 5
+    assert lib.mep_norm_rope_store(*_heads(B=0), *store, 8, 0, None, None) == 0
+    assert lib.mep_norm_rope_store(*_heads(T=0), *store, 8, 8, None, None) == 0
+    attend = [None, 0, 0, 0, None, None, None, None, 8, None, 0, 0, None, None, None, 0, 1.0, None,
+              None, 0, None]
+    assert lib.mep_cache_attention(*_heads(B=0), *attend) == 0
+    assert lib.mep_cache_attention(*_heads(T=0), *attend) == 0
+    assert lib.mep_sample(0, None, 0, 5, 5, *[None] * 5, 1.0, 0, 1.0, 0.0, None, None, None) == 0
+
+
+@pytest.mark.parametrize("args,word", [
+    ((2, 2, 5, 5, 1.0, 0, 1.0, 0.0), b"dtype"), ((0, -1, 5, 5, 1.0, 0, 1.0, 0.0), b"rows"),
+    ((0, 2, 0, 5, 1.0, 0, 1.0, 0.0), b"vocab"), ((0, 2, 1 << 25, 1 << 25, 1.0, 0, 1.0, 0.0), b"vocab"),
+    ((0, 2, 5, -5, 1.0, 0, 1.0, 0.0), b"stride"), ((0, 2, 5, 5, -1.0, 0, 1.0, 0.0), b"temperature"),
+    ((0, 2, 5, 5, float("nan"), 0, 1.0, 0.0), b"temperature"),
+    ((0, 2, 5, 5, 1.0, -1, 1.0, 0.0), b"top_k"), ((0, 2, 5, 5, 1.0, 0, 0.0, 0.0), b"top_p"),
+    ((0, 2, 5, 5, 1.0, 0, 1.0, 1.1), b"min_p"), ((0, 2, 5, 5, 1.0, 0, 1.0, 0.0), b"null")], ids=str)
+def test_bad_sampling_arguments(lib, args, word):
+    dtype, rows, vocab, stride, t, k, p, m = args
+    assert lib.mep_sample(dtype, None, rows, vocab, stride, *[None] * 5, t, k, p, m, None, None,
+                          None) == 1
+    assert word in lib.mep_last_error(None)
+
+
+def test_workspace_is_host_arithmetic(lib):
+    n = C.c_int64(-1)
+    assert lib.mep_cache_attention_workspace(*_heads(), 4096, 4000, 512, C.byref(n)) == 0
+    assert n.value >= 0
+    assert lib.mep_cache_attention_workspace(*_heads(), 4096, 4000, 512, None) == 1

@@ -5,6 +5,13 @@
 // c >= prompt_cols):
 //   s = scale * q.k, out = sum exp(s - m) v / sum exp(s - m), m = max s,
 // in fp32, rounded once to the model dtype; zeros where nothing is visible.
+//
+// One pass over the keys with a running maximum and sum. The queries that
+// share a key/value head are the rows of one matrix: for the own columns the
+// T * (q_heads / kv_heads) queries of a batch row, for the prefix those of the
+// whole batch, so that each key is read once for all of them. The keys are cut
+// into splits that run on different SMs; their partial results (fp32 sums, the
+// maximum in base 2) meet in k_attn_join.
 #include <cstdint>
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
@@ -30,60 +37,755 @@ struct AttnArgs {
   void* out;
 };
 
-template <typename C>
-__device__ __forceinline__ float elt(const void* p, int64_t i) {
-  return Elt<C>::to_f(static_cast<const C*>(p)[i]);
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kThreads = 128;  // four warps a CTA
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
-template <>
-__device__ __forceinline__ float elt<uint8_t>(const void* p, int64_t i) {
-  return __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<const uint8_t*>(p)[i], __NV_E4M3)));
+__device__ __forceinline__ void cp16(void* dst, const void* src, bool real) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src),
+               "r"(real ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void cp4(void* dst, const void* src, bool real) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(src),
+               "r"(real ? 4 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], const void* p) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(smem_u32(p)));
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], const void* p) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(smem_u32(p)));
+}
+__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                        uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t tf32(float x) {
+  uint32_t r;
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
+  return r;
+}
+// x = hi + lo, each with the 11 bits a tf32 operand holds: products of split
+// operands leave out only lo * lo, 2^-22 of the product
+__device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
+  hi = tf32(x);
+  lo = tf32(x - __uint_as_float(hi));
+}
+__device__ __forceinline__ uint32_t e4m3x2_f16x2(uint32_t two) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, __NV_E4M3);
+  return (uint32_t)h.x | (uint32_t)h.y << 16;
+}
+__device__ __forceinline__ float half_lo(uint32_t h2) {
+  return __half2float(__ushort_as_half((unsigned short)(h2 & 0xffff)));
+}
+__device__ __forceinline__ float half_hi(uint32_t h2) {
+  return __half2float(__ushort_as_half((unsigned short)(h2 >> 16)));
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float quad_max(float x) {
+  x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+  return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+}
+__device__ __forceinline__ float quad_sum(float x) {
+  x += __shfl_xor_sync(0xffffffffu, x, 1);
+  return x + __shfl_xor_sync(0xffffffffu, x, 2);
 }
 
-// one warp per query head; the lanes share the head's values
-template <typename T, typename C>
-__global__ void __launch_bounds__(128) k_attn(const AttnArgs a) {
-  const int lane = lane_id(), D = a.head_dim;
-  const int64_t i = (int64_t)blockIdx.x * 4 + warp_id();
-  if (i >= a.batch * a.tokens * a.q_heads) return;
-  const int h = (int)(i % a.q_heads);
-  const int64_t bt = i / a.q_heads, b = bt / a.tokens, t = bt - b * a.tokens;
-  const int kh = h / (a.q_heads / a.kv_heads);
-  const int64_t col = a.col_dev ? *a.col_dev : a.col;
-  const T* q = static_cast<const T*>(a.q.p) + b * a.q.sb + t * a.q.st + h * a.q.sh;
-  float x[4] = {}, o[4] = {}, m = -INFINITY, l = 0.f;
-#pragma unroll
-  for (int e = 0; e < 4; ++e)
-    if (lane + 32 * e < D) x[e] = Elt<T>::to_f(q[lane + 32 * e]);
-  auto see = [&](auto tag, const void* k, const void* v, int64_t row, float ks, float vs) {
-    using E = decltype(tag);
-    float s = 0.f;
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (lane + 32 * e < D) s += x[e] * elt<E>(k, row * D + lane + 32 * e);
-#pragma unroll
-    for (int w = 16; w > 0; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
-    s *= ks * a.scale;
-    const float mn = fmaxf(m, s), keep = expf(m - mn), p = expf(s - mn);
-    m = mn;
-    l = l * keep + p;
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (lane + 32 * e < D) o[e] = o[e] * keep + p * vs * elt<E>(v, row * D + lane + 32 * e);
-  };
-  for (int64_t c = 0; c < a.prefix_cols; ++c)
-    see(T{}, a.kp, a.vp, kh * a.prefix_cols + c, 1.f, 1.f);
-  const int64_t end = min(col + t + 1, a.c.capacity);
-  const int64_t len = a.lengths ? a.lengths[b] : end;
-  for (int64_t c = 0; c < end; ++c) {
-    if (c >= len && c < a.prompt_cols) continue;
-    const int64_t row = (b * a.kv_heads + kh) * a.c.capacity + c;
-    see(C{}, a.c.k, a.c.v, row, sizeof(C) == 1 ? a.c.ks[row] : 1.f,
-        sizeof(C) == 1 ? a.c.vs[row] : 1.f);
+// The columns that rows of one matrix see, as one run of indices j in [0, n):
+// columns [0, n1), then those from `skip` columns further on.
+struct Span {
+  int64_t n, n1, skip;
+  __device__ int64_t column(int64_t j) const { return j < n1 ? j : j + skip; }
+};
+
+// Geometry of a launch. Rows of a matrix: own columns, the tokens * group
+// queries of one batch row (matrix index = batch row); prefix, those of the
+// whole batch (one matrix). A partial result of row r of matrix i is slot
+// [split][(i * rows + r)'s output row].
+struct PartArgs {
+  AttnArgs a;
+  int group;             // query heads of a key/value head
+  int64_t rows;          // rows of a matrix
+  int row_tiles, splits;
+  int64_t out_rows;      // batch * tokens * q_heads
+  float* part_o;         // [splits][out_rows][head_dim], or null: write `out`
+  float2* part_ml;       // [splits][out_rows]: maximum (base 2), sum
+};
+
+// The kernel for one (element types, padded head width, warp layout).
+// KS (key split): the four warps share 16 rows and take a quarter of each tile
+// of keys each, for matrices of few rows, where the keys' bytes bound it: a
+// warp streams its own keys and meets the others only at the end. Otherwise
+// each warp has 16 of 64 rows and every key of the tile.
+template <typename QT, typename CT, int DP, bool KS>
+struct Tile {
+  static constexpr int kElt = sizeof(CT);
+  static constexpr int kRow = DP * kElt;  // bytes of a staged row
+  // keys a warp works on at a time: 8 KB of keys and values a warp when the
+  // keys are split (4 KB of codes)
+  static constexpr int kN = KS ? (kRow >= 256 ? 16 : 32) : (kRow >= 512 ? 32 : 64);
+  static constexpr int kKeys = KS ? 4 * kN : kN;  // keys of a CTA's tile
+  static constexpr int kStages = KS ? 3 : 2;
+  static constexpr int kRows = KS ? 16 : 64;
+  static constexpr bool kScaled = sizeof(CT) == 1;
+  static constexpr int kScaleBytes = kScaled ? kKeys * 8 : 0;
+  static constexpr int kStageBytes = 2 * kKeys * kRow + kScaleBytes;
+  static constexpr bool kF32 = sizeof(QT) == 4;
+  // fp32 queries stay in shared memory (their split halves do not fit the
+  // registers), rows 4 floats apart in the banks
+  static constexpr int kQRow = DP + 4;
+  static constexpr int kQBytes = kF32 ? kRows * kQRow * 4 : 0;
+  static constexpr int kJoin = KS ? 4 * 16 * DP * 4 + 4 * 16 * 8 : 0;
+  static constexpr int kBody = kStages * kStageBytes + kQBytes;
+  static constexpr int kSmem = kBody > kJoin ? kBody : kJoin;
+  // place of 16-byte chunk c of staged row r, so that the accesses of a warp
+  // fall into different banks
+  __device__ static int k_chunk(int r, int c) {
+    if (sizeof(CT) == 2) return c ^ (r & 7);
+    return kRow >= 128 ? c ^ ((r & 1) << 2) : c;
   }
-  T* out = static_cast<T*>(a.out) + i * D;
+  __device__ static int v_chunk(int r, int c) {
+    if (sizeof(CT) == 4) return c ^ (((r >> 1) & 3) << 1);
+    return kRow >= 128 ? c ^ (r & 7) : c ^ ((r >> 1) & 3);
+  }
+};
+
+template <typename QT, typename CT, int DP, bool KS, bool PREFIX>
+__global__ void __launch_bounds__(kThreads) k_attn_part(const PartArgs p) {
+  using X = Tile<QT, CT, DP, KS>;
+  constexpr int N = X::kN, NT = N / 8, OT = DP / 8;
+  constexpr bool kF32 = X::kF32, kScaled = X::kScaled;
+  extern __shared__ __align__(128) unsigned char smem[];
+  const AttnArgs& a = p.a;
+  const int lane = lane_id(), warp = warp_id(), g = lane >> 2, t4 = lane & 3;
+  const int D = a.head_dim;
+  const int kh = blockIdx.y;
+  const int split = blockIdx.x % p.splits;
+  const int64_t tile_id = blockIdx.x / p.splits;
+  const int rt = (int)(tile_id % p.row_tiles);
+  const int64_t mat = tile_id / p.row_tiles;  // batch row (own columns)
+  const int64_t r0 = (int64_t)rt * X::kRows;
+  const int64_t rN = min(r0 + X::kRows, p.rows);  // rows of this CTA: [r0, rN)
+
+  // row r of the matrix: its query and its output row
+  auto query_of = [&](int64_t r, int64_t& b, int64_t& t, int& h) {
+    const int64_t bt = r / p.group;
+    h = kh * p.group + (int)(r - bt * p.group);
+    b = PREFIX ? bt / a.tokens : mat;
+    t = PREFIX ? bt - b * a.tokens : bt;
+  };
+  auto out_row = [&](int64_t r) {
+    int64_t b, t;
+    int h;
+    query_of(r, b, t, h);
+    return (b * a.tokens + t) * a.q_heads + h;
+  };
+
+  // ---- the columns these rows see
+  Span span;
+  const int64_t col = PREFIX ? 0 : a.col_dev ? *a.col_dev : a.col;
+  if (PREFIX) {
+    span = {a.prefix_cols, a.prefix_cols, 0};
+  } else {
+    const int64_t tmax = (rN - 1) / p.group;
+    const int64_t end = max((int64_t)0, min(col + tmax + 1, a.c.capacity));
+    int64_t len = a.lengths ? max((int64_t)0, a.lengths[mat]) : end;
+    if (len >= a.prompt_cols) len = end;
+    span.n1 = min(len, end);
+    const int64_t more = end - max(a.prompt_cols, span.n1);
+    span.skip = a.prompt_cols - span.n1;
+    span.n = span.n1 + (span.n1 < end && more > 0 ? more : 0);
+  }
+  // this split's share of them, in whole tiles
+  const int64_t tiles = (span.n + X::kKeys - 1) / X::kKeys;
+  const int64_t tile0 = tiles * split / p.splits, tile1 = tiles * (split + 1) / p.splits;
+
+  const int64_t head_row = PREFIX ? kh * a.prefix_cols : (mat * a.kv_heads + kh) * a.c.capacity;
+  const unsigned char* kbase =
+      static_cast<const unsigned char*>(PREFIX ? a.kp : a.c.k) + head_row * D * X::kElt;
+  const unsigned char* vbase =
+      static_cast<const unsigned char*>(PREFIX ? a.vp : a.c.v) + head_row * D * X::kElt;
+  const int chunks = D * X::kElt / 16;  // 16-byte pieces of a row
+
+  // ---- staging: 16-byte copies of the tile's rows, zeros past the span
+  // (rows that nobody sees are never read, whatever they hold)
+  auto stage = [&](int64_t tile) {
+    unsigned char* s = smem + (tile % X::kStages) * X::kStageBytes;
+    const int first = KS ? warp * N : 0;
+    const int who = KS ? lane : threadIdx.x, step = KS ? 32 : kThreads;
+    for (int i = who; i < N * chunks; i += step) {
+      const int r = first + i / chunks, c = i % chunks;
+      const int64_t j = tile * X::kKeys + r;
+      const bool real = j < span.n;
+      const int64_t at = (real ? span.column(j) : 0) * D * X::kElt + c * 16;
+      cp16(s + r * X::kRow + X::k_chunk(r, c) * 16, kbase + at, real);
+      cp16(s + X::kKeys * X::kRow + r * X::kRow + X::v_chunk(r, c) * 16, vbase + at, real);
+    }
+    if (kScaled) {
+      float* sc = reinterpret_cast<float*>(s + 2 * X::kKeys * X::kRow);
+      for (int i = who; i < 2 * N; i += step) {
+        const int r = first + (i % N);
+        const int64_t j = tile * X::kKeys + r;
+        const bool real = j < span.n;
+        const float* src = (i < N ? a.c.ks : a.c.vs) + head_row + (real ? span.column(j) : 0);
+        cp4(sc + (i < N ? 0 : X::kKeys) + r, src, real);
+      }
+    }
+  };
+  auto sync = [&] {
+    if (KS)
+      __syncwarp();
+    else
+      __syncthreads();
+  };
+  // padding between D and DP holds zeros from the start
+  if (D < DP) {
+    const int padc = DP * X::kElt / 16;
+    for (int i = threadIdx.x; i < X::kStages * 2 * X::kKeys * padc; i += kThreads) {
+      const int c = i % padc, r = (i / padc) % X::kKeys, kv = (i / padc / X::kKeys) % 2;
+      const int st = i / padc / X::kKeys / 2;
+      if (c >= chunks)
+        *reinterpret_cast<uint4*>(smem + st * X::kStageBytes + kv * X::kKeys * X::kRow +
+                                  r * X::kRow + (kv ? X::v_chunk(r, c) : X::k_chunk(r, c)) * 16) =
+            make_uint4(0, 0, 0, 0);
+    }
+  }
+  float* qs = reinterpret_cast<float*>(smem + X::kStages * X::kStageBytes);
+  if (kF32) {
+    for (int i = threadIdx.x; i < X::kRows * DP; i += kThreads) {
+      const int r = i / DP, d = i % DP;
+      float x = 0.f;
+      if (r0 + r < rN && d < D) {
+        int64_t b, t;
+        int h;
+        query_of(r0 + r, b, t, h);
+        x = static_cast<const float*>(a.q.p)[b * a.q.sb + t * a.q.st + h * a.q.sh + d];
+      }
+      qs[r * X::kQRow + d] = x;
+    }
+  }
+  if (D < DP || kF32) __syncthreads();
 #pragma unroll
-  for (int e = 0; e < 4; ++e)
-    if (lane + 32 * e < D) out[lane + 32 * e] = Elt<T>::from_f(l > 0.f ? o[e] / l : 0.f);
+  for (int i = 0; i < X::kStages - 1; ++i) {
+    if (tile0 + i < tile1) stage(tile0 + i);
+    cp_commit();
+  }
+
+  // ---- queries of this thread: rows row[0] and row[1] = row[0] + 8
+  const int wrow = KS ? 0 : warp * 16;
+  int64_t row[2], tq[2];
+  float rscale[2];
+  uint32_t qf[kF32 ? 1 : DP / 16][4];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    row[u] = r0 + wrow + g + 8 * u;
+    tq[u] = row[u] < rN ? row[u] / p.group : 0;
+    rscale[u] = a.scale * kLog2e;
+  }
+  if (!kF32) {
+    const __nv_bfloat16* qp[2] = {nullptr, nullptr};
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      if (row[u] < rN) {
+        int64_t b, t;
+        int h;
+        query_of(row[u], b, t, h);
+        qp[u] = static_cast<const __nv_bfloat16*>(a.q.p) + b * a.q.sb + t * a.q.st + h * a.q.sh;
+      }
+    if (!kScaled) {
+#pragma unroll
+      for (int k = 0; k < DP / 16; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int d = k * 16 + t4 * 2 + (i >> 1) * 8;
+          qf[k][i] = qp[i & 1] && d < D ? *reinterpret_cast<const uint32_t*>(qp[i & 1] + d) : 0u;
+        }
+    } else {
+      // Codes are exact in fp16, so the products are fp16 ones. A query row is
+      // scaled by a power of two to a largest magnitude in [1, 2): its bf16
+      // values stay exact down to 2^-14 of it, and below that are off by 2^-25
+      // of it at most.
+      float qv[2][DP / 4];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        float m = 0.f;
+#pragma unroll
+        for (int i = 0; i < DP / 4; ++i) {
+          const int d = (i / 16) * 64 + t4 * 16 + (i % 16);
+          qv[u][i] = qp[u] && d < D ? __bfloat162float(qp[u][d]) : 0.f;
+          m = fmaxf(m, fabsf(qv[u][i]));
+        }
+        m = quad_max(m);
+        const int ex = (int)(__float_as_uint(m) >> 23) - 127;
+        const int e = m > 0.f && ex < 128 ? min(max(ex, -126), 126) : 0;
+        const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+        rscale[u] *= __uint_as_float((uint32_t)(127 + e) << 23);
+#pragma unroll
+        for (int i = 0; i < DP / 4; ++i) qv[u][i] *= down;
+      }
+      // k-step k of a 64-wide block takes values 4k..4k+3 of each thread's 16
+#pragma unroll
+      for (int k = 0; k < DP / 16; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          qf[k][i] = pack_f16x2(qv[i & 1][k * 4 + (i >> 1) * 2], qv[i & 1][k * 4 + (i >> 1) * 2 + 1]);
+    }
+  }
+
+  float o[OT][4];
+#pragma unroll
+  for (int i = 0; i < OT; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  float vref = 0.f;  // what o counts in, for scaled values: their largest scale so far
+
+  for (int64_t tile = tile0; tile < tile1; ++tile) {
+    cp_wait<X::kStages - 2>();
+    sync();
+    if (tile + X::kStages - 1 < tile1) stage(tile + X::kStages - 1);
+    cp_commit();
+    const unsigned char* ks = smem + (tile % X::kStages) * X::kStageBytes;
+    const unsigned char* vs = ks + X::kKeys * X::kRow;
+    const float* sc = reinterpret_cast<const float*>(vs + X::kKeys * X::kRow);
+    const int kr0 = KS ? warp * N : 0;  // first staged row of this warp's keys
+    const int64_t j0 = tile * X::kKeys + kr0;
+    if (KS && j0 >= span.n) continue;
+
+    // ---- scores
+    float s[NT][4];
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
+    if constexpr (!kF32 && !kScaled) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        const int r = kr0 + i * 8 + (lane & 7);
+#pragma unroll
+        for (int k = 0; k < DP / 16; k += 2) {
+          uint32_t b[4];
+          ldsm4(b, ks + r * X::kRow + X::k_chunk(r, k * 2 + (lane >> 3)) * 16);
+          mma_bf16(s[i], qf[k], b[0], b[1]);
+          mma_bf16(s[i], qf[k + 1], b[2], b[3]);
+        }
+      }
+    } else if constexpr (!kF32) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        const int r = kr0 + i * 8 + g;
+#pragma unroll
+        for (int w = 0; w < DP / 64; ++w) {
+          const uint4 v = *reinterpret_cast<const uint4*>(ks + r * X::kRow + X::k_chunk(r, w * 4 + t4) * 16);
+          const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            mma_f16(s[i], qf[w * 4 + k], e4m3x2_f16x2(u[k] & 0xffff), e4m3x2_f16x2(u[k] >> 16));
+        }
+      }
+    } else {
+      const float* q0 = qs + (wrow + g) * X::kQRow;
+      const float* q1 = q0 + 8 * X::kQRow;
+      constexpr int kBlocks = DP / 16;  // 16 values of a row: two k-steps, 4 a thread
+#pragma unroll
+      for (int w = 0; w < kBlocks; ++w) {
+        // scaled: chunk of 16 codes a thread, 4 of them here
+        const int d = kScaled ? (w / 4) * 64 + t4 * 16 + (w % 4) * 4 : w * 16 + t4 * 4;
+        const float4 x0 = *reinterpret_cast<const float4*>(q0 + d);
+        const float4 x1 = *reinterpret_cast<const float4*>(q1 + d);
+        uint32_t h[2][4], e[2][4];
+        split_tf32(x0.x, h[0][0], e[0][0]), split_tf32(x1.x, h[0][1], e[0][1]);
+        split_tf32(x0.y, h[0][2], e[0][2]), split_tf32(x1.y, h[0][3], e[0][3]);
+        split_tf32(x0.z, h[1][0], e[1][0]), split_tf32(x1.z, h[1][1], e[1][1]);
+        split_tf32(x0.w, h[1][2], e[1][2]), split_tf32(x1.w, h[1][3], e[1][3]);
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          const int r = kr0 + i * 8 + g;
+          if constexpr (kScaled) {
+            const uint32_t v = *reinterpret_cast<const uint32_t*>(
+                ks + r * X::kRow + X::k_chunk(r, (w / 4) * 4 + t4) * 16 + (w % 4) * 4);
+            const uint32_t lo = e4m3x2_f16x2(v & 0xffff), hi = e4m3x2_f16x2(v >> 16);
+            const uint32_t b[4] = {__float_as_uint(half_lo(lo)), __float_as_uint(half_hi(lo)),
+                                   __float_as_uint(half_lo(hi)), __float_as_uint(half_hi(hi))};
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              mma_tf32(s[i], e[k], b[2 * k], b[2 * k + 1]);
+              mma_tf32(s[i], h[k], b[2 * k], b[2 * k + 1]);
+            }
+          } else {
+            const float4 v = *reinterpret_cast<const float4*>(ks + r * X::kRow +
+                                                              X::k_chunk(r, w * 4 + t4) * 16);
+            uint32_t bh[4], bl[4];
+            split_tf32(v.x, bh[0], bl[0]), split_tf32(v.y, bh[1], bl[1]);
+            split_tf32(v.z, bh[2], bl[2]), split_tf32(v.w, bh[3], bl[3]);
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              mma_tf32(s[i], h[k], bl[2 * k], bl[2 * k + 1]);
+              mma_tf32(s[i], e[k], bh[2 * k], bh[2 * k + 1]);
+              mma_tf32(s[i], h[k], bh[2 * k], bh[2 * k + 1]);
+            }
+          }
+        }
+      }
+    }
+
+    // ---- scale, mask, running maximum
+    const bool edge = j0 + N > span.n || (!PREFIX && a.tokens > 1);
+    float mx[2] = {m[0], m[1]};
+    float vmax = vref;
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      float f[2] = {1.f, 1.f};
+      if (kScaled) {
+        const float2 kk = *reinterpret_cast<const float2*>(sc + kr0 + i * 8 + t4 * 2);
+        const float2 vv = *reinterpret_cast<const float2*>(sc + X::kKeys + kr0 + i * 8 + t4 * 2);
+        f[0] = kk.x, f[1] = kk.y;
+        vmax = fmaxf(vmax, fmaxf(vv.x, vv.y));
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        s[i][j] *= kScaled ? rscale[j >> 1] * f[j & 1] : rscale[j >> 1];
+        if (edge) {
+          const int64_t jj = j0 + i * 8 + t4 * 2 + (j & 1);
+          const bool see = jj < span.n && (PREFIX || span.column(jj) <= col + tq[j >> 1]);
+          if (!see) s[i][j] = -INFINITY;
+        }
+        mx[j >> 1] = fmaxf(mx[j >> 1], s[i][j]);
+      }
+    }
+    float keep[2], base[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      mx[u] = quad_max(mx[u]);
+      base[u] = mx[u] == -INFINITY ? 0.f : mx[u];
+      keep[u] = ex2(m[u] - base[u]);
+      m[u] = mx[u];
+      l[u] *= keep[u];
+    }
+    float vinv = 1.f;
+    if (kScaled) {
+      vmax = quad_max(vmax);
+      vinv = vmax > 1e-37f ? 1.f / vmax : 0.f;
+      const float r = vref * vinv;
+      keep[0] *= r, keep[1] *= r;
+      vref = vmax;
+    }
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        s[i][j] = ex2(s[i][j] - base[j >> 1]);
+        l[j >> 1] += s[i][j];
+      }
+#pragma unroll
+    for (int i = 0; i < OT; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[i][j] *= keep[j >> 1];
+    if (kScaled) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        const float2 vv = *reinterpret_cast<const float2*>(sc + X::kKeys + kr0 + i * 8 + t4 * 2);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[i][j] *= (j & 1 ? vv.y : vv.x) * vinv;
+      }
+    }
+
+    // ---- o += p v
+    if constexpr (!kF32 && !kScaled) {
+#pragma unroll
+      for (int k = 0; k < N / 16; ++k) {
+        const uint32_t pa[4] = {pack_bf16(s[2 * k][0], s[2 * k][1]),
+                                pack_bf16(s[2 * k][2], s[2 * k][3]),
+                                pack_bf16(s[2 * k + 1][0], s[2 * k + 1][1]),
+                                pack_bf16(s[2 * k + 1][2], s[2 * k + 1][3])};
+        const int r = kr0 + k * 16 + (lane & 15);
+#pragma unroll
+        for (int n = 0; n < OT; n += 2) {
+          uint32_t b[4];
+          ldsm4t(b, vs + r * X::kRow + X::v_chunk(r, n + (lane >> 4)) * 16);
+          mma_bf16(o[n], pa, b[0], b[1]);
+          mma_bf16(o[n + 1], pa, b[2], b[3]);
+        }
+      }
+    } else if constexpr (!kF32) {
+      // 16 keys by 32 values a load; of the byte pair a thread gets for a key,
+      // the first goes to an even output tile and the second to an odd one:
+      // accumulator (2n + e, column c) is value 16 n + 2 c + e
+#pragma unroll
+      for (int k = 0; k < N / 16; ++k) {
+        const uint32_t pa[4] = {pack_f16x2(s[2 * k][0], s[2 * k][1]),
+                                pack_f16x2(s[2 * k][2], s[2 * k][3]),
+                                pack_f16x2(s[2 * k + 1][0], s[2 * k + 1][1]),
+                                pack_f16x2(s[2 * k + 1][2], s[2 * k + 1][3])};
+        const int r = kr0 + k * 16 + (lane & 15);
+#pragma unroll
+        for (int n = 0; n < OT / 2; n += 2) {
+          uint32_t b[4];
+          ldsm4t(b, vs + r * X::kRow + X::v_chunk(r, n + (lane >> 4)) * 16);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t c0 = __byte_perm(b[2 * e], 0, 0x3120);
+            const uint32_t c1 = __byte_perm(b[2 * e + 1], 0, 0x3120);
+            mma_f16(o[2 * (n + e)], pa, e4m3x2_f16x2(c0 & 0xffff), e4m3x2_f16x2(c1 & 0xffff));
+            mma_f16(o[2 * (n + e) + 1], pa, e4m3x2_f16x2(c0 >> 16), e4m3x2_f16x2(c1 >> 16));
+          }
+        }
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < NT; ++k) {
+        // keys 2 t4 and 2 t4 + 1 of each 8 are this thread's k indices
+        uint32_t h[4], e[4];
+        split_tf32(s[k][0], h[0], e[0]), split_tf32(s[k][2], h[1], e[1]);
+        split_tf32(s[k][1], h[2], e[2]), split_tf32(s[k][3], h[3], e[3]);
+        if constexpr (kScaled) {
+          const int r = kr0 + k * 8 + (lane & 7);
+#pragma unroll
+          for (int n = 0; n < OT / 2; n += 4) {
+            uint32_t b[4];
+            ldsm4t(b, vs + r * X::kRow + X::v_chunk(r, n + (lane >> 3)) * 16);
+#pragma unroll
+            for (int e2 = 0; e2 < 4; ++e2) {
+              const uint32_t c0 = e4m3x2_f16x2(b[e2] & 0xffff), c1 = e4m3x2_f16x2(b[e2] >> 16);
+              mma_tf32(o[2 * (n + e2)], e, __float_as_uint(half_lo(c0)), __float_as_uint(half_lo(c1)));
+              mma_tf32(o[2 * (n + e2)], h, __float_as_uint(half_lo(c0)), __float_as_uint(half_lo(c1)));
+              mma_tf32(o[2 * (n + e2) + 1], e, __float_as_uint(half_hi(c0)), __float_as_uint(half_hi(c1)));
+              mma_tf32(o[2 * (n + e2) + 1], h, __float_as_uint(half_hi(c0)), __float_as_uint(half_hi(c1)));
+            }
+          }
+        } else {
+          const int ra = kr0 + k * 8 + 2 * t4, rb = ra + 1;
+#pragma unroll
+          for (int n = 0; n < OT; ++n) {
+            const int d = n * 8 + g;
+            const float va = *reinterpret_cast<const float*>(vs + ra * X::kRow + X::v_chunk(ra, d >> 2) * 16 + (d & 3) * 4);
+            const float vb = *reinterpret_cast<const float*>(vs + rb * X::kRow + X::v_chunk(rb, d >> 2) * 16 + (d & 3) * 4);
+            uint32_t ah, al, bh, bl;
+            split_tf32(va, ah, al), split_tf32(vb, bh, bl);
+            mma_tf32(o[n], h, al, bl);
+            mma_tf32(o[n], e, ah, bh);
+            mma_tf32(o[n], h, ah, bh);
+          }
+        }
+      }
+    }
+  }
+  cp_wait<0>();
+#pragma unroll
+  for (int u = 0; u < 2; ++u) l[u] = quad_sum(l[u]);
+  if (kScaled)
+#pragma unroll
+    for (int i = 0; i < OT; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[i][j] *= vref;
+
+  // value index of accumulator element (tile n, j)
+  auto value_of = [&](int n, int j) {
+    return kScaled ? (n >> 1) * 16 + (t4 * 2 + (j & 1)) * 2 + (n & 1) : n * 8 + t4 * 2 + (j & 1);
+  };
+  if constexpr (KS) {
+    // ---- the four warps' sums meet in shared memory
+    __syncthreads();
+    float* jo = reinterpret_cast<float*>(smem);                      // [4][16][DP]
+    float2* jm = reinterpret_cast<float2*>(smem + 4 * 16 * DP * 4);  // [4][16]
+#pragma unroll
+    for (int i = 0; i < OT; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        jo[(warp * 16 + g + 8 * (j >> 1)) * DP + value_of(i, j)] = o[i][j];
+    if (t4 == 0) {
+      jm[warp * 16 + g] = make_float2(m[0], l[0]);
+      jm[warp * 16 + g + 8] = make_float2(m[1], l[1]);
+    }
+    __syncthreads();
+    const int nrow = (int)(rN - r0);
+    for (int i = threadIdx.x; i < nrow * D; i += kThreads) {
+      const int r = i / D, d = i - r * D;
+      float mm = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) mm = fmaxf(mm, jm[w * 16 + r].x);
+      const float base = mm == -INFINITY ? 0.f : mm;
+      float ll = 0.f, oo = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float f = ex2(jm[w * 16 + r].x - base);
+        ll += jm[w * 16 + r].y * f;
+        oo += jo[(w * 16 + r) * DP + d] * f;
+      }
+      const int64_t orow = out_row(r0 + r);
+      if (p.part_o) {
+        const int64_t slot = split * p.out_rows + orow;
+        p.part_o[slot * D + d] = oo;
+        if (d == 0) p.part_ml[slot] = make_float2(mm, ll);
+      } else {
+        static_cast<QT*>(a.out)[orow * D + d] = Elt<QT>::from_f(ll == 0.f ? 0.f : oo / ll);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      if (row[u] >= rN) continue;
+      const int64_t orow = out_row(row[u]);
+      const int64_t slot = split * p.out_rows + orow;
+      const float inv = l[u] == 0.f ? 0.f : 1.f / l[u];
+#pragma unroll
+      for (int i = 0; i < OT; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int d = value_of(i, j);
+          if (d >= D) continue;
+          if (p.part_o)
+            p.part_o[slot * D + d] = o[i][2 * u + j];
+          else
+            static_cast<QT*>(a.out)[orow * D + d] = Elt<QT>::from_f(o[i][2 * u + j] * inv);
+        }
+      if (p.part_o && t4 == 0) p.part_ml[slot] = make_float2(m[u], l[u]);
+    }
+  }
+}
+
+// joins the partial results of an output row, in the order of the splits
+template <typename T>
+__global__ void __launch_bounds__(128) k_attn_join(const float* part_o, const float2* part_ml,
+                                                   int splits, int64_t out_rows, int D, T* out) {
+  const int per = D >> 2;  // 4 values a thread
+  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  if (i >= out_rows * per) return;
+  const int64_t r = i / per;
+  const int d = (int)(i - r * per) * 4;
+  float m = -INFINITY, l = 0.f, x[4] = {};
+  for (int s = 0; s < splits; ++s) m = fmaxf(m, part_ml[s * out_rows + r].x);
+  const float base = m == -INFINITY ? 0.f : m;
+  for (int s = 0; s < splits; ++s) {
+    const float2 ml = part_ml[s * out_rows + r];
+    const float f = ex2(ml.x - base);
+    const float4 v = *reinterpret_cast<const float4*>(part_o + (s * out_rows + r) * D + d);
+    l += ml.y * f;
+    x[0] += v.x * f, x[1] += v.y * f, x[2] += v.z * f, x[3] += v.w * f;
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) out[r * D + d + e] = Elt<T>::from_f(l == 0.f ? 0.f : x[e] / l);
+}
+
+// How a call is cut: splits of the own columns and of the prefix.
+struct Plan {
+  bool own_ks, prefix_ks;
+  int own_splits, prefix_splits;
+  int64_t out_rows, bytes;
+};
+
+constexpr int kSlots = 296;    // CTAs resident at a time: 148 SMs, two each
+constexpr int64_t kMinKeys = 256;  // keys of a split, at least
+
+int splits_for(int64_t keys, int64_t ctas) {
+  if (keys <= kMinKeys || ctas >= kSlots) return 1;
+  const int64_t want = (2 * kSlots) / ctas;
+  const int64_t most = (keys + kMinKeys - 1) / kMinKeys;
+  return (int)(want < most ? want : most);
+}
+
+Plan plan_for(int64_t batch, int64_t tokens, int q_heads, int kv_heads, int head_dim,
+              int64_t capacity, int64_t col, int64_t prefix_cols) {
+  Plan p{};
+  const int group = q_heads / kv_heads;
+  const int64_t keys = col < 0 ? capacity : col + tokens;
+  const int64_t own_rows = tokens * group, pre_rows = batch * own_rows;
+  p.own_ks = own_rows <= 16;
+  p.prefix_ks = pre_rows <= 16;
+  const int ot = p.own_ks ? 16 : 64, pt = p.prefix_ks ? 16 : 64;
+  p.own_splits = splits_for(keys, batch * kv_heads * ((own_rows + ot - 1) / ot));
+  p.prefix_splits =
+      prefix_cols > 0 ? splits_for(prefix_cols, kv_heads * ((pre_rows + pt - 1) / pt)) : 0;
+  p.out_rows = batch * tokens * q_heads;
+  const int total = p.own_splits + p.prefix_splits;
+  p.bytes = total > 1 ? total * p.out_rows * (head_dim * 4 + 8) : 0;
+  return p;
+}
+
+template <typename QT, typename CT, int DP, bool KS, bool PREFIX>
+int run_part(const PartArgs& p, int64_t mats, cudaStream_t st) {
+  using X = Tile<QT, CT, DP, KS>;
+  auto* k = k_attn_part<QT, CT, DP, KS, PREFIX>;
+  const cudaError_t e =
+      cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, X::kSmem);
+  if (e != cudaSuccess) return (int)e;
+  const dim3 grid((unsigned)(mats * p.row_tiles * p.splits), (unsigned)p.a.kv_heads);
+  k<<<grid, kThreads, X::kSmem, st>>>(p);
+  return 0;
+}
+template <typename QT, typename CT, bool KS, bool PREFIX>
+int run_dp(const PartArgs& p, int64_t mats, cudaStream_t st) {
+  return p.a.head_dim <= 64 ? run_part<QT, CT, 64, KS, PREFIX>(p, mats, st)
+                            : run_part<QT, CT, 128, KS, PREFIX>(p, mats, st);
+}
+
+template <typename QT, typename CT>
+int run_attention(const AttnArgs& a, const Plan& pl, void* workspace, cudaStream_t st) {
+  const int group = a.q_heads / a.kv_heads;
+  const int total = pl.own_splits + pl.prefix_splits;
+  float* po = total > 1 ? static_cast<float*>(workspace) : nullptr;
+  float2* pm = total > 1 ? reinterpret_cast<float2*>(po + total * pl.out_rows * a.head_dim) : nullptr;
+  PartArgs p{a, group, a.tokens * group, 0, pl.own_splits, pl.out_rows, po, pm};
+  p.row_tiles = (int)((p.rows + (pl.own_ks ? 15 : 63)) / (pl.own_ks ? 16 : 64));
+  int rc = pl.own_ks ? run_dp<QT, CT, true, false>(p, a.batch, st)
+                     : run_dp<QT, CT, false, false>(p, a.batch, st);
+  if (rc) return rc;
+  if (pl.prefix_splits) {
+    PartArgs x{a, group, a.batch * a.tokens * group, 0, pl.prefix_splits, pl.out_rows,
+               po + pl.own_splits * pl.out_rows * a.head_dim,
+               pm + pl.own_splits * pl.out_rows};
+    x.row_tiles = (int)((x.rows + (pl.prefix_ks ? 15 : 63)) / (pl.prefix_ks ? 16 : 64));
+    rc = pl.prefix_ks ? run_dp<QT, QT, true, true>(x, 1, st) : run_dp<QT, QT, false, true>(x, 1, st);
+    if (rc) return rc;
+  }
+  if (total > 1) {
+    const int64_t n = pl.out_rows * (a.head_dim / 4);
+    k_attn_join<QT><<<(unsigned)((n + 127) / 128), 128, 0, st>>>(po, pm, total, pl.out_rows,
+                                                                  a.head_dim,
+                                                                  static_cast<QT*>(a.out));
+  }
+  return 0;
 }
 
 }  // namespace
@@ -100,8 +802,10 @@ extern "C" int mep_cache_attention_workspace(int dtype, int cache_dtype, int64_t
     return serve_invalid(op, why);
   if (capacity < 0 || prefix_cols < 0) return serve_invalid(op, "negative columns");
   if (!bytes_out) return serve_invalid(op, "bytes_out is required");
-  (void)col;
-  *bytes_out = 0;
+  *bytes_out = batch && tokens ? plan_for(batch, tokens, q_heads, kv_heads, head_dim, capacity, col,
+                                          prefix_cols)
+                                     .bytes
+                               : 0;
   return MEP_OK;
 }
 
@@ -132,19 +836,18 @@ extern "C" int mep_cache_attention(int dtype, int cache_dtype, int64_t batch, in
   if (bad_strides(a.q, dtype == MEP_BF16 ? 2 : 4) || !aligned16(k_cache) || !aligned16(v_cache) ||
       !aligned16(k_prefix) || !aligned16(v_prefix) || !aligned16(out))
     return serve_invalid(op, "tensors and row strides must be multiples of 16 bytes");
-  (void)workspace, (void)workspace_bytes;
+  const Plan pl = plan_for(batch, tokens, q_heads, kv_heads, head_dim, capacity,
+                           col_dev ? -1 : col, prefix_cols);
+  if (pl.bytes > 0 && (!workspace || workspace_bytes < pl.bytes || !aligned16(workspace)))
+    return serve_invalid(op, "workspace of " + std::to_string(pl.bytes) + " bytes needed");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const unsigned grid = (unsigned)((batch * tokens * q_heads + 3) / 4);
-  if (dtype == MEP_BF16) {
-    if (cache_dtype == MEP_E4M3)
-      k_attn<__nv_bfloat16, uint8_t><<<grid, 128, 0, st>>>(a);
-    else
-      k_attn<__nv_bfloat16, __nv_bfloat16><<<grid, 128, 0, st>>>(a);
-  } else {
-    if (cache_dtype == MEP_E4M3)
-      k_attn<float, uint8_t><<<grid, 128, 0, st>>>(a);
-    else
-      k_attn<float, float><<<grid, 128, 0, st>>>(a);
-  }
+  int rc;
+  if (dtype == MEP_BF16)
+    rc = cache_dtype == MEP_E4M3 ? run_attention<__nv_bfloat16, uint8_t>(a, pl, workspace, st)
+                                 : run_attention<__nv_bfloat16, __nv_bfloat16>(a, pl, workspace, st);
+  else
+    rc = cache_dtype == MEP_E4M3 ? run_attention<float, uint8_t>(a, pl, workspace, st)
+                                 : run_attention<float, float>(a, pl, workspace, st);
+  if (rc) return serve_cuda(op, (cudaError_t)rc);
   return serve_launched(op);
 }

@@ -18,6 +18,10 @@ inline int serve_invalid(const char* op, const std::string& msg) {
   set_global_error(std::string(op) + ": " + msg);
   return MEP_ERR_INVALID;
 }
+inline int serve_cuda(const char* op, cudaError_t e) {
+  set_global_error(std::string(op) + ": " + cudaGetErrorString(e));
+  return MEP_ERR_CUDA;
+}
 // status of the launches just enqueued
 inline int serve_launched(const char* op) {
   const cudaError_t e = cudaGetLastError();
@@ -55,6 +59,7 @@ inline const char* bad_heads(int dtype, int cache_dtype, int64_t batch, int64_t 
   if (batch > 65535 || tokens > (1 << 24)) return "batch up to 65535, tokens up to 2^24";
   if (kv_heads < 1 || q_heads < 1 || q_heads % kv_heads != 0 || q_heads > 1024)
     return "q_heads must be a multiple of kv_heads, up to 1024";
+  if (batch * tokens * q_heads > 0x7fffffff) return "batch * tokens * q_heads up to 2^31 - 1";
   if (head_dim < 16 || head_dim > kMaxHeadDim || head_dim % 16 != 0)
     return "head_dim must be a multiple of 16 up to 128";
   return nullptr;

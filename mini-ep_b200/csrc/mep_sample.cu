@@ -8,10 +8,11 @@
 // logit counts as -inf; several +inf logits share the mass.
 //
 // Whether a token is drawn is decided at borders of running sums, so the
-// weights are held as 64-bit fixed-point numbers (scaled so that a row's sum
-// fits 62 bits): integer sums do not depend on their order, and the rounding
-// of each weight, computed in 64 bits, is below 2^-44 of the best token's.
+// weights are held as 64-bit fixed-point numbers (the best token's is 2^46, or
+// less where the row's sum would pass 62 bits): integer sums do not depend on
+// their order, and a weight, computed in 64 bits, is off by half a unit.
 #include <cstdint>
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
 #include "mep_device.cuh"
@@ -19,6 +20,8 @@
 
 namespace mep {
 namespace {
+
+namespace cg = cooperative_groups;
 
 struct SampleArgs {
   const void* logits;
@@ -49,179 +52,577 @@ __device__ __forceinline__ float logit_of(uint32_t k) {
 }
 constexpr uint32_t kKeyNegInf = 0x007fffffu;  // key_of(-inf), the smallest
 
-struct Row {
-  float lmax, t;
-  double one;  // fixed-point value of weight 1
-  __device__ double weight(uint32_t key) const {
-    const float l = logit_of(key);
-    if (l == lmax) return 1.0;
-    return t > 0.f ? exp(((double)l - (double)lmax) / (double)t) : 0.0;
+// ---- weights
+// exp2 by table and polynomial (P. T. P. Tang, "Table-driven implementation of
+// the exponential function in IEEE floating-point arithmetic", ACM TOMS 15(2),
+// 1989): with (l - lmax) * 256 log2(e) / T = k + r, |r| <= 1/2, the weight is
+// 2^(k >> 8) * 2^((k & 255) / 256) * e^(r ln2 / 256), the last factor to the
+// fourth power of r ln2 / 256 <= 0.00136 (4e-17 left).
+struct Weights {
+  float lmax, lcut;   // logits below lcut weigh less than half a unit
+  double top, c;      // lmax; 256 log2(e) / temperature
+  int scale;          // weight 1 is 2^scale
+  const double* tab;  // 2^(j / 256)
+  __device__ u64 operator()(float l) const {
+    if (l == lmax) return 1ull << scale;
+    if (!(l >= lcut)) return 0;
+    constexpr double kMagic = 6755399441055744.0;        // 1.5 * 2^52: rounds to an integer
+    constexpr double a1 = 0.693147180559945309417 / 256;  // ln 2 / 256
+    const double d = (double)l - top;
+    const double z = fma(d, c, kMagic);
+    const int k = __double2loint(z);
+    const double r = fma(d, c, kMagic - z);
+    const double q = r * fma(r, fma(r, fma(r, a1 * a1 * a1 * a1 / 24, a1 * a1 * a1 / 6),
+                                    a1 * a1 / 2), a1);
+    const double t = tab[k & 255];
+    const double w = fma(t, q, t);
+    // times 2^((k >> 8) + scale) in the exponent field, then to an integer by
+    // adding 2^52 (weights stay below 2^47)
+    const double y = __hiloint2double(__double2hiint(w) + (((k >> 8) + scale) << 20),
+                                      __double2loint(w));
+    return (u64)__double_as_longlong(y + 4503599627370496.0) & 0xfffffffffffffull;
   }
-  __device__ u64 fixed(uint32_t key) const { return __double2ull_rn(weight(key) * one); }
 };
 
-template <int T>
-__device__ u64 block_sum(u64 v, u64* buf) {
-  __syncthreads();
+constexpr int kNT = 512;        // threads of a CTA
+constexpr int kNW = kNT / 32;
+constexpr int kBins = 1024;
+constexpr int kList = 1024;     // candidates the leading CTA can finish alone
+constexpr int kMaxCtas = 8;     // CTAs of a row
+
+struct Shared {
+  double tab[256];
+  uint32_t cnt[kBins], lo[kBins], hi[kBins];  // this CTA's histogram
+  u64 tmass[kBins];                           // the row's
+  uint32_t tcnt[kBins];
+  u64 item[kList], w[kList];
+  u64 wmass[kMaxCtas * kNW];     // of every warp of the row
+  uint32_t wties[kMaxCtas * kNW];
+  u64 best[kMaxCtas];
+  float lmin[kMaxCtas];
+  u64 red[kNW], red2[kNW];
+  uint32_t n_items;
+  // results that one thread finds for all
+  uint32_t r_bin, r_cnt, r_hi;
+  u64 r_above, r_mass;
+};
+
+// 16 bytes of a row: ids at `first` + 0..E-1, -inf outside [0, vocab)
+template <typename T>
+struct Vec {
+  static constexpr int E = 16 / sizeof(T);
+};
+__device__ __forceinline__ void unpack(const uint4& v, float (&x)[4]) {
+  x[0] = __uint_as_float(v.x), x[1] = __uint_as_float(v.y), x[2] = __uint_as_float(v.z),
+  x[3] = __uint_as_float(v.w);
+}
+__device__ __forceinline__ void unpack(const uint4& v, float (&x)[8]) {
+  const uint32_t u[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if (lane_id() == 0) buf[warp_id()] = v;
-  __syncthreads();
-  u64 s = 0;
-  for (int i = 0; i < T / 32; ++i) s += buf[i];
-  return s;
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = __uint_as_float(u[i] << 16);
+    x[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+  }
+}
+template <typename T>
+__device__ __forceinline__ uint4 fetch(const T* row, int64_t id, int64_t vocab) {
+  constexpr int E = Vec<T>::E;
+  if (id >= 0 && id + E <= vocab) return *reinterpret_cast<const uint4*>(row + id);
+  __align__(16) T x[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i)
+    x[i] = id + i >= 0 && id + i < vocab ? row[id + i] : Elt<T>::from_f(-INFINITY);
+  return *reinterpret_cast<const uint4*>(x);
 }
 
-// One CTA per row. The top-k and top-p borders are found by building, bit by
-// bit, the smallest key whose count (mass) above it is still below the limit.
-template <typename T>
-__global__ void __launch_bounds__(1024) k_sample(const SampleArgs a) {
-  constexpr int NT = 1024;
-  __shared__ u64 buf[32];
-  __shared__ u64 scan_w[32], scan_c[32];
-  const int64_t row = blockIdx.x, V = a.vocab;
+__device__ __forceinline__ u64 warp_sum(u64 v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+__device__ __forceinline__ u64 warp_scan(u64 v) {  // inclusive
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const u64 y = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane_id() >= o) v += y;
+  }
+  return v;
+}
+// exclusive prefix over the CTA's threads, and the whole sum
+__device__ __forceinline__ u64 block_scan(u64 v, u64* buf, u64& total) {
+  const u64 inc = warp_scan(v);
+  __syncthreads();
+  if (lane_id() == 31) buf[warp_id()] = inc;
+  __syncthreads();
+  u64 before = 0;
+  total = 0;
+#pragma unroll
+  for (int i = 0; i < kNW; ++i) {
+    if (i < warp_id()) before += buf[i];
+    total += buf[i];
+  }
+  return before + inc - v;
+}
+
+// descending bitonic sort of x[0..n), n a power of two
+__device__ void sort_desc(u64* x, int n) {
+  for (int k = 2; k <= n; k <<= 1)
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      __syncthreads();
+      for (int i = threadIdx.x; i < n / 2; i += kNT) {
+        const int a = ((i & ~(j - 1)) << 1) | (i & (j - 1)), b = a | j;
+        const u64 p = x[a], q = x[b];
+        if ((p < q) == ((a & k) == 0)) x[a] = q, x[b] = p;
+      }
+    }
+  __syncthreads();
+}
+
+// A cluster of CTAs takes a row; each keeps a run of its ids in shared memory
+// (CACHED) or re-reads it, each warp a run of that, so that sums over ids stay
+// in order. Without a filter the weights are summed per warp, and the warp
+// whose share holds the target finds the token. With top_k or top_p a
+// histogram over the logits (counts, or masses) tells which bins can hold kept
+// tokens; when those are at most kList, as good as always, the leading CTA
+// sorts and finishes them alone, else the borders are found by histograms over
+// ever narrower key ranges. All sums are of integers: their order is free.
+template <typename T, bool CACHED>
+__global__ void __launch_bounds__(kNT) k_sample(const SampleArgs a) {
+  constexpr int E = Vec<T>::E;
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  Shared& S = *reinterpret_cast<Shared*>(smem_raw);
+  uint4* cache = reinterpret_cast<uint4*>(smem_raw + (sizeof(Shared) + 15) / 16 * 16);
+  cg::cluster_group cluster = cg::this_cluster();
+  const int nc = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const int64_t row = blockIdx.x / nc, V = a.vocab;
+  const int tid = threadIdx.x, lane = lane_id(), warp = warp_id();
   const T* x = static_cast<const T*>(a.logits) + row * a.stride;
   const float temp = a.temperature ? a.temperature[row] : a.temperature_s;
   const int64_t top_k = a.top_k ? a.top_k[row] : a.top_k_s;
   const float top_p = a.top_p ? a.top_p[row] : a.top_p_s;
   const float min_p = a.min_p ? a.min_p[row] : a.min_p_s;
-  const int tid = threadIdx.x;
-  auto key_at = [&](int64_t i) { return key_of(Elt<T>::to_f(x[i])); };
 
-  // the best token: largest key, lowest id
+  // 16-byte pieces of the row on the grid of its addresses; piece p holds the
+  // ids from p * E - shift on. This CTA has [p0, p1), this warp [w0, w1).
+  const int shift = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
+  const int64_t pieces = (shift + V + E - 1) / E;
+  const int64_t per = (pieces + nc - 1) / nc;
+  const int64_t p0 = min(pieces, per * rank), p1 = min(pieces, p0 + per);
+  const int64_t per_w = ((p1 - p0 + kNW - 1) / kNW + 31) / 32 * 32;
+  const int64_t w0 = min(p1, p0 + per_w * warp), w1 = min(p1, w0 + per_w);
+
+  auto piece = [&](int64_t p) -> uint4 {
+    return CACHED ? cache[p - p0] : fetch<T>(x, p * E - shift, V);
+  };
+  // f(l, id) for this warp's ids
+  auto each = [&](auto f) {
+    for (int64_t p = w0 + lane; p < w1; p += 32) {
+      float l[E];
+      unpack(piece(p), l);
+#pragma unroll
+      for (int i = 0; i < E; ++i) f(l[i], p * E - shift + i);
+    }
+  };
+
+  // ---- the best token and the smallest finite logit
+  if (tid < 256) S.tab[tid] = exp2(tid / 256.0);
+  for (int i = tid; i < kBins; i += kNT) S.cnt[i] = S.lo[i] = S.hi[i] = 0;
+  if (tid == 0) S.n_items = 0;
   u64 best = 0;
-  for (int64_t i = tid; i < V; i += NT) {
-    const u64 c = (u64)key_at(i) << 32 | (uint32_t)~(uint32_t)i;
-    best = c > best ? c : best;
+  float lmin = INFINITY;
+  for (int64_t p = w0 + lane; p < w1; p += 32) {
+    const uint4 v = fetch<T>(x, p * E - shift, V);
+    if (CACHED) cache[p - p0] = v;
+    float l[E];
+    unpack(v, l);
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const int64_t id = p * E - shift + i;
+      if (id >= 0 && id < V) {
+        const u64 c = (u64)key_of(l[i]) << 32 | (uint32_t)~(uint32_t)id;
+        best = c > best ? c : best;
+      }
+      if (l[i] > -INFINITY) lmin = fminf(lmin, l[i]);
+    }
   }
-  __syncthreads();
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const u64 c = __shfl_xor_sync(0xffffffffu, best, o);
     best = c > best ? c : best;
+    lmin = fminf(lmin, __shfl_xor_sync(0xffffffffu, lmin, o));
   }
-  if (lane_id() == 0) buf[warp_id()] = best;
+  if (lane == 0) S.red[warp] = best, S.red2[warp] = __float_as_uint(lmin);
   __syncthreads();
-  for (int i = 0; i < NT / 32; ++i) best = buf[i] > best ? buf[i] : best;
-  const uint32_t kmax = (uint32_t)(best >> 32);
-  if (kmax == kKeyNegInf) {  // nothing to draw
-    if (tid == 0) {
-      a.tokens[row] = -1;
-      if (a.logprobs) a.logprobs[row] = -INFINITY;
+  if (tid < nc) {
+    for (int i = 0; i < kNW; ++i) {
+      best = S.red[i] > best ? S.red[i] : best;
+      lmin = fminf(lmin, __uint_as_float((uint32_t)S.red2[i]));
     }
-    return;
+    Shared* to = cluster.map_shared_rank(&S, tid);
+    to->best[rank] = best;
+    to->lmin[rank] = lmin;
   }
-  if (!(temp > 0.f)) {
-    if (tid == 0) {
-      a.tokens[row] = (uint32_t)~(uint32_t)best;
-      if (a.logprobs) a.logprobs[row] = 0.f;
+  cluster.sync();
+  best = 0;
+  for (int i = 0; i < nc; ++i) {
+    best = S.best[i] > best ? S.best[i] : best;
+    lmin = fminf(lmin, S.lmin[i]);
+  }
+  const uint32_t kmax = (uint32_t)(best >> 32);
+  if (kmax == kKeyNegInf || !(temp > 0.f)) {  // nothing to draw, or the best token
+    if (rank == 0 && tid == 0) {
+      const bool none = kmax == kKeyNegInf;
+      a.tokens[row] = none ? -1 : (int64_t)(uint32_t)~(uint32_t)best;
+      if (a.logprobs) a.logprobs[row] = none ? -INFINITY : 0.f;
     }
     return;
   }
   int bits = 0;
   while ((1ll << bits) < V) ++bits;
-  const Row r{logit_of(kmax), temp, (double)(1ull << (62 - bits < 47 ? 62 - bits : 47))};
+  Weights W;
+  W.lmax = logit_of(kmax);
+  // 34 temperatures below the best a weight is 2^-49; lmax = inf leaves only
+  // its equals, -inf never weighs
+  W.lcut = fmaxf(W.lmax - 34.f * temp, -3.402823466e38f);
+  W.top = W.lmax;
+  W.c = 369.329930467574632284 / (double)temp;  // 256 log2(e)
+  W.scale = min(46, 62 - bits);
+  W.tab = S.tab;
+  const double one = (double)(1ull << W.scale);
+  const double floor_p = (double)min_p * one;
+  const bool by_k = top_k > 0 && top_k < V, by_p = top_p < 1.f;
+  const double u = a.u[row];
+  auto target_of = [&](u64 total) {
+    const u64 t = (u64)((u > 0.0 ? (u < 1.0 ? u : 1.0) : 0.0) * (double)total);
+    return t < total ? t : total - 1;  // u = 1: the last kept token
+  };
+  auto answer = [&](int64_t id, u64 w, u64 total) {
+    a.tokens[row] = id;
+    if (a.logprobs) a.logprobs[row] = (float)log((double)w / (double)total);
+  };
+  auto add_mass = [&](int b, u64 w) {  // 64-bit sum in two 32-bit halves, carry by hand
+    const uint32_t lo = (uint32_t)w;
+    const uint32_t old = atomicAdd(&S.lo[b], lo);
+    atomicAdd(&S.hi[b], (uint32_t)(w >> 32) + (old + lo < old));
+  };
+  // the CTAs' histograms summed into everyone's tcnt / tmass
+  auto join = [&] {
+    cluster.sync();
+    const int share = kBins / nc;
+    for (int i = tid; i < share; i += kNT) {
+      const int b = rank * share + i;
+      uint32_t c = 0;
+      u64 m = 0;
+      for (int r = 0; r < nc; ++r) {
+        const Shared* from = cluster.map_shared_rank(&S, r);
+        c += from->cnt[b];
+        m += (u64)from->hi[b] << 32 | 0ull;
+        m += from->lo[b];
+      }
+      for (int r = 0; r < nc; ++r) {
+        Shared* to = cluster.map_shared_rank(&S, r);
+        to->tcnt[b] = c;
+        to->tmass[b] = m;
+      }
+    }
+    cluster.sync();
+  };
 
-  // kept: keys above `edge`, and the first `ties` ids of key `edge`
-  uint32_t edge = 0;
+  uint32_t edge = 0;  // kept: keys above `edge`, and the first `ties` ids of key `edge`
   u64 ties = ~0ull;
-  if (top_k > 0 && top_k < V) {
-    for (int bit = 31; bit >= 0; --bit) {
-      const uint32_t tryk = edge | (1u << bit);
-      u64 n = 0;
-      for (int64_t i = tid; i < V; i += NT) n += key_at(i) >= tryk;
-      if (block_sum<NT>(n, buf) >= (u64)top_k) edge = tryk;
+  if (by_k || by_p) {
+    // ---- bins of equal width in the logit, best first
+    const float range = fminf(W.lmax - W.lcut, W.lmax - lmin);
+    const float bscale = range > 0.f && range < INFINITY ? (float)kBins / range : 0.f;
+    auto bin_of = [&](float l) {
+      return l == W.lmax ? 0 : (int)fminf((W.lmax - l) * bscale, (float)(kBins - 1));
+    };
+    each([&](float l, int64_t) {
+      if (l >= W.lcut) {
+        const int b = bin_of(l);
+        atomicAdd(&S.cnt[b], 1u);
+        if (!by_k) add_mass(b, W(l));
+      }
+    });
+    join();
+    // exclusive sums over the bins, two a thread
+    const uint32_t c0 = S.tcnt[2 * tid], c1 = S.tcnt[2 * tid + 1];
+    const u64 m0 = S.tmass[2 * tid], m1 = S.tmass[2 * tid + 1];
+    u64 nall, mall;
+    const u64 cb = block_scan(c0 + c1, S.red, nall);
+    const u64 mb = block_scan(m0 + m1, S.red2, mall);
+    const double limit = (double)top_p * (double)mall;
+    // candidates: bins that begin before the border
+    if (tid == 0) S.r_bin = 0, S.r_cnt = S.tcnt[0];
+    __syncthreads();
+#pragma unroll
+    for (int e = 1; e >= 0; --e) {
+      const u64 cx = cb + (e ? c0 : 0), mx = mb + (e ? m0 : 0);
+      const bool in = by_k ? cx < (u64)top_k : (double)mx < limit;
+      if (in) {
+        atomicMax(&S.r_bin, (uint32_t)(2 * tid + e));
+        break;
+      }
     }
-    u64 n = 0;
-    for (int64_t i = tid; i < V; i += NT) n += key_at(i) > edge;
-    ties = (u64)top_k - block_sum<NT>(n, buf);
-  }
-  if (top_p < 1.f) {
-    u64 w = 0, same = 0;
-    for (int64_t i = tid; i < V; i += NT) {
-      const uint32_t k = key_at(i);
-      if (k > edge) w += r.fixed(k);
-      same += k == edge;
+    __syncthreads();
+    if (S.r_bin / 2 == tid) S.r_cnt = (uint32_t)(cb + c0 + (S.r_bin & 1 ? c1 : 0));
+    __syncthreads();
+    const uint32_t last = S.r_bin, n = S.r_cnt;
+    if (n <= kList) {
+      // ---- candidates to the leading CTA
+      Shared* lead = cluster.map_shared_rank(&S, 0);
+      each([&](float l, int64_t id) {
+        if (l >= W.lcut && (uint32_t)bin_of(l) <= last)
+          lead->item[atomicAdd(&lead->n_items, 1u)] = (u64)key_of(l) << 32 | (uint32_t)~(uint32_t)id;
+      });
+      cluster.sync();
+      if (rank != 0) return;
+      int n2 = 32;
+      while (n2 < (int)n) n2 <<= 1;
+      for (int i = (int)n + tid; i < n2; i += kNT) S.item[i] = 0;
+      sort_desc(S.item, n2);
+      // two neighbours a thread: their weights, and the mass before them
+      u64 w[2], before, mass;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int i = 2 * tid + e;
+        w[e] = i < (int)n && !(by_k && i >= top_k) ? W(logit_of((uint32_t)(S.item[i] >> 32))) : 0;
+      }
+      before = block_scan(w[0] + w[1], S.red, mass);
+      const double lim = by_k ? (double)top_p * (double)mass : limit;
+      bool keep[2];
+      u64 kept = 0;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const u64 bf = before + (e ? w[0] : 0);
+        keep[e] = w[e] > 0 && (2 * tid + e == 0 ||
+                               ((!by_p || (double)bf < lim) && (double)w[e] >= floor_p));
+        kept += keep[e];
+      }
+      u64 nkept;
+      block_scan(kept, S.red2, nkept);  // the kept are the first nkept of the list
+      // the kept by id: ~id in the upper half, descending
+      n2 = 32;
+      while (n2 < (int)nkept) n2 <<= 1;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int i = 2 * tid + e;
+        S.w[i] = w[e];
+        if (i < n2) S.item[i] = keep[e] ? S.item[i] << 32 | (uint32_t)i : 0;
+      }
+      sort_desc(S.item, n2);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int i = 2 * tid + e;
+        w[e] = i < (int)nkept ? S.w[(uint32_t)S.item[i]] : 0;
+      }
+      u64 total;
+      u64 run = block_scan(w[0] + w[1], S.red, total);
+      const u64 target = target_of(total);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        if (run <= target && run + w[e] > target)
+          answer((uint32_t)~(uint32_t)(S.item[2 * tid + e] >> 32), w[e], total);
+        run += w[e];
+      }
+      return;
     }
-    const u64 above = block_sum<NT>(w, buf), eq = block_sum<NT>(same, buf);
-    const u64 total = above + (eq < ties ? eq : ties) * r.fixed(edge);
-    const double limit = (double)top_p * (double)total;
-    // the smallest key at least one of whose tokens is kept: mass above it < limit
-    uint32_t low = edge;
-    if (!((double)above < limit)) {
-      // largest key whose mass at or above it reaches the limit
-      uint32_t k2 = 0;
-      for (int bit = 31; bit >= 0; --bit) {
-        const uint32_t tryk = k2 | (1u << bit);
-        u64 s = 0;
-        for (int64_t i = tid; i < V; i += NT) {
-          const uint32_t k = key_at(i);
-          if (k >= tryk) s += r.fixed(k);
+    // ---- too many candidates: borders by histograms over key ranges.
+    // largest key whose count (mass) at or above it reaches `want`, and what is above it
+    auto border = [&](bool mass, double want, u64& above_out) {
+      uint32_t lo = edge, hi = kmax;
+      const uint32_t kcut = key_of(W.lcut);
+      if (lo < kcut) lo = kcut;
+      u64 above = 0;
+      for (;;) {
+        const uint32_t span = hi - lo;
+        const int sh = max(0, 32 - __clz(span) - 10);
+        cluster.sync();  // nobody still reads the last histogram
+        for (int i = tid; i < kBins; i += kNT) S.cnt[i] = S.lo[i] = S.hi[i] = 0;
+        __syncthreads();
+        each([&](float l, int64_t id) {
+          const uint32_t k = key_of(l);
+          if (id >= 0 && id < V && k >= lo && k <= hi) {
+            const int b = kBins - 1 - (int)((k - lo) >> sh);  // best first
+            if (mass)
+              add_mass(b, W(l));
+            else
+              atomicAdd(&S.cnt[b], 1u);
+          }
+        });
+        join();
+        u64 v[2], all;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) v[e] = mass ? S.tmass[2 * tid + e] : S.tcnt[2 * tid + e];
+        u64 run = above + block_scan(v[0] + v[1], S.red, all);
+        // where nothing reaches it: the last bin
+        if (tid == 0) S.r_bin = kBins - 1 - (span >> sh), S.r_above = above;
+        __syncthreads();
+        const bool none = !((double)(above + all) >= want);
+        if (none) {
+          if (tid == kNT - 1) S.r_bin = kBins - 1, S.r_above = run + v[0];
+        } else {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            if ((double)run < want && (double)(run + v[e]) >= want)
+              S.r_bin = 2 * tid + e, S.r_above = run;
+            run += v[e];
+          }
         }
-        if ((double)block_sum<NT>(s, buf) >= limit) k2 = tryk;
+        __syncthreads();
+        const uint32_t b = kBins - 1 - S.r_bin;
+        above = S.r_above;
+        __syncthreads();
+        const uint32_t nlo = lo + (b << sh);
+        hi = min(hi, nlo + ((1u << sh) - 1));
+        lo = nlo;
+        if (sh == 0) break;
       }
-      low = k2 > kmax ? kmax : k2;  // limit <= 0 or NaN: the best key alone
-      ties = ~0ull;
-    }
-    u64 s = 0;
-    for (int64_t i = tid; i < V; i += NT) {
-      const uint32_t k = key_at(i);
-      if (k > low) s += r.fixed(k);
-    }
-    const u64 mass = block_sum<NT>(s, buf), w1 = r.fixed(low);
-    if (w1 > 0) {
-      const double n = ceil((limit - (double)mass) / (double)w1);
-      const u64 m = n < 1.0 ? 1 : (u64)n;
-      if (m < ties) ties = m;
-    }
-    edge = low;
-  }
-  // draw: running sums in id order, one tile of NT ids at a time
-  u64 target = 0, total = 0;
-  for (int pass = 0; pass < 2; ++pass) {
-    u64 run_w = 0, run_c = 0;
-    for (int64_t base = 0; base < V; base += NT) {
-      const int64_t i = base + tid;
-      const uint32_t k = i < V ? key_at(i) : 0;
-      u64 eq = k == edge && i < V, c = eq;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const u64 y = __shfl_up_sync(0xffffffffu, c, o);
-        if (lane_id() >= o) c += y;
-      }
-      __syncthreads();
-      if (lane_id() == 31) scan_c[warp_id()] = c;
-      __syncthreads();
-      u64 before = run_c;
-      for (int w = 0; w < warp_id(); ++w) before += scan_c[w];
-      for (int w = 0; w < 32; ++w) run_c += scan_c[w];
-      const bool in = i < V && (k > edge || (eq && before + c <= ties)) &&
-                      (k == kmax || r.weight(k) >= (double)min_p);
-      const u64 w1 = in ? r.fixed(k) : 0;
-      u64 w = w1;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const u64 y = __shfl_up_sync(0xffffffffu, w, o);
-        if (lane_id() >= o) w += y;
-      }
-      if (lane_id() == 31) scan_w[warp_id()] = w;
-      __syncthreads();
-      u64 sum = run_w + w;
-      for (int q = 0; q < warp_id(); ++q) sum += scan_w[q];
-      for (int q = 0; q < 32; ++q) run_w += scan_w[q];
-      if (pass == 1 && w1 > 0 && sum > target && sum - w1 <= target) {
-        a.tokens[row] = i;
-        if (a.logprobs) a.logprobs[row] = (float)log((double)w1 / (double)total);
+      above_out = above;
+      return lo;
+    };
+    u64 above;
+    // sums over the whole row of what f gives for each id
+    auto row_sum = [&](auto f) {
+      u64 s = 0, all;
+      each([&](float l, int64_t id) { s += f(l, id); });
+      block_scan(s, S.red, all);
+      if (tid < nc) cluster.map_shared_rank(&S, tid)->best[rank] = all;
+      cluster.sync();
+      all = 0;
+      for (int i = 0; i < nc; ++i) all += S.best[i];
+      cluster.sync();
+      return all;
+    };
+    double lim = limit;
+    bool found = !by_p;
+    if (by_k) {
+      edge = border(false, (double)top_k, above);
+      ties = (u64)top_k - above;
+      if (by_p) {
+        const uint32_t ed = edge;
+        const u64 m = row_sum([&](float l, int64_t) { return key_of(l) > ed ? W(l) : 0ull; });
+        const u64 eq = row_sum([&](float l, int64_t id) {
+          return (u64)(id >= 0 && id < V && key_of(l) == ed);
+        });
+        lim = (double)top_p * (double)(m + min(ties, eq) * W(logit_of(edge)));
+        if ((double)m < lim) {  // the border lies among the edge's own ties, or behind them
+          const u64 w1 = W(logit_of(edge));
+          if (w1 > 0) ties = min(ties, (u64)ceil((lim - (double)m) / (double)w1));
+          found = true;
+        }
       }
     }
-    if (pass == 0) {
-      total = run_w;
-      const double u = a.u[row];
-      const double g = (u > 0.0 ? (u < 1.0 ? u : 1.0) : 0.0) * (double)total;
-      target = (u64)g;
-      if (target >= total) target = total - 1;  // u = 1: the last kept token
+    if (!found) {
+      edge = border(true, lim, above);
+      const u64 w1 = W(logit_of(edge));
+      ties = w1 > 0 ? (u64)fmax(1.0, ceil((lim - (double)above) / (double)w1)) : ~0ull;
     }
   }
+
+  // ---- each warp's kept mass and its tokens on the edge, to every CTA
+  const u64 wedge = W(logit_of(edge));
+  auto low = [&](u64 w) { return (double)w < floor_p && w < 1ull << W.scale; };
+  u64 mass = 0;
+  uint32_t on_edge = 0;
+  each([&](float l, int64_t id) {
+    const uint32_t k = key_of(l);
+    if (k > edge) {
+      const u64 w = W(l);
+      if (!low(w)) mass += w;
+    }
+    on_edge += k == edge && id >= 0 && id < V;
+  });
+  mass = warp_sum(mass);
+  on_edge = __reduce_add_sync(0xffffffffu, on_edge);
+  if (lane < nc) {
+    Shared* to = cluster.map_shared_rank(&S, lane);
+    to->wmass[rank * kNW + warp] = mass;
+    to->wties[rank * kNW + warp] = on_edge;
+  }
+  cluster.sync();
+  // this warp's share begins at `start`; the row's kept mass is `total`
+  const bool edge_kept = edge && wedge > 0 && !low(wedge);
+  u64 start = 0, total = 0, ties_before = 0, seen = 0;
+  for (int i = 0; i < nc * kNW; ++i) {
+    if (i == rank * kNW + warp) start = total, ties_before = seen;
+    const u64 left = ties > seen ? ties - seen : 0;
+    total += S.wmass[i] + (edge_kept ? min((u64)S.wties[i], left) * wedge : 0);
+    seen += S.wties[i];
+  }
+  const u64 target = target_of(total);
+  u64 own = mass;
+  if (edge_kept) own += min((u64)on_edge, ties > ties_before ? ties - ties_before : 0) * wedge;
+  if (target < start || target >= start + own) return;
+  for (int64_t p = w0; p < w1; p += 32) {
+    float l[E];
+    const bool have = p + lane < w1;
+    if (have) unpack(piece(p + lane), l);
+    u64 w[E], sum = 0;
+    uint32_t eq = 0;
+    const int64_t id0 = (p + lane) * E - shift;
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+      eq += have && id0 + i >= 0 && id0 + i < V && key_of(l[i]) == edge;
+    u64 rank_eq = ties_before + warp_scan(eq) - eq;
+    ties_before += __reduce_add_sync(0xffffffffu, eq);
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      w[i] = 0;
+      if (have && id0 + i >= 0 && id0 + i < V) {
+        const uint32_t k = key_of(l[i]);
+        if (k > edge) {
+          w[i] = W(l[i]);
+          if (low(w[i])) w[i] = 0;
+        } else if (k == edge) {
+          if (edge_kept && rank_eq < ties) w[i] = wedge;
+          ++rank_eq;
+        }
+      }
+      sum += w[i];
+    }
+    u64 run = warp_scan(sum);
+    const u64 step = __shfl_sync(0xffffffffu, run, 31);
+    run += start - sum;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      if (run <= target && run + w[i] > target) answer(id0 + i, w[i], total);
+      run += w[i];
+    }
+    start += step;
+    if (start > target) return;
+  }
+}
+
+constexpr int kSharedBytes = (int)((sizeof(Shared) + 15) / 16 * 16);
+constexpr int64_t kSliceBytes = 64 << 10;       // of a row in a CTA: two CTAs an SM
+constexpr int64_t kMostSliceBytes = 160 << 10;  // one
+
+template <typename T>
+int launch_sample(const SampleArgs& a, int64_t rows, cudaStream_t st) {
+  const int64_t bytes = a.vocab * (int64_t)sizeof(T) + 32;
+  // CTAs of a row: enough for the row to fit their shared memory, and to give
+  // every SM work when the rows are few, at least 512 ids each
+  int nc = 1;
+  while (nc < kMaxCtas && (bytes > nc * kSliceBytes || (rows * nc * 2 <= 148 && a.vocab >= nc * 1024)))
+    nc *= 2;
+  const int64_t per = (bytes / 16 + 2 + nc - 1) / nc * 16;
+  const bool cached = per <= kMostSliceBytes;
+  const int smem = kSharedBytes + (cached ? (int)per : 0);
+  auto* k = cached ? k_sample<T, true> : k_sample<T, false>;
+  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return (int)e;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(rows * nc));
+  cfg.blockDim = dim3(kNT);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = nc, at.val.clusterDim.y = 1, at.val.clusterDim.z = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return (int)cudaLaunchKernelEx(&cfg, k, a);
 }
 
 }  // namespace
@@ -237,7 +638,7 @@ extern "C" int mep_sample(int dtype, const void* logits, int64_t rows, int64_t v
   const char* op = "mep_sample";
   if (dtype != MEP_F32 && dtype != MEP_BF16)
     return serve_invalid(op, "dtype must be MEP_F32 or MEP_BF16");
-  if (rows < 0 || rows > 0x7fffffff) return serve_invalid(op, "rows out of range");
+  if (rows < 0 || rows > 0x7fffffff / kMaxCtas) return serve_invalid(op, "rows out of range");
   if (vocab < 1 || vocab > (1 << 24)) return serve_invalid(op, "vocab must be 1..2^24");
   if (stride < 0) return serve_invalid(op, "negative row stride");
   if (!temperature && !(temperature_all >= 0.f && temperature_all < INFINITY))
@@ -251,9 +652,8 @@ extern "C" int mep_sample(int dtype, const void* logits, int64_t rows, int64_t v
   const SampleArgs a{logits, vocab, stride, u, temperature, top_k, top_p, min_p, temperature_all,
                      top_k_all, top_p_all, min_p_all, tokens, logprobs};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (dtype == MEP_BF16)
-    k_sample<__nv_bfloat16><<<(unsigned)rows, 1024, 0, st>>>(a);
-  else
-    k_sample<float><<<(unsigned)rows, 1024, 0, st>>>(a);
+  const int rc = dtype == MEP_BF16 ? launch_sample<__nv_bfloat16>(a, rows, st)
+                                   : launch_sample<float>(a, rows, st);
+  if (rc) return serve_cuda(op, (cudaError_t)rc);
   return serve_launched(op);
 }

@@ -355,7 +355,9 @@ def test_attention_offsets_past_32_bits():
 def draw_rows(logits, u, temperature, top_k, top_p, min_p):
     tok, lp = sample_tokens(logits, u, temperature, top_k, top_p, min_p, return_logprobs=True)
     B = logits.shape[0]
-    pick = lambda x, i: x[i].item() if isinstance(x, torch.Tensor) else x  # noqa: E731
+    # numbers reach the kernel in fp32
+    pick = lambda x, i: x[i].item() if isinstance(x, torch.Tensor) else \
+        x if isinstance(x, int) else torch.tensor(x).item()  # noqa: E731
     rows, us = logits.float().cpu().tolist(), u.cpu().tolist()
     undecided = 0
     for i in range(B):
@@ -406,6 +408,26 @@ def test_sample_rows_of_their_own_and_strides():
         draw_rows(logits, u, t, k, p, m)
         wide = randn(g, V, B, dtype=dtype).T  # vocabulary not contiguous
         draw_rows(wide, u, t, k, p, m)
+
+
+@pytest.mark.parametrize("filt", [(1.0, 0, 1.0, 0.0), (3.0, 5000, 0.9, 0.0), (4.0, 0, 0.9, 1e-4),
+                                  (1.0, 20000, 1.0, 0.0), (9.0, 30000, 0.5, 0.0)], ids=str)
+def test_sample_wide_rows_and_nuclei(filt):
+    """Thousands of tokens kept, vocabularies past what a CTA keeps on chip."""
+    for V, dtype in ((40001, F32), (262147, BF), (700001, BF), (400003, F32)):
+        g = gen(V)
+        logits = randn(g, 2, V, dtype=dtype, std=2.0)
+        draw_rows(logits, torch.rand(2, generator=g, device="cuda"), *filt)
+    tied = torch.randint(0, 3, (4, 30011), generator=gen(1), device="cuda").float()
+    draw_rows(tied, torch.rand(4, generator=gen(2), device="cuda"), *filt)
+
+
+def test_sample_every_row_count():
+    """Row counts that change how many CTAs share a row."""
+    for B in (1, 9, 18, 37, 74, 150, 300):
+        g = gen(B)
+        logits = randn(g, B, 8200, dtype=BF, std=2.0)
+        draw_rows(logits, torch.rand(B, generator=g, device="cuda"), 0.9, 30, 0.9, 0.0)
 
 
 def test_sample_ties_take_the_lowest_ids():

@@ -442,6 +442,7 @@ __global__ void __launch_bounds__(kThreads) k_attn_part(const PartArgs p) {
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
           const int r = kr0 + i * 8 + g;
+          float d4[4] = {0.f, 0.f, 0.f, 0.f};  // added to s in fp32, see `fresh` below
           if constexpr (kScaled) {
             const uint32_t v = *reinterpret_cast<const uint32_t*>(
                 ks + r * X::kRow + X::k_chunk(r, (w / 4) * 4 + t4) * 16 + (w % 4) * 4);
@@ -450,8 +451,8 @@ __global__ void __launch_bounds__(kThreads) k_attn_part(const PartArgs p) {
                                    __float_as_uint(half_lo(hi)), __float_as_uint(half_hi(hi))};
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-              mma_tf32(s[i], e[k], b[2 * k], b[2 * k + 1]);
-              mma_tf32(s[i], h[k], b[2 * k], b[2 * k + 1]);
+              mma_tf32(d4, e[k], b[2 * k], b[2 * k + 1]);
+              mma_tf32(d4, h[k], b[2 * k], b[2 * k + 1]);
             }
           } else {
             const float4 v = *reinterpret_cast<const float4*>(ks + r * X::kRow +
@@ -461,11 +462,13 @@ __global__ void __launch_bounds__(kThreads) k_attn_part(const PartArgs p) {
             split_tf32(v.z, bh[2], bl[2]), split_tf32(v.w, bh[3], bl[3]);
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-              mma_tf32(s[i], h[k], bl[2 * k], bl[2 * k + 1]);
-              mma_tf32(s[i], e[k], bh[2 * k], bh[2 * k + 1]);
-              mma_tf32(s[i], h[k], bh[2 * k], bh[2 * k + 1]);
+              mma_tf32(d4, h[k], bl[2 * k], bl[2 * k + 1]);
+              mma_tf32(d4, e[k], bh[2 * k], bh[2 * k + 1]);
+              mma_tf32(d4, h[k], bh[2 * k], bh[2 * k + 1]);
             }
           }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[i][j] += d4[j];
         }
       }
     }
@@ -518,10 +521,12 @@ __global__ void __launch_bounds__(kThreads) k_attn_part(const PartArgs p) {
         s[i][j] = ex2(s[i][j] - base[j >> 1]);
         l[j >> 1] += s[i][j];
       }
+    if (!kF32) {
 #pragma unroll
-    for (int i = 0; i < OT; ++i)
+      for (int i = 0; i < OT; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) o[i][j] *= keep[j >> 1];
+        for (int j = 0; j < 4; ++j) o[i][j] *= keep[j >> 1];
+    }
     if (kScaled) {
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
@@ -573,6 +578,14 @@ __global__ void __launch_bounds__(kThreads) k_attn_part(const PartArgs p) {
         }
       }
     } else {
+      // The tensor cores cut the low bits of a product that joins a larger sum.
+      // fp32 results keep their precision with a fresh accumulator for each
+      // tile of keys (each 16 values of a score), added to the sum in fp32.
+      float fresh[OT][4];
+#pragma unroll
+      for (int i = 0; i < OT; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) fresh[i][j] = 0.f;
 #pragma unroll
       for (int k = 0; k < NT; ++k) {
         // keys 2 t4 and 2 t4 + 1 of each 8 are this thread's k indices
@@ -588,10 +601,10 @@ __global__ void __launch_bounds__(kThreads) k_attn_part(const PartArgs p) {
 #pragma unroll
             for (int e2 = 0; e2 < 4; ++e2) {
               const uint32_t c0 = e4m3x2_f16x2(b[e2] & 0xffff), c1 = e4m3x2_f16x2(b[e2] >> 16);
-              mma_tf32(o[2 * (n + e2)], e, __float_as_uint(half_lo(c0)), __float_as_uint(half_lo(c1)));
-              mma_tf32(o[2 * (n + e2)], h, __float_as_uint(half_lo(c0)), __float_as_uint(half_lo(c1)));
-              mma_tf32(o[2 * (n + e2) + 1], e, __float_as_uint(half_hi(c0)), __float_as_uint(half_hi(c1)));
-              mma_tf32(o[2 * (n + e2) + 1], h, __float_as_uint(half_hi(c0)), __float_as_uint(half_hi(c1)));
+              mma_tf32(fresh[2 * (n + e2)], e, __float_as_uint(half_lo(c0)), __float_as_uint(half_lo(c1)));
+              mma_tf32(fresh[2 * (n + e2)], h, __float_as_uint(half_lo(c0)), __float_as_uint(half_lo(c1)));
+              mma_tf32(fresh[2 * (n + e2) + 1], e, __float_as_uint(half_hi(c0)), __float_as_uint(half_hi(c1)));
+              mma_tf32(fresh[2 * (n + e2) + 1], h, __float_as_uint(half_hi(c0)), __float_as_uint(half_hi(c1)));
             }
           }
         } else {
@@ -603,12 +616,16 @@ __global__ void __launch_bounds__(kThreads) k_attn_part(const PartArgs p) {
             const float vb = *reinterpret_cast<const float*>(vs + rb * X::kRow + X::v_chunk(rb, d >> 2) * 16 + (d & 3) * 4);
             uint32_t ah, al, bh, bl;
             split_tf32(va, ah, al), split_tf32(vb, bh, bl);
-            mma_tf32(o[n], h, al, bl);
-            mma_tf32(o[n], e, ah, bh);
-            mma_tf32(o[n], h, ah, bh);
+            mma_tf32(fresh[n], h, al, bl);
+            mma_tf32(fresh[n], e, ah, bh);
+            mma_tf32(fresh[n], h, ah, bh);
           }
         }
       }
+#pragma unroll
+      for (int i = 0; i < OT; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[i][j] = o[i][j] * keep[j >> 1] + fresh[i][j];
     }
   }
   cp_wait<0>();

@@ -125,7 +125,7 @@ __device__ __forceinline__ void unpack(const uint4& v, float (&x)[8]) {
   }
 }
 template <typename T>
-__device__ __forceinline__ uint4 fetch(const T* row, int64_t id, int64_t vocab) {
+__device__ __forceinline__ uint4 fetch(const T* row, int id, int vocab) {
   constexpr int E = Vec<T>::E;
   if (id >= 0 && id + E <= vocab) return *reinterpret_cast<const uint4*>(row + id);
   __align__(16) T x[E];
@@ -183,9 +183,11 @@ __device__ void sort_desc(u64* x, int n) {
 // in order. Without a filter the weights are summed per warp, and the warp
 // whose share holds the target finds the token. With top_k or top_p a
 // histogram over the logits (counts, or masses) tells which bins can hold kept
-// tokens; when those are at most kList, as good as always, the leading CTA
-// sorts and finishes them alone, else the borders are found by histograms over
-// ever narrower key ranges. All sums are of integers: their order is free.
+// tokens. When those are at most kList the leading CTA sorts and finishes them
+// alone. Else it sorts the bin of the border, and the kept weights are summed
+// per warp as without a filter. A bin too large for that, and a second border
+// behind a wide top_k, are found by histograms over ever narrower key ranges.
+// All sums are of integers: their order is free.
 template <typename T, bool CACHED>
 __global__ void __launch_bounds__(kNT) k_sample(const SampleArgs a) {
   constexpr int E = Vec<T>::E;
@@ -194,7 +196,8 @@ __global__ void __launch_bounds__(kNT) k_sample(const SampleArgs a) {
   uint4* cache = reinterpret_cast<uint4*>(smem_raw + (sizeof(Shared) + 15) / 16 * 16);
   cg::cluster_group cluster = cg::this_cluster();
   const int nc = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-  const int64_t row = blockIdx.x / nc, V = a.vocab;
+  const int64_t row = blockIdx.x / nc;
+  const int V = (int)a.vocab;
   const int tid = threadIdx.x, lane = lane_id(), warp = warp_id();
   const T* x = static_cast<const T*>(a.logits) + row * a.stride;
   const float temp = a.temperature ? a.temperature[row] : a.temperature_s;
@@ -205,18 +208,18 @@ __global__ void __launch_bounds__(kNT) k_sample(const SampleArgs a) {
   // 16-byte pieces of the row on the grid of its addresses; piece p holds the
   // ids from p * E - shift on. This CTA has [p0, p1), this warp [w0, w1).
   const int shift = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
-  const int64_t pieces = (shift + V + E - 1) / E;
-  const int64_t per = (pieces + nc - 1) / nc;
-  const int64_t p0 = min(pieces, per * rank), p1 = min(pieces, p0 + per);
-  const int64_t per_w = ((p1 - p0 + kNW - 1) / kNW + 31) / 32 * 32;
-  const int64_t w0 = min(p1, p0 + per_w * warp), w1 = min(p1, w0 + per_w);
+  const int pieces = (shift + V + E - 1) / E;
+  const int per = (pieces + nc - 1) / nc;
+  const int p0 = min(pieces, per * rank), p1 = min(pieces, p0 + per);
+  const int per_w = ((p1 - p0 + kNW - 1) / kNW + 31) / 32 * 32;
+  const int w0 = min(p1, p0 + per_w * warp), w1 = min(p1, w0 + per_w);
 
-  auto piece = [&](int64_t p) -> uint4 {
+  auto piece = [&](int p) -> uint4 {
     return CACHED ? cache[p - p0] : fetch<T>(x, p * E - shift, V);
   };
   // f(l, id) for this warp's ids
   auto each = [&](auto f) {
-    for (int64_t p = w0 + lane; p < w1; p += 32) {
+    for (int p = w0 + lane; p < w1; p += 32) {
       float l[E];
       unpack(piece(p), l);
 #pragma unroll
@@ -230,14 +233,14 @@ __global__ void __launch_bounds__(kNT) k_sample(const SampleArgs a) {
   if (tid == 0) S.n_items = 0;
   u64 best = 0;
   float lmin = INFINITY;
-  for (int64_t p = w0 + lane; p < w1; p += 32) {
+  for (int p = w0 + lane; p < w1; p += 32) {
     const uint4 v = fetch<T>(x, p * E - shift, V);
     if (CACHED) cache[p - p0] = v;
     float l[E];
     unpack(v, l);
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-      const int64_t id = p * E - shift + i;
+      const int id = p * E - shift + i;
       if (id >= 0 && id < V) {
         const u64 c = (u64)key_of(l[i]) << 32 | (uint32_t)~(uint32_t)id;
         best = c > best ? c : best;
@@ -278,7 +281,7 @@ __global__ void __launch_bounds__(kNT) k_sample(const SampleArgs a) {
     return;
   }
   int bits = 0;
-  while ((1ll << bits) < V) ++bits;
+  while ((1 << bits) < V) ++bits;
   Weights W;
   W.lmax = logit_of(kmax);
   // 34 temperatures below the best a weight is 2^-49; lmax = inf leaves only
@@ -333,11 +336,13 @@ __global__ void __launch_bounds__(kNT) k_sample(const SampleArgs a) {
   if (by_k || by_p) {
     // ---- bins of equal width in the logit, best first
     const float range = fminf(W.lmax - W.lcut, W.lmax - lmin);
-    const float bscale = range > 0.f && range < INFINITY ? (float)kBins / range : 0.f;
+    const float bscale = range > 0.f && range < INFINITY ? (float)(kBins - 1) / range : 0.f;
+    // rounded to an integer in the low bits of 2^23 + x: x up to kBins - 1
     auto bin_of = [&](float l) {
-      return l == W.lmax ? 0 : (int)fminf((W.lmax - l) * bscale, (float)(kBins - 1));
+      const float x = l == W.lmax ? 0.f : fminf((W.lmax - l) * bscale, (float)(kBins - 1));
+      return __float_as_int(x + 8388608.f) & (kBins - 1);
     };
-    each([&](float l, int64_t) {
+    each([&](float l, int) {
       if (l >= W.lcut) {
         const int b = bin_of(l);
         atomicAdd(&S.cnt[b], 1u);
@@ -352,30 +357,45 @@ __global__ void __launch_bounds__(kNT) k_sample(const SampleArgs a) {
     const u64 cb = block_scan(c0 + c1, S.red, nall);
     const u64 mb = block_scan(m0 + m1, S.red2, mall);
     const double limit = (double)top_p * (double)mall;
-    // candidates: bins that begin before the border
-    if (tid == 0) S.r_bin = 0, S.r_cnt = S.tcnt[0];
+    // the bin of the border: the last that begins before it
+    if (tid == 0) S.r_bin = 0;
     __syncthreads();
 #pragma unroll
     for (int e = 1; e >= 0; --e) {
       const u64 cx = cb + (e ? c0 : 0), mx = mb + (e ? m0 : 0);
-      const bool in = by_k ? cx < (u64)top_k : (double)mx < limit;
+      const bool in = (e ? c1 : c0) && (by_k ? cx < (u64)top_k : (double)mx < limit);
       if (in) {
         atomicMax(&S.r_bin, (uint32_t)(2 * tid + e));
         break;
       }
     }
     __syncthreads();
-    if (S.r_bin / 2 == tid) S.r_cnt = (uint32_t)(cb + c0 + (S.r_bin & 1 ? c1 : 0));
+    const uint32_t last = S.r_bin;
+    if (last / 2 == tid) {  // candidates up to it, its own, and what lies above it
+      S.r_cnt = (uint32_t)(cb + c0 + (last & 1 ? c1 : 0));
+      S.r_hi = last & 1 ? c1 : c0;
+      S.r_above = by_k ? cb + (last & 1 ? c0 : 0) : mb + (last & 1 ? m0 : 0);
+    }
     __syncthreads();
-    const uint32_t last = S.r_bin, n = S.r_cnt;
-    if (n <= kList) {
-      // ---- candidates to the leading CTA
+    const uint32_t n = S.r_cnt, n_bin = S.r_hi;
+    const u64 above0 = S.r_above;
+    // all candidates to the leading CTA if it can finish them alone, else the
+    // border's bin alone, if it can sort that
+    const bool whole = n <= kList;
+    if (whole || n_bin <= kList) {
       Shared* lead = cluster.map_shared_rank(&S, 0);
-      each([&](float l, int64_t id) {
-        if (l >= W.lcut && (uint32_t)bin_of(l) <= last)
-          lead->item[atomicAdd(&lead->n_items, 1u)] = (u64)key_of(l) << 32 | (uint32_t)~(uint32_t)id;
+      const uint32_t from = whole ? 0 : last;
+      each([&](float l, int id) {
+        if (l >= W.lcut) {
+          const uint32_t b = bin_of(l);
+          if (b <= last && b >= from)
+            lead->item[atomicAdd(&lead->n_items, 1u)] =
+                (u64)key_of(l) << 32 | (uint32_t)~(uint32_t)id;
+        }
       });
       cluster.sync();
+    }
+    if (whole) {
       if (rank != 0) return;
       int n2 = 32;
       while (n2 < (int)n) n2 <<= 1;
@@ -427,6 +447,48 @@ __global__ void __launch_bounds__(kNT) k_sample(const SampleArgs a) {
       }
       return;
     }
+    // the key at the border of its sorted bin, and how many tokens of that key are kept
+    auto border_of_bin = [&](bool mass, double want) {
+      if (rank == 0) {
+        const int m = (int)S.n_items;
+        int n2 = 32;
+        while (n2 < m) n2 <<= 1;
+        for (int i = m + tid; i < n2; i += kNT) S.item[i] = 0;
+        sort_desc(S.item, n2);
+        u64 v[2], all;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int i = 2 * tid + e;
+          v[e] = i >= m ? 0 : mass ? W(logit_of((uint32_t)(S.item[i] >> 32))) : 1;
+        }
+        u64 run = above0 + block_scan(v[0] + v[1], S.red, all);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          // the last token that begins before the border (the first there is, if none does)
+          const int i = 2 * tid + e;
+          const u64 next = run + v[e];
+          if (i < m && ((double)run < want || i == 0) && (!((double)next < want) || i == m - 1)) {
+            const uint32_t k = (uint32_t)(S.item[i] >> 32);
+            int first = 0;  // the first of its key
+            for (int up = i; first < up;) {
+              const int mid = (first + up) / 2;
+              if ((uint32_t)(S.item[mid] >> 32) > k)
+                first = mid + 1;
+              else
+                up = mid;
+            }
+            for (int r = 0; r < nc; ++r) {
+              Shared* to = cluster.map_shared_rank(&S, r);
+              to->r_bin = k;
+              to->r_cnt = i + 1 - first;
+            }
+          }
+          run = next;
+        }
+        if (tid == 0) S.n_items = 0;
+      }
+      cluster.sync();
+    };
     // ---- too many candidates: borders by histograms over key ranges.
     // largest key whose count (mass) at or above it reaches `want`, and what is above it
     auto border = [&](bool mass, double want, u64& above_out) {
@@ -440,7 +502,7 @@ __global__ void __launch_bounds__(kNT) k_sample(const SampleArgs a) {
         cluster.sync();  // nobody still reads the last histogram
         for (int i = tid; i < kBins; i += kNT) S.cnt[i] = S.lo[i] = S.hi[i] = 0;
         __syncthreads();
-        each([&](float l, int64_t id) {
+        each([&](float l, int id) {
           const uint32_t k = key_of(l);
           if (id >= 0 && id < V && k >= lo && k <= hi) {
             const int b = kBins - 1 - (int)((k - lo) >> sh);  // best first
@@ -485,7 +547,7 @@ __global__ void __launch_bounds__(kNT) k_sample(const SampleArgs a) {
     // sums over the whole row of what f gives for each id
     auto row_sum = [&](auto f) {
       u64 s = 0, all;
-      each([&](float l, int64_t id) { s += f(l, id); });
+      each([&](float l, int id) { s += f(l, id); });
       block_scan(s, S.red, all);
       if (tid < nc) cluster.map_shared_rank(&S, tid)->best[rank] = all;
       cluster.sync();
@@ -496,21 +558,26 @@ __global__ void __launch_bounds__(kNT) k_sample(const SampleArgs a) {
     };
     double lim = limit;
     bool found = !by_p;
-    if (by_k) {
+    if (n_bin <= kList) {
+      border_of_bin(!by_k, by_k ? (double)top_k : limit);
+      edge = S.r_bin;
+      ties = S.r_cnt;
+      found = !by_k || !by_p;
+    } else if (by_k) {
       edge = border(false, (double)top_k, above);
       ties = (u64)top_k - above;
-      if (by_p) {
-        const uint32_t ed = edge;
-        const u64 m = row_sum([&](float l, int64_t) { return key_of(l) > ed ? W(l) : 0ull; });
-        const u64 eq = row_sum([&](float l, int64_t id) {
-          return (u64)(id >= 0 && id < V && key_of(l) == ed);
-        });
-        lim = (double)top_p * (double)(m + min(ties, eq) * W(logit_of(edge)));
-        if ((double)m < lim) {  // the border lies among the edge's own ties, or behind them
-          const u64 w1 = W(logit_of(edge));
-          if (w1 > 0) ties = min(ties, (u64)ceil((lim - (double)m) / (double)w1));
-          found = true;
-        }
+    }
+    if (by_k && by_p) {
+      const uint32_t ed = edge;
+      const u64 m = row_sum([&](float l, int) { return key_of(l) > ed ? W(l) : 0ull; });
+      const u64 eq = row_sum([&](float l, int id) {
+        return (u64)(id >= 0 && id < V && key_of(l) == ed);
+      });
+      lim = (double)top_p * (double)(m + min(ties, eq) * W(logit_of(edge)));
+      if ((double)m < lim) {  // the border lies among the edge's own ties, or behind them
+        const u64 w1 = W(logit_of(edge));
+        if (w1 > 0) ties = min(ties, (u64)ceil((lim - (double)m) / (double)w1));
+        found = true;
       }
     }
     if (!found) {
@@ -525,7 +592,7 @@ __global__ void __launch_bounds__(kNT) k_sample(const SampleArgs a) {
   auto low = [&](u64 w) { return (double)w < floor_p && w < 1ull << W.scale; };
   u64 mass = 0;
   uint32_t on_edge = 0;
-  each([&](float l, int64_t id) {
+  each([&](float l, int id) {
     const uint32_t k = key_of(l);
     if (k > edge) {
       const u64 w = W(l);
@@ -554,13 +621,13 @@ __global__ void __launch_bounds__(kNT) k_sample(const SampleArgs a) {
   u64 own = mass;
   if (edge_kept) own += min((u64)on_edge, ties > ties_before ? ties - ties_before : 0) * wedge;
   if (target < start || target >= start + own) return;
-  for (int64_t p = w0; p < w1; p += 32) {
+  for (int p = w0; p < w1; p += 32) {
     float l[E];
     const bool have = p + lane < w1;
     if (have) unpack(piece(p + lane), l);
     u64 w[E], sum = 0;
     uint32_t eq = 0;
-    const int64_t id0 = (p + lane) * E - shift;
+    const int id0 = (p + lane) * E - shift;
 #pragma unroll
     for (int i = 0; i < E; ++i)
       eq += have && id0 + i >= 0 && id0 + i < V && key_of(l[i]) == edge;

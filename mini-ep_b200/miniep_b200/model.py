@@ -17,7 +17,12 @@ computation runs on the device:
     combine and residual on the GPU).
 
 Attention uses torch's fused scaled-dot-product attention (GQA without
-repeating K/V; the memory-efficient, flash or math kernels). In bf16 the RoPE tables are cast to the model dtype before
+repeating K/V; the memory-efficient, flash or math kernels), or, for a
+``Shard(kernels=True)``, the decode-step operators (``decode.py``): rotation,
+optional head norms and the cache write in one kernel, attention that reads
+only the visible columns, a cache quantised to e4m3 (``quantized=True``) and a
+prefix that all rows share (``prefix=``, from ``Engine.build_prefix``). A
+``Sampler`` draws the next tokens in place of the greedy choice. In bf16 the RoPE tables are cast to the model dtype before
 use, as HF GraniteMoe does; the reference multiplies bf16 activations by fp32
 tables, which turns q and k into fp32 and leaves its bf16 attention without a
 common dtype. In fp32 both are the same arithmetic.
@@ -32,6 +37,8 @@ from pathlib import Path
 import torch
 import torch.nn.functional as F
 from torch.nn.attention import SDPBackend, sdpa_kernel
+
+from .decode import KVCache, SharedPrefix, cache_attention, norm_rope_store
 
 # torch's cuDNN attention backend queries the device properties on every call
 # (tens of ms of host time per call on this image), so attention is kept on
@@ -59,6 +66,9 @@ class ModelConfig:
     max_position_embeddings: int
     eos_token_id: int = 0
     pad_token_id: int = 0
+    # RMS norm of each query and key head before the rotation, with weights
+    # self_attn.q_norm / k_norm (head_dim,); not in the reference's model
+    qk_norm: bool = False
 
     @property
     def head_dim(self) -> int:
@@ -97,6 +107,8 @@ def weight_keys(cfg: ModelConfig) -> list[tuple[str, tuple]]:
                 (p + "self_attn.k_proj.weight", (hk * d, H)),
                 (p + "self_attn.v_proj.weight", (hk * d, H)),
                 (p + "self_attn.o_proj.weight", (H, hq * d)),
+                *([(p + "self_attn.q_norm.weight", (d,)), (p + "self_attn.k_norm.weight", (d,))]
+                  if cfg.qk_norm else []),
                 (p + "post_attention_layernorm.weight", (H,)),
                 (p + "block_sparse_moe.router.layer.weight", (E, H)),
                 (p + "block_sparse_moe.input_linear.weight", (E, 2 * I, H)),
@@ -154,10 +166,16 @@ class Rope:
 
 class Shard:
     """One rank's right-padded slice of the batch (worker.py:38-75) with its KV
-    cache preallocated on the device for `max_new` decode steps."""
+    cache preallocated on the device for `max_new` decode steps.
+
+    kernels: attention by the decode-step operators (CUDA devices). quantized:
+    the cache holds e4m3 (implies kernels). prefix: keys and values that come
+    before every row's prompt (implies kernels); the rows' positions start
+    behind it."""
 
     def __init__(self, prompts: list[list[int]], cfg: ModelConfig, max_new: int, device,
-                 dtype):
+                 dtype, *, kernels: bool = False, quantized: bool = False,
+                 prefix: SharedPrefix | None = None):
         if not prompts:
             raise ValueError("a shard needs at least one prompt (use a dummy prompt to idle)")
         self.B = len(prompts)
@@ -168,11 +186,23 @@ class Shard:
         for i, p in enumerate(prompts):
             self.input[i, :len(p)] = torch.tensor(p)
         self.input = self.input.to(device)
-        shape = (cfg.num_hidden_layers, self.B, cfg.num_key_value_heads, self.cap, cfg.head_dim)
-        # zeroed: columns not yet written are masked out of attention, and a
-        # masked zero contributes exactly nothing (a masked NaN would not)
-        self.k = torch.zeros(shape, device=device, dtype=dtype)
-        self.v = torch.zeros(shape, device=device, dtype=dtype)
+        self.prefix = prefix
+        self.offset = 0 if prefix is None else prefix.columns  # position of column 0
+        self.cache = None
+        if kernels or quantized or prefix is not None:
+            if self.offset + self.cap > cfg.max_position_embeddings:
+                raise ValueError(f"{self.offset} shared + {self.cap} own positions exceed "
+                                 f"max_position_embeddings ({cfg.max_position_embeddings})")
+            self.cache = KVCache.empty(cfg.num_hidden_layers, self.B, cfg.num_key_value_heads,
+                                       self.cap, cfg.head_dim, dtype, quantized, device)
+            self.k, self.v = self.cache.k, self.cache.v
+        else:
+            shape = (cfg.num_hidden_layers, self.B, cfg.num_key_value_heads, self.cap,
+                     cfg.head_dim)
+            # zeroed: columns not yet written are masked out of attention, and a
+            # masked zero contributes exactly nothing (a masked NaN would not)
+            self.k = torch.zeros(shape, device=device, dtype=dtype)
+            self.v = torch.zeros(shape, device=device, dtype=dtype)
         self.used = 0  # cache columns written
         self.decoded = 0
         self.generated = [[] for _ in range(self.B)]
@@ -196,7 +226,7 @@ class Shard:
         return self.key_valid[:, None, None, :self.used + 1]
 
     def decode_positions(self):
-        return (self.lengths + self.decoded).unsqueeze(1)
+        return (self.lengths + (self.offset + self.decoded)).unsqueeze(1)
 
 
 class DeviceModel:
@@ -226,6 +256,18 @@ class DeviceModel:
         q = (x @ self.w[p + "q_proj.weight"].T).view(B, T, cfg.num_attention_heads, d).transpose(1, 2)
         k = (x @ self.w[p + "k_proj.weight"].T).view(B, T, cfg.num_key_value_heads, d).transpose(1, 2)
         v = (x @ self.w[p + "v_proj.weight"].T).view(B, T, cfg.num_key_value_heads, d).transpose(1, 2)
+        qn, kn = self.w.get(p + "q_norm.weight"), self.w.get(p + "k_norm.weight")
+        if shard.cache is not None:
+            q = norm_rope_store(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2),
+                                self.rope.cos, self.rope.sin, positions, shard.cache, l, col0,
+                                q_norm=qn, k_norm=kn, eps=cfg.rms_norm_eps)
+            o = cache_attention(q, shard.cache, l, col0, cfg.attention_multiplier,
+                                lengths=shard.lengths, prompt_cols=shard.T, prefix=shard.prefix)
+            return o.view(B, T, H) @ self.w[p + "o_proj.weight"].T
+        if qn is not None:
+            q = rms_norm(q, qn, cfg.rms_norm_eps)
+        if kn is not None:
+            k = rms_norm(k, kn, cfg.rms_norm_eps)
         q, k = self.rope.apply(q, k, positions)
         if isinstance(col0, torch.Tensor):
             shard.k[l].index_copy_(2, col0, k)
@@ -286,9 +328,10 @@ class DeviceModel:
 
 
 class Engine:
-    """Lockstep prefill / greedy decode over one rank's shard
-    (worker.py:100-138). Every rank runs the same number of forwards; a rank
-    without prompts runs dummy forwards that add no expert load."""
+    """Lockstep prefill / decode over one rank's shard (worker.py:100-138).
+    Every rank runs the same number of forwards; a rank without prompts runs
+    dummy forwards that add no expert load. The next tokens are the greedy
+    ones, or what a ``Sampler`` draws where one is given."""
 
     def __init__(self, model: DeviceModel, reset_rr=None):
         self.model = model
@@ -296,22 +339,37 @@ class Engine:
         self.steps = 0
 
     @torch.no_grad()
-    def prefill(self, shard: Shard, dummy: bool = False):
+    def build_prefix(self, tokens: list[int], dummy: bool = False) -> SharedPrefix:
+        """Keys and values of a common prompt, computed once: shards built with
+        ``prefix=`` see it in front of every row. Every rank calls it (one
+        lockstep forward over a shard of one row)."""
+        shard = Shard([tokens], self.model.cfg, 0, self.model.device, self.model.dtype,
+                      kernels=True)
+        self.prefill(shard, dummy=dummy)
+        return SharedPrefix.from_cache(shard.cache, 0, shard.T)
+
+    @staticmethod
+    def _next(logits, sampler, u=None):
+        return logits.argmax(dim=-1) if sampler is None else sampler(logits, u)
+
+    @torch.no_grad()
+    def prefill(self, shard: Shard, dummy: bool = False, sampler=None):
         self.reset_rr()
         _, valid = shard.prefill_masks()
         if dummy:
             valid = torch.zeros_like(valid)
-        pos = torch.arange(shard.T, device=shard.input.device).unsqueeze(0).expand(shard.B, -1)
+        pos = torch.arange(shard.offset, shard.offset + shard.T,
+                           device=shard.input.device).unsqueeze(0).expand(shard.B, -1)
         logits = self.model.forward(shard.input, pos, shard, 0, None, valid,
                                     logits_at=shard.lengths - 1)
         shard.used = shard.T
         self.steps += 1
         shard.last_prefill_logits = logits[:, 0]
-        shard.last_tokens = logits[:, 0].argmax(dim=-1)
+        shard.last_tokens = self._next(logits[:, 0], sampler)
         return shard.last_tokens
 
     @torch.no_grad()
-    def decode_step(self, shard: Shard, active=None):
+    def decode_step(self, shard: Shard, active=None, sampler=None):
         self.reset_rr()
         toks = shard.last_tokens.tolist()
         act = None if active is None else active.tolist()
@@ -326,12 +384,12 @@ class Engine:
         shard.decoded += 1
         self.steps += 1
         shard.last_logits = logits[:, -1]
-        shard.last_tokens = shard.last_logits.argmax(dim=-1)
+        shard.last_tokens = self._next(shard.last_logits, sampler)
         return shard.last_tokens
 
     @torch.no_grad()
-    def decode_graphed(self, shard: Shard, steps: int, idle: bool = False):
-        """`steps` greedy decode steps of every row (all active), each one
+    def decode_graphed(self, shard: Shard, steps: int, idle: bool = False, sampler=None):
+        """`steps` decode steps of every row (all active), each one
         CUDA-graph replay: attention runs over every cache column with the
         unwritten ones masked on the device, and the cache column, the
         positions and the fed-back tokens are device tensors the graph
@@ -345,12 +403,15 @@ class Engine:
         m, dev = self.model, shard.input.device
         cols = torch.arange(shard.cap, device=dev)
         col = torch.full((1,), shard.used, dtype=torch.long, device=dev)
-        pos = (shard.lengths + shard.decoded).unsqueeze(1).clone()
+        pos = shard.decode_positions().clone()
         tok = shard.last_tokens.clone()
         gen = torch.zeros(shard.B, steps, dtype=torch.long, device=dev)
         j = torch.zeros(1, dtype=torch.long, device=dev)
         last = torch.empty(shard.B, m.cfg.vocab_size, dtype=m.dtype, device=dev)
         moe_valid = torch.zeros(shard.B, 1, dtype=torch.bool, device=dev) if idle else None
+        # the steps' uniform numbers are drawn ahead: the replays read row j
+        u = None if sampler is None else \
+            torch.stack([sampler.uniform(shard.B, device=dev) for _ in range(steps)])
 
         def step():
             self.reset_rr()
@@ -358,7 +419,7 @@ class Engine:
             mask = (shard.key_valid & (cols[None, :] <= col))[:, None, None, :]
             logits = m.forward(tok.unsqueeze(1), pos, shard, col, mask, moe_valid)
             last.copy_(logits[:, -1])
-            tok.copy_(last.argmax(dim=-1))
+            tok.copy_(self._next(last, sampler, None if u is None else u.index_select(0, j)[0]))
             col.add_(1)
             pos.add_(1)
             j.add_(1)
@@ -380,14 +441,14 @@ class Engine:
         shard.last_tokens = tok
         return tok
 
-    def generate(self, shard: Shard, max_new: int, dummy: bool = False):
+    def generate(self, shard: Shard, max_new: int, dummy: bool = False, sampler=None):
         """Prefill then `max_new` decode steps; returns (generated ids per row,
         positions processed, seconds). Positions follow worker.py:214-217:
         valid prompt positions plus one per row per decode step."""
         t0 = time.perf_counter()
-        self.prefill(shard, dummy=dummy)
+        self.prefill(shard, dummy=dummy, sampler=sampler)
         for _ in range(max_new):
-            self.decode_step(shard)
+            self.decode_step(shard, sampler=sampler)
         if self.model.device.type == "cuda":
             torch.cuda.synchronize(self.model.device)
         dt = time.perf_counter() - t0

@@ -25,48 +25,50 @@ constexpr float kE4M3Max = 448.f;
 // would come near the end of the fp32 range
 constexpr float kTinyRow = 7.888609e-31f;  // 2^-100
 
-// 8 consecutive values of a row
+// 4 consecutive values of a row, as loaded and in fp32
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&x)[8]);
-template <>
-__device__ __forceinline__ void load8<float>(const float* p, float (&x)[8]) {
-  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-  x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-}
-template <>
-__device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16* p, float (&x)[8]) {
-  const uint4 v = *reinterpret_cast<const uint4*>(p);
-  const uint32_t u[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    x[2 * i] = __uint_as_float(u[i] << 16);
-    x[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+struct Raw4 {
+  uint2 v;
+  __device__ void load(const T* p) { v = *reinterpret_cast<const uint2*>(p); }
+  __device__ void get(float* x) const {
+    x[0] = __uint_as_float(v.x << 16), x[1] = __uint_as_float(v.x & 0xffff0000u);
+    x[2] = __uint_as_float(v.y << 16), x[3] = __uint_as_float(v.y & 0xffff0000u);
   }
+};
+template <>
+struct Raw4<float> {
+  float4 v;
+  __device__ void load(const float* p) { v = *reinterpret_cast<const float4*>(p); }
+  __device__ void get(float* x) const { x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w; }
+};
+template <typename T>
+__device__ __forceinline__ void load4(const T* p, float* x) {
+  Raw4<T> r;
+  r.load(p);
+  r.get(x);
+}
+__device__ __forceinline__ void store4(float* p, const float* x) {
+  *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+}
+__device__ __forceinline__ uint32_t bf16x2(float a, float b) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ void store4(__nv_bfloat16* p, const float* x) {
+  *reinterpret_cast<uint2*>(p) = make_uint2(bf16x2(x[0], x[1]), bf16x2(x[2], x[3]));
+}
+__device__ __forceinline__ void store4(__nv_fp8_storage_t* p, const float* x) {
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x[0], x[1]), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(x[2], x[3]), __NV_SATFINITE, __NV_E4M3);
+  *reinterpret_cast<uint32_t*>(p) = lo | hi << 16;
 }
 __device__ __forceinline__ void store8(float* p, const float (&x)[8]) {
-  reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
-  reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+  store4(p, x);
+  store4(p + 4, x + 4);
 }
 __device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&x)[8]) {
-  uint32_t u[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const __nv_bfloat162 b = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
-    u[i] = *reinterpret_cast<const uint32_t*>(&b);
-  }
-  *reinterpret_cast<uint4*>(p) = make_uint4(u[0], u[1], u[2], u[3]);
-}
-__device__ __forceinline__ void store8(__nv_fp8_storage_t* p, const float (&x)[8]) {
-  uint32_t u[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(x[4 * i], x[4 * i + 1]),
-                                                 __NV_SATFINITE, __NV_E4M3);
-    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(x[4 * i + 2], x[4 * i + 3]),
-                                                 __NV_SATFINITE, __NV_E4M3);
-    u[i] = lo | hi << 16;
-  }
-  *reinterpret_cast<uint2*>(p) = make_uint2(u[0], u[1]);
+  *reinterpret_cast<uint4*>(p) = make_uint4(bf16x2(x[0], x[1]), bf16x2(x[2], x[3]),
+                                            bf16x2(x[4], x[5]), bf16x2(x[6], x[7]));
 }
 
 struct StoreArgs {
@@ -90,15 +92,28 @@ struct StoreArgs {
   const int64_t* col_dev;
 };
 
-// sum / maximum over the `n` lanes of a row's group (lane `j` of it), in every lane
+// sum / maximum over a row's group of lanes, in every lane. L: lanes of a
+// group when that is a power of two, else 0 (n lanes, this one the j-th).
+template <int L>
 __device__ __forceinline__ float group_sum(float x, int j, int n, int first) {
+  if (L) {
+#pragma unroll
+    for (int o = 1; o < L; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+    return x;
+  }
   for (int o = 1; o < n; o <<= 1) {
     const float y = __shfl_down_sync(0xffffffffu, x, o);
     if (j + o < n) x += y;
   }
   return __shfl_sync(0xffffffffu, x, first);
 }
+template <int L>
 __device__ __forceinline__ float group_max(float x, int j, int n, int first) {
+  if (L) {
+#pragma unroll
+    for (int o = 1; o < L; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+    return x;
+  }
   for (int o = 1; o < n; o <<= 1) {
     const float y = __shfl_down_sync(0xffffffffu, x, o);
     if (j + o < n) x = fmaxf(x, y);
@@ -106,115 +121,178 @@ __device__ __forceinline__ float group_max(float x, int j, int n, int first) {
   return __shfl_sync(0xffffffffu, x, first);
 }
 
-// D/8 lanes per head row, 32 / (D/8) rows a warp. T: model type, C: cache
-// element, W: type of the rotation tables.
-template <typename T, typename C, typename W>
-__global__ void __launch_bounds__(256) k_norm_rope_store(const StoreArgs a) {
-  const int D = a.head_dim, L = D >> 3, half = L >> 1;
+// A lane holds values 4j..4j+3 of a head row and the same of its other half,
+// so that the rotation needs no exchange; D/8 lanes a row, 32 / (D/8) rows a
+// pass of a warp, all q, all k or all v. A warp takes `share` passes of one
+// token, the next pass's rows loaded while it works on this one's, the token's
+// table rows in registers throughout. T: model type, C: cache element, W: type
+// of the tables, LT: D/8 where that is a power of two, else 0.
+template <typename T, typename C, typename W, int LT>
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 3)
+    k_norm_rope_store(const StoreArgs a, int share, int parts) {
+  const int D = a.head_dim, L = LT ? LT : D >> 3, half = D >> 1;
   const int per_warp = 32 / L, lane = lane_id();
   const int sub = lane / L, j = lane - sub * L, first = sub * L;
-  const int heads = a.q_heads + 2 * a.kv_heads;
-  const int64_t rows = a.batch * a.tokens * heads;
-  const int64_t row = ((int64_t)blockIdx.x * (blockDim.x >> 5) + warp_id()) * per_warp + sub;
-  const bool live = sub < per_warp && row < rows;
-  const int64_t tok = live ? row / heads : 0;
-  const int head = live ? (int)(row - tok * heads) : 0;
+  const int qp = (a.q_heads + per_warp - 1) / per_warp;
+  const int kp = (a.kv_heads + per_warp - 1) / per_warp;
+  const int64_t item = (int64_t)blockIdx.x * (blockDim.x >> 5) + warp_id();
+  const int64_t tok = item / parts;
+  if (tok >= a.batch * a.tokens) return;
+  const int p0 = (int)(item - tok * parts) * share, p1 = min(qp + 2 * kp, p0 + share);
   const int64_t b = tok / a.tokens, t = tok - b * a.tokens;
-  const int kind = head < a.q_heads ? 0 : head < a.q_heads + a.kv_heads ? 1 : 2;
-  const int h = kind == 0 ? head : kind == 1 ? head - a.q_heads : head - a.q_heads - a.kv_heads;
-  const HeadsView& in = kind == 0 ? a.q : kind == 1 ? a.k : a.v;
-  float x[8] = {};
-  if (live) load8<T>(static_cast<const T*>(in.p) + b * in.sb + t * in.st + h * in.sh + j * 8, x);
-  const void* nw = kind == 0 ? a.q_norm : kind == 1 ? a.k_norm : nullptr;
-  if (a.q_norm || a.k_norm) {
-    float ss = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) ss += x[i] * x[i];
-    ss = group_sum(ss, j, L, first);
-    if (nw && live) {
-      const float r = rsqrtf(ss / (float)D + a.eps);
-      float w[8];
-      load8<T>(static_cast<const T*>(nw) + j * 8, w);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = x[i] * r * w[i];
+
+  // pass p: its kind (0 q, 1 k, 2 v), this lane's head of it
+  auto kind_of = [&](int p) { return p < qp ? 0 : p < qp + kp ? 1 : 2; };
+  auto head_of = [&](int p, int kind) {
+    return (p - (kind == 0 ? 0 : kind == 1 ? qp : qp + kp)) * per_warp + sub;
+  };
+  auto live = [&](int kind, int h) {
+    return sub < per_warp && h < (kind == 0 ? a.q_heads : a.kv_heads);
+  };
+  Raw4<T> raw[2];
+  auto load = [&](int p) {
+    const int kind = kind_of(p), h = head_of(p, kind);
+    if (live(kind, h)) {
+      const HeadsView& in = kind == 0 ? a.q : kind == 1 ? a.k : a.v;
+      const T* x = static_cast<const T*>(in.p) + b * in.sb + t * in.st + h * in.sh + 4 * j;
+      raw[0].load(x);
+      raw[1].load(x + half);
     }
-  }
-  const int other = first + (j < half ? j + half : j - half);
-  float y[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) y[i] = __shfl_sync(0xffffffffu, x[i], other & 31);
-  if (live && kind < 2) {
+  };
+  load(p0);
+
+  const int64_t col = (a.col_dev ? *a.col_dev : a.col) + t;
+  const bool stored = col >= 0 && col < a.capacity;
+  float c[8], s[8];
+  if (p0 < qp + kp) {
     const int64_t p = a.positions[b * a.psb + t * a.pst];
     if (p >= 0 && p < a.table_rows) {
-      float c[8], s[8];
-      load8<W>(static_cast<const W*>(a.cos) + p * D + j * 8, c);
-      load8<W>(static_cast<const W*>(a.sin) + p * D + j * 8, s);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = x[i] * c[i] + (j < half ? -y[i] : y[i]) * s[i];
+      const W* cw = static_cast<const W*>(a.cos) + p * D + 4 * j;
+      const W* sw = static_cast<const W*>(a.sin) + p * D + 4 * j;
+      load4<W>(cw, c), load4<W>(cw + half, c + 4);
+      load4<W>(sw, s), load4<W>(sw + half, s + 4);
     } else {  // no such position: NaN rather than a read outside the tables
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = __int_as_float(0x7fffffff);
+      for (int i = 0; i < 8; ++i) c[i] = s[i] = __int_as_float(0x7fffffff);
     }
   }
-  if (live && kind == 0) {
-    store8(static_cast<T*>(a.q_out) + (tok * a.q_heads + h) * D + j * 8, x);
-  }
-  const int64_t col = (a.col_dev ? *a.col_dev : a.col) + t;
-  const bool keep = live && kind > 0 && col >= 0 && col < a.capacity;
-  const int64_t at = ((b * a.kv_heads + h) * a.capacity + col);
-  if (sizeof(C) == 1) {
-    float m = 0.f;
+  for (int p = p0; p < p1; ++p) {
+    const int kind = kind_of(p), h = head_of(p, kind);
+    const bool on = live(kind, h);
+    float x[8];
+    raw[0].get(x);
+    raw[1].get(x + 4);
+    if (!on)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(x[i]));
-    m = group_max(m, j, L, first);
-    const bool some = m >= kTinyRow;
-    const float inv = some ? kE4M3Max / m : 0.f;
-    if (keep) {
+      for (int i = 0; i < 8; ++i) x[i] = 0.f;
+    if (p + 1 < p1) load(p + 1);
+    if (kind < 2) {
+      const T* nw = static_cast<const T*>(kind == 0 ? a.q_norm : a.k_norm);
+      if (nw) {
+        float ss = 0.f, w[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ss += x[i] * x[i];
+        ss = group_sum<LT>(ss, j, L, first);
+        const float r = rsqrtf(ss / (float)D + a.eps);
+        const int at = sub < per_warp ? 4 * j : 0;
+        load4<T>(nw + at, w), load4<T>(nw + at + half, w + 4);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = x[i] * r * w[i];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float lo = x[i], hi = x[i + 4];
+        x[i] = lo * c[i] - hi * s[i];
+        x[i + 4] = hi * c[i + 4] + lo * s[i + 4];
+      }
+    }
+    if (kind == 0) {
+      if (on) {
+        T* out = static_cast<T*>(a.q_out) + (tok * a.q_heads + h) * D + 4 * j;
+        store4(out, x);
+        store4(out + half, x + 4);
+      }
+      continue;
+    }
+    const int64_t at = (b * a.kv_heads + h) * a.capacity + col;
+    if (sizeof(C) == 1) {
+      float m = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(x[i]));
+      m = group_max<LT>(m, j, L, first);
+      const bool some = m >= kTinyRow;
+      const float inv = some ? kE4M3Max / m : 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) x[i] *= inv;
-      if (j == 0) (kind == 1 ? a.ks : a.vs)[at] = some ? m / kE4M3Max : 0.f;
+      if (on && stored && j == 0) (kind == 1 ? a.ks : a.vs)[at] = some ? m / kE4M3Max : 0.f;
+    }
+    if (on && stored) {
+      C* out = static_cast<C*>(kind == 1 ? a.kc : a.vc) + at * D + 4 * j;
+      store4(out, x);
+      store4(out + half, x + 4);
     }
   }
-  if (keep) store8(static_cast<C*>(kind == 1 ? a.kc : a.vc) + at * D + j * 8, x);
 }
 
+template <typename T, typename C, typename W, int LT>
+void launch_store_l(const StoreArgs& a, cudaStream_t st) {
+  const int per_warp = 32 / (a.head_dim / 8);
+  const int passes = (a.q_heads + per_warp - 1) / per_warp + 2 * ((a.kv_heads + per_warp - 1) / per_warp);
+  const int64_t tokens = a.batch * a.tokens;
+  // few tokens: one pass a warp, for the latency; many (32 warps on each of
+  // 148 SMs, four passes each): up to 12, which share the table rows
+  const int share = tokens * passes < (int64_t)148 * 32 * 4 ? 1 : passes <= 12 ? passes : (passes + 1) / 2;
+  const int parts = (passes + share - 1) / share;
+  const int warps = share == 1 ? 4 : 8;
+  k_norm_rope_store<T, C, W, LT>
+      <<<(unsigned)((tokens * parts + warps - 1) / warps), warps * 32, 0, st>>>(a, share, parts);
+}
+template <typename T, typename C, typename W>
+void launch_store_w(const StoreArgs& a, cudaStream_t st) {
+  if (a.head_dim == 64)
+    launch_store_l<T, C, W, 8>(a, st);
+  else if (a.head_dim == 128)
+    launch_store_l<T, C, W, 16>(a, st);
+  else
+    launch_store_l<T, C, W, 0>(a, st);
+}
 template <typename T, typename C>
 void launch_store(const StoreArgs& a, int table_f32, cudaStream_t st) {
-  const int per_warp = 32 / (a.head_dim / 8);
-  const int64_t rows = a.batch * a.tokens * (a.q_heads + 2 * a.kv_heads);
-  const unsigned grid = (unsigned)((rows + 8 * per_warp - 1) / (8 * per_warp));
   if (table_f32)
-    k_norm_rope_store<T, C, float><<<grid, 256, 0, st>>>(a);
+    launch_store_w<T, C, float>(a, st);
   else
-    k_norm_rope_store<T, C, T><<<grid, 256, 0, st>>>(a);
+    launch_store_w<T, C, T>(a, st);
 }
 
 // columns [start, start + n) of a quantised layer, code * scale rounded once:
-// 8 values a thread, K and V in one launch (blockIdx.y)
+// 16 codes a thread (one 16-byte load), K and V of a head (blockIdx.y, z)
 template <typename T>
-__global__ void __launch_bounds__(256) k_kv_read(CacheView c, int64_t heads, int D, int64_t start,
-                                                 int64_t n, T* k_out, T* v_out) {
-  const int per_row = D >> 3;
-  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= heads * n * per_row) return;
-  const int64_t row = i / per_row;
-  const int j = (int)(i - row * per_row);
-  const int64_t bh = row / n;
-  const int64_t at = bh * c.capacity + start + (row - bh * n);
-  const uint8_t* codes = static_cast<const uint8_t*>(blockIdx.y ? c.v : c.k);
-  const float scale = (blockIdx.y ? c.vs : c.ks)[at];
-  const uint2 u = *reinterpret_cast<const uint2*>(codes + at * D + j * 8);
-  float x[8];
+__global__ void __launch_bounds__(256) k_kv_read(CacheView c, int D, int64_t start, int64_t n,
+                                                 T* k_out, T* v_out) {
+  const unsigned per_row = (unsigned)D >> 4;
+  const unsigned bh = blockIdx.z, kv = blockIdx.y;
+  const uint8_t* codes = static_cast<const uint8_t*>(kv ? c.v : c.k);
+  const float* scales = (kv ? c.vs : c.ks) + bh * c.capacity + start;
+  codes += (bh * c.capacity + start) * D;
+  T* out = (kv ? v_out : k_out) + bh * n * D;
+  const unsigned pieces = (unsigned)n * per_row;
+  for (unsigned i = blockIdx.x * blockDim.x + threadIdx.x; i < pieces;
+       i += gridDim.x * blockDim.x) {
+    const float scale = scales[i / per_row];
+    const uint4 u = reinterpret_cast<const uint4*>(codes)[i];
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    float x[2][8];
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const uint32_t w = q < 2 ? u.x : u.y;
-    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(
-        (__nv_fp8x2_storage_t)(q & 1 ? w >> 16 : w & 0xffff), __NV_E4M3);
-    const float2 f = __half22float2(__half2(h));
-    x[2 * q] = f.x * scale;
-    x[2 * q + 1] = f.y * scale;
+    for (int q = 0; q < 8; ++q) {
+      const uint32_t two = q & 1 ? w[q >> 1] >> 16 : w[q >> 1] & 0xffff;
+      const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, __NV_E4M3);
+      const float2 f = __half22float2(__half2(h));
+      x[q >> 2][(2 * q) & 7] = f.x * scale;
+      x[q >> 2][(2 * q + 1) & 7] = f.y * scale;
+    }
+    store8(out + (size_t)i * 16, x[0]);
+    store8(out + (size_t)i * 16 + 8, x[1]);
   }
-  store8((blockIdx.y ? v_out : k_out) + row * D + j * 8, x);
 }
 
 }  // namespace
@@ -282,16 +360,21 @@ extern "C" int mep_kv_read(int dtype, int64_t batch, int kv_heads, int head_dim,
     return serve_invalid(op, "null tensor");
   if (!aligned16(k_cache) || !aligned16(v_cache) || !aligned16(k_out) || !aligned16(v_out))
     return serve_invalid(op, "tensors must start on a 16-byte boundary");
-  const int64_t heads = batch * kv_heads, n = heads * columns * (head_dim / 8);
-  const dim3 grid((unsigned)((n + 255) / 256), 2);
+  const int64_t heads = batch * kv_heads;
+  if (heads > 65535) return serve_invalid(op, "batch * kv_heads up to 65535");
+  if (columns * head_dim > 0xffffffffll) return serve_invalid(op, "columns * head_dim up to 2^32 - 1");
+  const int64_t pieces = columns * (head_dim / 16);
+  const int64_t most = 148 * 64 / heads + 1;  // CTAs of a head: some 64 an SM in all
+  const int64_t want = (pieces + 255) / 256;
+  const dim3 grid((unsigned)(want < most ? want : most), 2, (unsigned)heads);
   const CacheView c{k_cache, v_cache, k_scale, v_scale, capacity};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == MEP_BF16)
-    k_kv_read<__nv_bfloat16><<<grid, 256, 0, st>>>(c, heads, head_dim, start, columns,
+    k_kv_read<__nv_bfloat16><<<grid, 256, 0, st>>>(c, head_dim, start, columns,
                                                    static_cast<__nv_bfloat16*>(k_out),
                                                    static_cast<__nv_bfloat16*>(v_out));
   else
-    k_kv_read<float><<<grid, 256, 0, st>>>(c, heads, head_dim, start, columns,
+    k_kv_read<float><<<grid, 256, 0, st>>>(c, head_dim, start, columns,
                                            static_cast<float*>(k_out), static_cast<float*>(v_out));
   return serve_launched(op);
 }

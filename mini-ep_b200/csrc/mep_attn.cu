@@ -13,6 +13,7 @@
 // into splits that run on different SMs; their partial results (fp32 sums, the
 // maximum in base 2) meet in k_attn_join.
 #include <cstdint>
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 
@@ -21,6 +22,8 @@
 
 namespace mep {
 namespace {
+
+namespace cg = cooperative_groups;
 
 struct AttnArgs {
   int64_t batch, tokens;
@@ -106,8 +109,9 @@ __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) 
   lo = tf32(x - __uint_as_float(hi));
 }
 __device__ __forceinline__ uint32_t e4m3x2_f16x2(uint32_t two) {
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, __NV_E4M3);
-  return (uint32_t)h.x | (uint32_t)h.y << 16;
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((unsigned short)two));
+  return r;
 }
 __device__ __forceinline__ float half_lo(uint32_t h2) {
   return __half2float(__ushort_as_half((unsigned short)(h2 & 0xffff)));
@@ -135,29 +139,31 @@ __device__ __forceinline__ float quad_sum(float x) {
 // The columns that rows of one matrix see, as one run of indices j in [0, n):
 // columns [0, n1), then those from `skip` columns further on.
 struct Span {
-  int64_t n, n1, skip;
-  __device__ int64_t column(int64_t j) const { return j < n1 ? j : j + skip; }
+  int n, n1, skip;
+  __device__ int column(int j) const { return j < n1 ? j : j + skip; }
 };
 
 // Geometry of a launch. Rows of a matrix: own columns, the tokens * group
 // queries of one batch row (matrix index = batch row); prefix, those of the
-// whole batch (one matrix). A partial result of row r of matrix i is slot
-// [split][(i * rows + r)'s output row].
+// whole batch (one matrix). A partial result is slot [split][output row].
 struct PartArgs {
   AttnArgs a;
   int group;             // query heads of a key/value head
-  int64_t rows;          // rows of a matrix
+  int rows;              // rows of a matrix
   int row_tiles, splits;
+  int joined;            // the splits are a cluster, which joins them and writes `out`
+  int extra;             // partial results of others that are joined with these
   int64_t out_rows;      // batch * tokens * q_heads
-  float* part_o;         // [splits][out_rows][head_dim], or null: write `out`
-  float2* part_ml;       // [splits][out_rows]: maximum (base 2), sum
+  float* part_o;         // [extra + splits][out_rows][head_dim]
+  float2* part_ml;       // [extra + splits][out_rows]: maximum (base 2), sum
 };
 
 // The kernel for one (element types, padded head width, warp layout).
 // KS (key split): the four warps share 16 rows and take a quarter of each tile
 // of keys each, for matrices of few rows, where the keys' bytes bound it: a
-// warp streams its own keys and meets the others only at the end. Otherwise
-// each warp has 16 of 64 rows and every key of the tile.
+// warp streams its own keys and meets the others only at the end; a cluster of
+// up to 8 CTAs, one a split, then joins its sums over distributed shared
+// memory. Otherwise each warp has 16 of 64 rows and every key of the tile.
 template <typename QT, typename CT, int DP, bool KS>
 struct Tile {
   static constexpr int kElt = sizeof(CT);
@@ -176,7 +182,7 @@ struct Tile {
   // registers), rows 4 floats apart in the banks
   static constexpr int kQRow = DP + 4;
   static constexpr int kQBytes = kF32 ? kRows * kQRow * 4 : 0;
-  static constexpr int kJoin = KS ? 4 * 16 * DP * 4 + 4 * 16 * 8 : 0;
+  static constexpr int kJoin = KS ? 5 * 16 * (DP * 4 + 8) : 0;
   static constexpr int kBody = kStages * kStageBytes + kQBytes;
   static constexpr int kSmem = kBody > kJoin ? kBody : kJoin;
   // place of 16-byte chunk c of staged row r, so that the accesses of a warp
@@ -199,77 +205,91 @@ __global__ void __launch_bounds__(kThreads) k_attn_part(const PartArgs p) {
   extern __shared__ __align__(128) unsigned char smem[];
   const AttnArgs& a = p.a;
   const int lane = lane_id(), warp = warp_id(), g = lane >> 2, t4 = lane & 3;
-  const int D = a.head_dim;
+  const int D = a.head_dim, tokens = (int)a.tokens;
   const int kh = blockIdx.y;
   const int split = blockIdx.x % p.splits;
-  const int64_t tile_id = blockIdx.x / p.splits;
-  const int rt = (int)(tile_id % p.row_tiles);
-  const int64_t mat = tile_id / p.row_tiles;  // batch row (own columns)
-  const int64_t r0 = (int64_t)rt * X::kRows;
-  const int64_t rN = min(r0 + X::kRows, p.rows);  // rows of this CTA: [r0, rN)
+  const int tile_id = blockIdx.x / p.splits;
+  const int rt = tile_id % p.row_tiles;
+  const int mat = tile_id / p.row_tiles;  // batch row (own columns)
+  const int r0 = rt * X::kRows;
+  const int rN = min(r0 + X::kRows, p.rows);  // rows of this CTA: [r0, rN)
 
-  // row r of the matrix: its query and its output row
-  auto query_of = [&](int64_t r, int64_t& b, int64_t& t, int& h) {
-    const int64_t bt = r / p.group;
-    h = kh * p.group + (int)(r - bt * p.group);
-    b = PREFIX ? bt / a.tokens : mat;
-    t = PREFIX ? bt - b * a.tokens : bt;
+  // row r of the matrix: its query, and its output row
+  auto query_of = [&](int r, int& b, int& t, int& h) {
+    const int bt = r / p.group;
+    h = kh * p.group + (r - bt * p.group);
+    b = PREFIX ? bt / tokens : mat;
+    t = PREFIX ? bt - b * tokens : bt;
   };
-  auto out_row = [&](int64_t r) {
-    int64_t b, t;
-    int h;
+  auto query_ptr = [&](int r) {
+    int b, t, h;
     query_of(r, b, t, h);
-    return (b * a.tokens + t) * a.q_heads + h;
+    return static_cast<const QT*>(a.q.p) + b * a.q.sb + t * a.q.st + h * a.q.sh;
+  };
+  auto out_row = [&](int r) {
+    int b, t, h;
+    query_of(r, b, t, h);
+    return ((int64_t)b * tokens + t) * a.q_heads + h;
   };
 
   // ---- the columns these rows see
   Span span;
   const int64_t col = PREFIX ? 0 : a.col_dev ? *a.col_dev : a.col;
   if (PREFIX) {
-    span = {a.prefix_cols, a.prefix_cols, 0};
+    span = {(int)a.prefix_cols, (int)a.prefix_cols, 0};
   } else {
-    const int64_t tmax = (rN - 1) / p.group;
+    const int tmax = (rN - 1) / p.group;
     const int64_t end = max((int64_t)0, min(col + tmax + 1, a.c.capacity));
     int64_t len = a.lengths ? max((int64_t)0, a.lengths[mat]) : end;
     if (len >= a.prompt_cols) len = end;
-    span.n1 = min(len, end);
-    const int64_t more = end - max(a.prompt_cols, span.n1);
-    span.skip = a.prompt_cols - span.n1;
-    span.n = span.n1 + (span.n1 < end && more > 0 ? more : 0);
+    const int64_t n1 = min(len, end);
+    const int64_t more = end - max(a.prompt_cols, n1);
+    span.n1 = (int)n1;
+    span.skip = n1 < end && more > 0 ? (int)(a.prompt_cols - n1) : 0;
+    span.n = (int)(n1 + (n1 < end && more > 0 ? more : 0));
   }
   // this split's share of them, in whole tiles
-  const int64_t tiles = (span.n + X::kKeys - 1) / X::kKeys;
-  const int64_t tile0 = tiles * split / p.splits, tile1 = tiles * (split + 1) / p.splits;
+  const int tiles = (span.n + X::kKeys - 1) / X::kKeys;
+  const int tile0 = (int)((int64_t)tiles * split / p.splits);
+  const int tile1 = (int)((int64_t)tiles * (split + 1) / p.splits);
 
-  const int64_t head_row = PREFIX ? kh * a.prefix_cols : (mat * a.kv_heads + kh) * a.c.capacity;
-  const unsigned char* kbase =
-      static_cast<const unsigned char*>(PREFIX ? a.kp : a.c.k) + head_row * D * X::kElt;
-  const unsigned char* vbase =
-      static_cast<const unsigned char*>(PREFIX ? a.vp : a.c.v) + head_row * D * X::kElt;
-  const int chunks = D * X::kElt / 16;  // 16-byte pieces of a row
-
+  const int64_t head_row = PREFIX ? (int64_t)kh * a.prefix_cols
+                                  : ((int64_t)mat * a.kv_heads + kh) * a.c.capacity;
+  const int row_bytes = D * X::kElt;
   // ---- staging: 16-byte copies of the tile's rows, zeros past the span
-  // (rows that nobody sees are never read, whatever they hold)
-  auto stage = [&](int64_t tile) {
-    unsigned char* s = smem + (tile % X::kStages) * X::kStageBytes;
-    const int first = KS ? warp * N : 0;
-    const int who = KS ? lane : threadIdx.x, step = KS ? 32 : kThreads;
-    for (int i = who; i < N * chunks; i += step) {
-      const int r = first + i / chunks, c = i % chunks;
-      const int64_t j = tile * X::kKeys + r;
-      const bool real = j < span.n;
-      const int64_t at = (real ? span.column(j) : 0) * D * X::kElt + c * 16;
-      cp16(s + r * X::kRow + X::k_chunk(r, c) * 16, kbase + at, real);
-      cp16(s + X::kKeys * X::kRow + r * X::kRow + X::v_chunk(r, c) * 16, vbase + at, real);
+  // (rows that nobody sees are never read, whatever they hold). A thread
+  // copies piece `pc` of every kSweep-th row.
+  constexpr int kPieces = DP * X::kElt / 16, kWho = KS ? 32 : kThreads;
+  constexpr int kSweep = kWho / kPieces;
+  const int who = KS ? lane : threadIdx.x;
+  const int pc = who % kPieces, pr = (KS ? warp * N : 0) + who / kPieces;
+  const bool has_piece = pc * 16 < row_bytes;
+  const unsigned char* kbase =
+      static_cast<const unsigned char*>(PREFIX ? a.kp : a.c.k) + head_row * row_bytes + pc * 16;
+  const unsigned char* vbase =
+      static_cast<const unsigned char*>(PREFIX ? a.vp : a.c.v) + head_row * row_bytes + pc * 16;
+  auto stage = [&](int tile, int buf) {
+    unsigned char* s = smem + buf * X::kStageBytes;
+    if (has_piece) {
+#pragma unroll
+      for (int it = 0; it < N / kSweep; ++it) {
+        const int r = pr + it * kSweep;
+        const int j = tile * X::kKeys + r;
+        const bool real = j < span.n;
+        const int64_t at = (int64_t)(real ? span.column(j) : 0) * row_bytes;
+        cp16(s + r * X::kRow + X::k_chunk(r, pc) * 16, kbase + at, real);
+        cp16(s + X::kKeys * X::kRow + r * X::kRow + X::v_chunk(r, pc) * 16, vbase + at, real);
+      }
     }
     if (kScaled) {
       float* sc = reinterpret_cast<float*>(s + 2 * X::kKeys * X::kRow);
-      for (int i = who; i < 2 * N; i += step) {
-        const int r = first + (i % N);
-        const int64_t j = tile * X::kKeys + r;
+      for (int i = who; i < N; i += kWho) {
+        const int r = (KS ? warp * N : 0) + i;
+        const int j = tile * X::kKeys + r;
         const bool real = j < span.n;
-        const float* src = (i < N ? a.c.ks : a.c.vs) + head_row + (real ? span.column(j) : 0);
-        cp4(sc + (i < N ? 0 : X::kKeys) + r, src, real);
+        const int64_t at = head_row + (real ? span.column(j) : 0);
+        cp4(sc + r, a.c.ks + at, real);
+        cp4(sc + X::kKeys + r, a.c.vs + at, real);
       }
     }
   };
@@ -281,95 +301,101 @@ __global__ void __launch_bounds__(kThreads) k_attn_part(const PartArgs p) {
   };
   // padding between D and DP holds zeros from the start
   if (D < DP) {
-    const int padc = DP * X::kElt / 16;
-    for (int i = threadIdx.x; i < X::kStages * 2 * X::kKeys * padc; i += kThreads) {
-      const int c = i % padc, r = (i / padc) % X::kKeys, kv = (i / padc / X::kKeys) % 2;
-      const int st = i / padc / X::kKeys / 2;
-      if (c >= chunks)
+    for (int i = threadIdx.x; i < X::kStages * 2 * X::kKeys * kPieces; i += kThreads) {
+      const int c = i % kPieces, r = (i / kPieces) % X::kKeys, kv = (i / kPieces / X::kKeys) % 2;
+      const int st = i / kPieces / X::kKeys / 2;
+      if (c * 16 >= row_bytes)
         *reinterpret_cast<uint4*>(smem + st * X::kStageBytes + kv * X::kKeys * X::kRow +
                                   r * X::kRow + (kv ? X::v_chunk(r, c) : X::k_chunk(r, c)) * 16) =
             make_uint4(0, 0, 0, 0);
     }
   }
+  // a negative scale turns the queries' sign, so that a larger score is always
+  // a larger product
+  const float turn = a.scale < 0.f ? -1.f : 1.f;
   float* qs = reinterpret_cast<float*>(smem + X::kStages * X::kStageBytes);
   if (kF32) {
     for (int i = threadIdx.x; i < X::kRows * DP; i += kThreads) {
       const int r = i / DP, d = i % DP;
       float x = 0.f;
-      if (r0 + r < rN && d < D) {
-        int64_t b, t;
-        int h;
-        query_of(r0 + r, b, t, h);
-        x = static_cast<const float*>(a.q.p)[b * a.q.sb + t * a.q.st + h * a.q.sh + d];
-      }
+      if (r0 + r < rN && d < D) x = Elt<QT>::to_f(query_ptr(r0 + r)[d]) * turn;
       qs[r * X::kQRow + d] = x;
     }
   }
   if (D < DP || kF32) __syncthreads();
 #pragma unroll
   for (int i = 0; i < X::kStages - 1; ++i) {
-    if (tile0 + i < tile1) stage(tile0 + i);
+    if (tile0 + i < tile1) stage(tile0 + i, i);
     cp_commit();
   }
 
   // ---- queries of this thread: rows row[0] and row[1] = row[0] + 8
   const int wrow = KS ? 0 : warp * 16;
-  int64_t row[2], tq[2];
+  int row[2];
+  int64_t tq[2];  // last column that the row sees
   float rscale[2];
   uint32_t qf[kF32 ? 1 : DP / 16][4];
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
     row[u] = r0 + wrow + g + 8 * u;
-    tq[u] = row[u] < rN ? row[u] / p.group : 0;
-    rscale[u] = a.scale * kLog2e;
+    tq[u] = col + (row[u] < rN ? row[u] / p.group : 0);
+    rscale[u] = a.scale * turn * kLog2e;
   }
-  if (!kF32) {
+  if constexpr (!kF32) {
+    const uint32_t flip = turn < 0.f ? 0x80008000u : 0u;
     const __nv_bfloat16* qp[2] = {nullptr, nullptr};
 #pragma unroll
     for (int u = 0; u < 2; ++u)
-      if (row[u] < rN) {
-        int64_t b, t;
-        int h;
-        query_of(row[u], b, t, h);
-        qp[u] = static_cast<const __nv_bfloat16*>(a.q.p) + b * a.q.sb + t * a.q.st + h * a.q.sh;
-      }
-    if (!kScaled) {
+      if (row[u] < rN) qp[u] = query_ptr(row[u]);
+    if constexpr (!kScaled) {
 #pragma unroll
       for (int k = 0; k < DP / 16; ++k)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int d = k * 16 + t4 * 2 + (i >> 1) * 8;
-          qf[k][i] = qp[i & 1] && d < D ? *reinterpret_cast<const uint32_t*>(qp[i & 1] + d) : 0u;
+          qf[k][i] = qp[i & 1] && d < D
+                         ? *reinterpret_cast<const uint32_t*>(qp[i & 1] + d) ^ flip : 0u;
         }
     } else {
       // Codes are exact in fp16, so the products are fp16 ones. A query row is
       // scaled by a power of two to a largest magnitude in [1, 2): its bf16
       // values stay exact down to 2^-14 of it, and below that are off by 2^-25
       // of it at most.
-      float qv[2][DP / 4];
+      uint4 raw[2][DP / 32];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int i = 0; i < DP / 32; ++i) {
+          const int d = (i / 2) * 64 + t4 * 16 + (i % 2) * 8;
+          raw[u][i] = qp[u] && d < D ? *reinterpret_cast<const uint4*>(qp[u] + d)
+                                     : make_uint4(0, 0, 0, 0);
+        }
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        float m = 0.f;
+        float qv[DP / 4], m = 0.f;
 #pragma unroll
-        for (int i = 0; i < DP / 4; ++i) {
-          const int d = (i / 16) * 64 + t4 * 16 + (i % 16);
-          qv[u][i] = qp[u] && d < D ? __bfloat162float(qp[u][d]) : 0.f;
-          m = fmaxf(m, fabsf(qv[u][i]));
+        for (int i = 0; i < DP / 32; ++i) {
+          const uint32_t w[4] = {raw[u][i].x, raw[u][i].y, raw[u][i].z, raw[u][i].w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            qv[i * 8 + 2 * e] = __uint_as_float((w[e] ^ flip) << 16);
+            qv[i * 8 + 2 * e + 1] = __uint_as_float((w[e] ^ flip) & 0xffff0000u);
+          }
         }
+#pragma unroll
+        for (int i = 0; i < DP / 4; ++i) m = fmaxf(m, fabsf(qv[i]));
         m = quad_max(m);
         const int ex = (int)(__float_as_uint(m) >> 23) - 127;
         const int e = m > 0.f && ex < 128 ? min(max(ex, -126), 126) : 0;
         const float down = __uint_as_float((uint32_t)(127 - e) << 23);
         rscale[u] *= __uint_as_float((uint32_t)(127 + e) << 23);
+        // k-step k of a 64-wide block takes values 4k..4k+3 of each thread's 16
 #pragma unroll
-        for (int i = 0; i < DP / 4; ++i) qv[u][i] *= down;
+        for (int k = 0; k < DP / 16; ++k) {
+          qf[k][u] = pack_f16x2(qv[k * 4] * down, qv[k * 4 + 1] * down);
+          qf[k][u + 2] = pack_f16x2(qv[k * 4 + 2] * down, qv[k * 4 + 3] * down);
+        }
       }
-      // k-step k of a 64-wide block takes values 4k..4k+3 of each thread's 16
-#pragma unroll
-      for (int k = 0; k < DP / 16; ++k)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          qf[k][i] = pack_f16x2(qv[i & 1][k * 4 + (i >> 1) * 2], qv[i & 1][k * 4 + (i >> 1) * 2 + 1]);
     }
   }
 
@@ -378,19 +404,22 @@ __global__ void __launch_bounds__(kThreads) k_attn_part(const PartArgs p) {
   for (int i = 0; i < OT; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};  // m before rscale
   float vref = 0.f;  // what o counts in, for scaled values: their largest scale so far
 
-  for (int64_t tile = tile0; tile < tile1; ++tile) {
+  int buf = 0, ahead = X::kStages - 1;
+  for (int tile = tile0; tile < tile1; ++tile) {
     cp_wait<X::kStages - 2>();
     sync();
-    if (tile + X::kStages - 1 < tile1) stage(tile + X::kStages - 1);
+    if (tile + X::kStages - 1 < tile1) stage(tile + X::kStages - 1, ahead);
     cp_commit();
-    const unsigned char* ks = smem + (tile % X::kStages) * X::kStageBytes;
+    const unsigned char* ks = smem + buf * X::kStageBytes;
     const unsigned char* vs = ks + X::kKeys * X::kRow;
     const float* sc = reinterpret_cast<const float*>(vs + X::kKeys * X::kRow);
+    buf = buf + 1 == X::kStages ? 0 : buf + 1;
+    ahead = ahead + 1 == X::kStages ? 0 : ahead + 1;
     const int kr0 = KS ? warp * N : 0;  // first staged row of this warp's keys
-    const int64_t j0 = tile * X::kKeys + kr0;
+    const int j0 = tile * X::kKeys + kr0;
     if (KS && j0 >= span.n) continue;
 
     // ---- scores
@@ -474,35 +503,34 @@ __global__ void __launch_bounds__(kThreads) k_attn_part(const PartArgs p) {
     }
 
     // ---- scale, mask, running maximum
-    const bool edge = j0 + N > span.n || (!PREFIX && a.tokens > 1);
+    const bool edge = j0 + N > span.n || (!PREFIX && tokens > 1);
     float mx[2] = {m[0], m[1]};
     float vmax = vref;
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
-      float f[2] = {1.f, 1.f};
       if (kScaled) {
         const float2 kk = *reinterpret_cast<const float2*>(sc + kr0 + i * 8 + t4 * 2);
         const float2 vv = *reinterpret_cast<const float2*>(sc + X::kKeys + kr0 + i * 8 + t4 * 2);
-        f[0] = kk.x, f[1] = kk.y;
+        s[i][0] *= kk.x, s[i][1] *= kk.y, s[i][2] *= kk.x, s[i][3] *= kk.y;
         vmax = fmaxf(vmax, fmaxf(vv.x, vv.y));
       }
+      if (edge) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        s[i][j] *= kScaled ? rscale[j >> 1] * f[j & 1] : rscale[j >> 1];
-        if (edge) {
-          const int64_t jj = j0 + i * 8 + t4 * 2 + (j & 1);
-          const bool see = jj < span.n && (PREFIX || span.column(jj) <= col + tq[j >> 1]);
+        for (int j = 0; j < 4; ++j) {
+          const int jj = j0 + i * 8 + t4 * 2 + (j & 1);
+          const bool see = jj < span.n && (PREFIX || span.column(jj) <= tq[j >> 1]);
           if (!see) s[i][j] = -INFINITY;
         }
-        mx[j >> 1] = fmaxf(mx[j >> 1], s[i][j]);
       }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) mx[j >> 1] = fmaxf(mx[j >> 1], s[i][j]);
     }
     float keep[2], base[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       mx[u] = quad_max(mx[u]);
-      base[u] = mx[u] == -INFINITY ? 0.f : mx[u];
-      keep[u] = ex2(m[u] - base[u]);
+      base[u] = mx[u] == -INFINITY ? 0.f : mx[u] * rscale[u];
+      keep[u] = m[u] == -INFINITY ? 0.f : ex2((m[u] - mx[u]) * rscale[u]);
       m[u] = mx[u];
       l[u] *= keep[u];
     }
@@ -518,10 +546,11 @@ __global__ void __launch_bounds__(kThreads) k_attn_part(const PartArgs p) {
     for (int i = 0; i < NT; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        s[i][j] = ex2(s[i][j] - base[j >> 1]);
+        s[i][j] = ex2(fmaf(s[i][j], rscale[j >> 1], -base[j >> 1]));
         l[j >> 1] += s[i][j];
       }
-    if (!kF32) {
+    // most tiles change neither maximum nor reference: nothing to rescale
+    if (!kF32 && __any_sync(0xffffffffu, keep[0] != 1.f || keep[1] != 1.f)) {
 #pragma unroll
       for (int i = 0; i < OT; ++i)
 #pragma unroll
@@ -531,8 +560,8 @@ __global__ void __launch_bounds__(kThreads) k_attn_part(const PartArgs p) {
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
         const float2 vv = *reinterpret_cast<const float2*>(sc + X::kKeys + kr0 + i * 8 + t4 * 2);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) s[i][j] *= (j & 1 ? vv.y : vv.x) * vinv;
+        const float v0 = vv.x * vinv, v1 = vv.y * vinv;
+        s[i][0] *= v0, s[i][1] *= v1, s[i][2] *= v0, s[i][3] *= v1;
       }
     }
 
@@ -637,15 +666,22 @@ __global__ void __launch_bounds__(kThreads) k_attn_part(const PartArgs p) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) o[i][j] *= vref;
 
+  // maxima in base 2 from here on
+#pragma unroll
+  for (int u = 0; u < 2; ++u) m[u] = m[u] == -INFINITY ? m[u] : m[u] * rscale[u];
+
   // value index of accumulator element (tile n, j)
   auto value_of = [&](int n, int j) {
     return kScaled ? (n >> 1) * 16 + (t4 * 2 + (j & 1)) * 2 + (n & 1) : n * 8 + t4 * 2 + (j & 1);
   };
+  const int nrow = rN - r0;
   if constexpr (KS) {
     // ---- the four warps' sums meet in shared memory
     __syncthreads();
-    float* jo = reinterpret_cast<float*>(smem);                      // [4][16][DP]
-    float2* jm = reinterpret_cast<float2*>(smem + 4 * 16 * DP * 4);  // [4][16]
+    float* jo = reinterpret_cast<float*>(smem);  // [4][16][DP], then the CTA's own [16][DP]
+    float2* jm = reinterpret_cast<float2*>(smem + 5 * 16 * DP * 4);  // [4][16], then [16]
+    float* co = jo + 4 * 16 * DP;
+    float2* cm = jm + 4 * 16;
 #pragma unroll
     for (int i = 0; i < OT; ++i)
 #pragma unroll
@@ -656,35 +692,73 @@ __global__ void __launch_bounds__(kThreads) k_attn_part(const PartArgs p) {
       jm[warp * 16 + g + 8] = make_float2(m[1], l[1]);
     }
     __syncthreads();
-    const int nrow = (int)(rN - r0);
-    for (int i = threadIdx.x; i < nrow * D; i += kThreads) {
-      const int r = i / D, d = i - r * D;
-      float mm = -INFINITY;
+    const int quads = D >> 2;
+    // four values of a row at a time, joined in the order of warps and splits
+    for (int i = threadIdx.x; i < nrow * quads; i += kThreads) {
+      const int r = i / quads, d = (i - r * quads) * 4;
+      float mm = -INFINITY, ll = 0.f;
 #pragma unroll
       for (int w = 0; w < 4; ++w) mm = fmaxf(mm, jm[w * 16 + r].x);
       const float base = mm == -INFINITY ? 0.f : mm;
-      float ll = 0.f, oo = 0.f;
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         const float f = ex2(jm[w * 16 + r].x - base);
+        const float4 y = *reinterpret_cast<const float4*>(jo + (w * 16 + r) * DP + d);
         ll += jm[w * 16 + r].y * f;
-        oo += jo[(w * 16 + r) * DP + d] * f;
+        x.x += y.x * f, x.y += y.y * f, x.z += y.z * f, x.w += y.w * f;
       }
-      const int64_t orow = out_row(r0 + r);
-      if (p.part_o) {
-        const int64_t slot = split * p.out_rows + orow;
-        p.part_o[slot * D + d] = oo;
+      if (!p.joined) {
+        const int64_t slot = (p.extra + split) * p.out_rows + out_row(r0 + r);
+        *reinterpret_cast<float4*>(p.part_o + slot * D + d) = x;
         if (d == 0) p.part_ml[slot] = make_float2(mm, ll);
       } else {
-        static_cast<QT*>(a.out)[orow * D + d] = Elt<QT>::from_f(ll == 0.f ? 0.f : oo / ll);
+        *reinterpret_cast<float4*>(co + r * DP + d) = x;
+        if (d == 0) cm[r] = make_float2(mm, ll);
       }
     }
+    if (!p.joined) return;
+    // ---- the splits' sums, and the extra ones, in this split's share of the rows
+    cg::cluster_group cluster = cg::this_cluster();
+    if (p.splits > 1)
+      cluster.sync();
+    else
+      __syncthreads();
+    for (int i = split * kThreads + threadIdx.x; i < nrow * quads; i += p.splits * kThreads) {
+      const int r = i / quads, d = (i - r * quads) * 4;
+      const int64_t orow = out_row(r0 + r);
+      float mm = -INFINITY, ll = 0.f;
+      for (int c = 0; c < p.splits; ++c)
+        mm = fmaxf(mm, (p.splits > 1 ? cluster.map_shared_rank(cm, c) : cm)[r].x);
+      for (int c = 0; c < p.extra; ++c) mm = fmaxf(mm, p.part_ml[c * p.out_rows + orow].x);
+      const float base = mm == -INFINITY ? 0.f : mm;
+      float x[4] = {};
+      auto add = [&](float2 ml, float4 y) {
+        const float f = ex2(ml.x - base);
+        ll += ml.y * f;
+        x[0] += y.x * f, x[1] += y.y * f, x[2] += y.z * f, x[3] += y.w * f;
+      };
+      for (int c = 0; c < p.extra; ++c) {
+        const int64_t slot = c * p.out_rows + orow;
+        add(p.part_ml[slot], *reinterpret_cast<const float4*>(p.part_o + slot * D + d));
+      }
+      for (int c = 0; c < p.splits; ++c) {
+        const float2* fm = p.splits > 1 ? cluster.map_shared_rank(cm, c) : cm;
+        const float* fo = p.splits > 1 ? cluster.map_shared_rank(co, c) : co;
+        add(fm[r], *reinterpret_cast<const float4*>(fo + r * DP + d));
+      }
+      const float inv = ll == 0.f ? 0.f : 1.f / ll;
+      QT* out = static_cast<QT*>(a.out) + orow * D + d;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) out[e] = Elt<QT>::from_f(x[e] * inv);
+    }
+    if (p.splits > 1) cluster.sync();  // nobody leaves while its sums are read
   } else {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       if (row[u] >= rN) continue;
       const int64_t orow = out_row(row[u]);
-      const int64_t slot = split * p.out_rows + orow;
+      const int64_t slot = (p.extra + split) * p.out_rows + orow;
       const float inv = l[u] == 0.f ? 0.f : 1.f / l[u];
 #pragma unroll
       for (int i = 0; i < OT; ++i)
@@ -692,12 +766,12 @@ __global__ void __launch_bounds__(kThreads) k_attn_part(const PartArgs p) {
         for (int j = 0; j < 2; ++j) {
           const int d = value_of(i, j);
           if (d >= D) continue;
-          if (p.part_o)
+          if (!p.joined)
             p.part_o[slot * D + d] = o[i][2 * u + j];
           else
             static_cast<QT*>(a.out)[orow * D + d] = Elt<QT>::from_f(o[i][2 * u + j] * inv);
         }
-      if (p.part_o && t4 == 0) p.part_ml[slot] = make_float2(m[u], l[u]);
+      if (!p.joined && t4 == 0) p.part_ml[slot] = make_float2(m[u], l[u]);
     }
   }
 }
@@ -725,15 +799,17 @@ __global__ void __launch_bounds__(128) k_attn_join(const float* part_o, const fl
   for (int e = 0; e < 4; ++e) out[r * D + d + e] = Elt<T>::from_f(l == 0.f ? 0.f : x[e] / l);
 }
 
-// How a call is cut: splits of the own columns and of the prefix.
+// How a call is cut: splits of the own columns and of the prefix, and whether
+// the own part's clusters join everything (else k_attn_join does).
 struct Plan {
-  bool own_ks, prefix_ks;
+  bool own_ks, prefix_ks, joined;
   int own_splits, prefix_splits;
   int64_t out_rows, bytes;
 };
 
-constexpr int kSlots = 296;    // CTAs resident at a time: 148 SMs, two each
-constexpr int64_t kMinKeys = 256;  // keys of a split, at least
+constexpr int kSlots = 296;         // CTAs resident at a time: 148 SMs, two each
+constexpr int64_t kMinKeys = 128;   // keys of a split, at least
+constexpr int kMaxCluster = 8;
 
 int splits_for(int64_t keys, int64_t ctas) {
   if (keys <= kMinKeys || ctas >= kSlots) return 1;
@@ -754,9 +830,13 @@ Plan plan_for(int64_t batch, int64_t tokens, int q_heads, int kv_heads, int head
   p.own_splits = splits_for(keys, batch * kv_heads * ((own_rows + ot - 1) / ot));
   p.prefix_splits =
       prefix_cols > 0 ? splits_for(prefix_cols, kv_heads * ((pre_rows + pt - 1) / pt)) : 0;
+  // a split or two more than a cluster holds costs less than another launch
+  if (p.own_ks && p.own_splits <= 2 * kMaxCluster && p.own_splits > kMaxCluster)
+    p.own_splits = kMaxCluster;
+  p.joined = p.own_ks ? p.own_splits <= kMaxCluster : p.own_splits + p.prefix_splits == 1;
   p.out_rows = batch * tokens * q_heads;
-  const int total = p.own_splits + p.prefix_splits;
-  p.bytes = total > 1 ? total * p.out_rows * (head_dim * 4 + 8) : 0;
+  const int parts = p.prefix_splits + (p.joined ? 0 : p.own_splits);
+  p.bytes = parts * p.out_rows * (head_dim * 4 + 8);
   return p;
 }
 
@@ -767,9 +847,18 @@ int run_part(const PartArgs& p, int64_t mats, cudaStream_t st) {
   const cudaError_t e =
       cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, X::kSmem);
   if (e != cudaSuccess) return (int)e;
-  const dim3 grid((unsigned)(mats * p.row_tiles * p.splits), (unsigned)p.a.kv_heads);
-  k<<<grid, kThreads, X::kSmem, st>>>(p);
-  return 0;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(mats * p.row_tiles * p.splits), (unsigned)p.a.kv_heads);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = X::kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = KS && p.joined ? p.splits : 1, at.val.clusterDim.y = 1,
+  at.val.clusterDim.z = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return (int)cudaLaunchKernelEx(&cfg, k, p);
 }
 template <typename QT, typename CT, bool KS, bool PREFIX>
 int run_dp(const PartArgs& p, int64_t mats, cudaStream_t st) {
@@ -780,25 +869,26 @@ int run_dp(const PartArgs& p, int64_t mats, cudaStream_t st) {
 template <typename QT, typename CT>
 int run_attention(const AttnArgs& a, const Plan& pl, void* workspace, cudaStream_t st) {
   const int group = a.q_heads / a.kv_heads;
-  const int total = pl.own_splits + pl.prefix_splits;
-  float* po = total > 1 ? static_cast<float*>(workspace) : nullptr;
-  float2* pm = total > 1 ? reinterpret_cast<float2*>(po + total * pl.out_rows * a.head_dim) : nullptr;
-  PartArgs p{a, group, a.tokens * group, 0, pl.own_splits, pl.out_rows, po, pm};
-  p.row_tiles = (int)((p.rows + (pl.own_ks ? 15 : 63)) / (pl.own_ks ? 16 : 64));
-  int rc = pl.own_ks ? run_dp<QT, CT, true, false>(p, a.batch, st)
-                     : run_dp<QT, CT, false, false>(p, a.batch, st);
-  if (rc) return rc;
+  const int parts = pl.prefix_splits + (pl.joined ? 0 : pl.own_splits);
+  float* po = parts ? static_cast<float*>(workspace) : nullptr;
+  float2* pm = parts ? reinterpret_cast<float2*>(po + parts * pl.out_rows * a.head_dim) : nullptr;
   if (pl.prefix_splits) {
-    PartArgs x{a, group, a.batch * a.tokens * group, 0, pl.prefix_splits, pl.out_rows,
-               po + pl.own_splits * pl.out_rows * a.head_dim,
-               pm + pl.own_splits * pl.out_rows};
-    x.row_tiles = (int)((x.rows + (pl.prefix_ks ? 15 : 63)) / (pl.prefix_ks ? 16 : 64));
-    rc = pl.prefix_ks ? run_dp<QT, QT, true, true>(x, 1, st) : run_dp<QT, QT, false, true>(x, 1, st);
+    PartArgs x{a, group, (int)(a.batch * a.tokens * group), 0, pl.prefix_splits, 0, 0, pl.out_rows,
+               po, pm};
+    x.row_tiles = (x.rows + (pl.prefix_ks ? 15 : 63)) / (pl.prefix_ks ? 16 : 64);
+    const int rc = pl.prefix_ks ? run_dp<QT, QT, true, true>(x, 1, st)
+                                : run_dp<QT, QT, false, true>(x, 1, st);
     if (rc) return rc;
   }
-  if (total > 1) {
+  PartArgs p{a, group, (int)(a.tokens * group), 0, pl.own_splits, pl.joined, pl.prefix_splits,
+             pl.out_rows, po, pm};
+  p.row_tiles = (p.rows + (pl.own_ks ? 15 : 63)) / (pl.own_ks ? 16 : 64);
+  const int rc = pl.own_ks ? run_dp<QT, CT, true, false>(p, a.batch, st)
+                           : run_dp<QT, CT, false, false>(p, a.batch, st);
+  if (rc) return rc;
+  if (!pl.joined) {
     const int64_t n = pl.out_rows * (a.head_dim / 4);
-    k_attn_join<QT><<<(unsigned)((n + 127) / 128), 128, 0, st>>>(po, pm, total, pl.out_rows,
+    k_attn_join<QT><<<(unsigned)((n + 127) / 128), 128, 0, st>>>(po, pm, parts, pl.out_rows,
                                                                   a.head_dim,
                                                                   static_cast<QT*>(a.out));
   }
@@ -840,6 +930,8 @@ extern "C" int mep_cache_attention(int dtype, int cache_dtype, int64_t batch, in
     return serve_invalid(op, why);
   if (capacity < 0 || prefix_cols < 0 || prompt_cols < 0)
     return serve_invalid(op, "negative columns");
+  if (capacity > 0x7fffffff - 1024 || prefix_cols > 0x7fffffff - 1024)
+    return serve_invalid(op, "columns up to 2^31 - 1025");
   if (!col_dev && (col < 0 || col + tokens > capacity))
     return serve_invalid(op, "columns [col, col + tokens) do not fit the cache");
   if (batch == 0 || tokens == 0) return MEP_OK;

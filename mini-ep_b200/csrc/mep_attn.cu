@@ -17,37 +17,16 @@
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 
+#include "mep_attn.cuh"
 #include "mep_device.cuh"
-#include "mep_serve.cuh"
 
 namespace mep {
 namespace {
 
 namespace cg = cooperative_groups;
 
-struct AttnArgs {
-  int64_t batch, tokens;
-  int q_heads, kv_heads, head_dim;
-  HeadsView q;
-  CacheView c;
-  const int64_t* lengths;
-  int64_t prompt_cols, col;
-  const int64_t* col_dev;
-  const void* kp;
-  const void* vp;
-  int64_t prefix_cols;
-  float scale;
-  void* out;
-};
-
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kThreads = 128;  // four warps a CTA
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ void cp16(void* dst, const void* src, bool real) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src),
                "r"(real ? 16 : 0)
@@ -740,7 +719,8 @@ __global__ void __launch_bounds__(kThreads) k_attn_part(const PartArgs p) {
       };
       for (int c = 0; c < p.extra; ++c) {
         const int64_t slot = c * p.out_rows + orow;
-        add(p.part_ml[slot], *reinterpret_cast<const float4*>(p.part_o + slot * D + d));
+        const float2 ml = p.part_ml[slot];  // an empty slot's values are unwritten
+        if (ml.y != 0.f) add(ml, *reinterpret_cast<const float4*>(p.part_o + slot * D + d));
       }
       for (int c = 0; c < p.splits; ++c) {
         const float2* fm = p.splits > 1 ? cluster.map_shared_rank(cm, c) : cm;
@@ -759,6 +739,26 @@ __global__ void __launch_bounds__(kThreads) k_attn_part(const PartArgs p) {
       if (row[u] >= rN) continue;
       const int64_t orow = out_row(row[u]);
       const int64_t slot = (p.extra + split) * p.out_rows + orow;
+      if (p.joined && p.extra) {
+        float mm = m[u];
+        for (int c = 0; c < p.extra; ++c) mm = fmaxf(mm, p.part_ml[c * p.out_rows + orow].x);
+        const float base = mm == -INFINITY ? 0.f : mm, f0 = ex2(m[u] - base);
+        l[u] *= f0;
+#pragma unroll
+        for (int i = 0; i < OT; ++i) o[i][2 * u] *= f0, o[i][2 * u + 1] *= f0;
+        for (int c = 0; c < p.extra; ++c) {
+          const float2 ml = p.part_ml[c * p.out_rows + orow];
+          if (ml.y == 0.f) continue;  // empty: its values are unwritten
+          const float f = ex2(ml.x - base);
+          l[u] += ml.y * f;
+          const float* y = p.part_o + (c * p.out_rows + orow) * D;
+#pragma unroll
+          for (int i = 0; i < OT; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+              if (value_of(i, j) < D) o[i][2 * u + j] += y[value_of(i, j)] * f;
+        }
+      }
       const float inv = l[u] == 0.f ? 0.f : 1.f / l[u];
 #pragma unroll
       for (int i = 0; i < OT; ++i)
@@ -790,6 +790,7 @@ __global__ void __launch_bounds__(128) k_attn_join(const float* part_o, const fl
   const float base = m == -INFINITY ? 0.f : m;
   for (int s = 0; s < splits; ++s) {
     const float2 ml = part_ml[s * out_rows + r];
+    if (ml.y == 0.f) continue;  // empty: its values may be unwritten
     const float f = ex2(ml.x - base);
     const float4 v = *reinterpret_cast<const float4*>(part_o + (s * out_rows + r) * D + d);
     l += ml.y * f;
@@ -802,8 +803,9 @@ __global__ void __launch_bounds__(128) k_attn_join(const float* part_o, const fl
 // How a call is cut: splits of the own columns and of the prefix, and whether
 // the own part's clusters join everything (else k_attn_join does).
 struct Plan {
-  bool own_ks, prefix_ks, joined;
+  bool own_ks, prefix_ks, joined, prefix_tc;
   int own_splits, prefix_splits;
+  PrefixTcPlan tc;
   int64_t out_rows, bytes;
 };
 
@@ -818,7 +820,9 @@ int splits_for(int64_t keys, int64_t ctas) {
   return (int)(want < most ? want : most);
 }
 
-Plan plan_for(int64_t batch, int64_t tokens, int q_heads, int kv_heads, int head_dim,
+constexpr int64_t kTcRows = 128;  // rows of a key/value head from which the prefix is tcgen05's
+
+Plan plan_for(int dtype, int64_t batch, int64_t tokens, int q_heads, int kv_heads, int head_dim,
               int64_t capacity, int64_t col, int64_t prefix_cols) {
   Plan p{};
   const int group = q_heads / kv_heads;
@@ -830,10 +834,15 @@ Plan plan_for(int64_t batch, int64_t tokens, int q_heads, int kv_heads, int head
   p.own_splits = splits_for(keys, batch * kv_heads * ((own_rows + ot - 1) / ot));
   p.prefix_splits =
       prefix_cols > 0 ? splits_for(prefix_cols, kv_heads * ((pre_rows + pt - 1) / pt)) : 0;
+  p.prefix_tc = dtype == MEP_BF16 && prefix_cols > 0 && pre_rows >= kTcRows;
+  if (p.prefix_tc) {
+    p.tc = plan_prefix_tc(pre_rows, kv_heads, prefix_cols);
+    p.prefix_splits = p.tc.slots;
+  }
   // a split or two more than a cluster holds costs less than another launch
   if (p.own_ks && p.own_splits <= 2 * kMaxCluster && p.own_splits > kMaxCluster)
     p.own_splits = kMaxCluster;
-  p.joined = p.own_ks ? p.own_splits <= kMaxCluster : p.own_splits + p.prefix_splits == 1;
+  p.joined = p.own_ks ? p.own_splits <= kMaxCluster : p.own_splits == 1;
   p.out_rows = batch * tokens * q_heads;
   const int parts = p.prefix_splits + (p.joined ? 0 : p.own_splits);
   p.bytes = parts * p.out_rows * (head_dim * 4 + 8);
@@ -872,7 +881,9 @@ int run_attention(const AttnArgs& a, const Plan& pl, void* workspace, cudaStream
   const int parts = pl.prefix_splits + (pl.joined ? 0 : pl.own_splits);
   float* po = parts ? static_cast<float*>(workspace) : nullptr;
   float2* pm = parts ? reinterpret_cast<float2*>(po + parts * pl.out_rows * a.head_dim) : nullptr;
-  if (pl.prefix_splits) {
+  if (pl.prefix_tc) {
+    if (const int rc = launch_prefix_tc(a, pl.tc, pl.out_rows, po, pm, st)) return rc;
+  } else if (pl.prefix_splits) {
     PartArgs x{a, group, (int)(a.batch * a.tokens * group), 0, pl.prefix_splits, 0, 0, pl.out_rows,
                po, pm};
     x.row_tiles = (x.rows + (pl.prefix_ks ? 15 : 63)) / (pl.prefix_ks ? 16 : 64);
@@ -909,7 +920,7 @@ extern "C" int mep_cache_attention_workspace(int dtype, int cache_dtype, int64_t
     return serve_invalid(op, why);
   if (capacity < 0 || prefix_cols < 0) return serve_invalid(op, "negative columns");
   if (!bytes_out) return serve_invalid(op, "bytes_out is required");
-  *bytes_out = batch && tokens ? plan_for(batch, tokens, q_heads, kv_heads, head_dim, capacity, col,
+  *bytes_out = batch && tokens ? plan_for(dtype, batch, tokens, q_heads, kv_heads, head_dim, capacity, col,
                                           prefix_cols)
                                      .bytes
                                : 0;
@@ -945,7 +956,7 @@ extern "C" int mep_cache_attention(int dtype, int cache_dtype, int64_t batch, in
   if (bad_strides(a.q, dtype == MEP_BF16 ? 2 : 4) || !aligned16(k_cache) || !aligned16(v_cache) ||
       !aligned16(k_prefix) || !aligned16(v_prefix) || !aligned16(out))
     return serve_invalid(op, "tensors and row strides must be multiples of 16 bytes");
-  const Plan pl = plan_for(batch, tokens, q_heads, kv_heads, head_dim, capacity,
+  const Plan pl = plan_for(dtype, batch, tokens, q_heads, kv_heads, head_dim, capacity,
                            col_dev ? -1 : col, prefix_cols);
   if (pl.bytes > 0 && (!workspace || workspace_bytes < pl.bytes || !aligned16(workspace)))
     return serve_invalid(op, "workspace of " + std::to_string(pl.bytes) + " bytes needed");
@@ -957,6 +968,7 @@ extern "C" int mep_cache_attention(int dtype, int cache_dtype, int64_t batch, in
   else
     rc = cache_dtype == MEP_E4M3 ? run_attention<float, uint8_t>(a, pl, workspace, st)
                                  : run_attention<float, float>(a, pl, workspace, st);
+  if (rc < 0) return serve_invalid(op, "tensor map error " + std::to_string(rc));
   if (rc) return serve_cuda(op, (cudaError_t)rc);
   return serve_launched(op);
 }

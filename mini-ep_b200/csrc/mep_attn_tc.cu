@@ -1,0 +1,430 @@
+// Attention over the shared prefix on the tcgen05 tensor cores, for bf16 models
+// and batches of many rows: the queries of the whole batch that share a
+// key/value head are the rows of one matrix product, so a prefix tile is read
+// once for 256 of them and the work is bound by the products and the
+// exponentials, not by the prefix's bytes.
+//
+// A CTA has 256 rows (two halves of 128, the MMA's M) and walks tiles of 128
+// keys: S = Q K^T into TMEM, a thread a row takes the running maximum and the
+// exponentials, P goes back to TMEM over S as bf16 and is the A operand of
+// O += P V, which stays in TMEM. The halves alternate: while one's warps work
+// on exponentials, the tensor cores run the other's products. Q lies in shared
+// memory, K and V come by TMA through rings (a 3D tensor map, so that the last
+// tile's missing keys read as zeros). O is rescaled only when a row's maximum
+// has grown by more than 2^8 since it was last fixed: weights up to 2^8 are
+// as exact in bf16 and fp32 as weights up to 1.
+//
+// Persistent: the (head, 256-row tile, key tile) units are dealt to the CTAs in
+// equal runs, so a tile's keys may be cut between CTAs. A run's result is a
+// partial one (fp32 sums, maximum in base 2) in the tile's next slot.
+#include <cstdint>
+#include <cuda_bf16.h>
+
+#include "mep_attn.cuh"
+#include "mep_device.cuh"
+#include "mep_tc.cuh"
+
+namespace mep {
+int encode_bf16_3d(CUtensorMap* m, const void* base, const uint64_t (&dims)[3],
+                   const uint32_t (&box)[3]);  // mep_ffn.cu
+namespace {
+namespace px {
+using namespace ::mep::tc;
+
+constexpr int kRows = 128;   // rows of a half
+constexpr int kKeys = 128;   // keys of a tile
+constexpr int kThreads = 320;  // two softmax warpgroups, an MMA and a TMA warp
+constexpr unsigned long long kWaitNs = 2000000000ull;
+constexpr float kGrow = 8.f;
+
+template <int DP>
+struct Cfg {
+  static constexpr int SUB = kKeys * 128;           // 128 rows of 64 bf16: one swizzled block
+  static constexpr int TILE = DP / 64 * SUB;        // Q half, K tile or V tile
+  static constexpr int STAGES = DP == 64 ? 4 : 2;   // of K, and of V
+  static constexpr int DATA = (2 + 2 * STAGES) * TILE;
+  static constexpr int SMEM = DATA + 1024 + 1024;   // data | barriers | alignment slack
+  // kind::f16, fp32 accumulators, bf16 operands, M = 128
+  static constexpr uint32_t BASE = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(kRows >> 4) << 24);
+  static constexpr uint32_t IDESC_S = BASE | ((uint32_t)(kKeys >> 3) << 17);
+  static constexpr uint32_t IDESC_O = BASE | ((uint32_t)(DP >> 3) << 17) | (1u << 16);  // V: N-major
+};
+
+struct Smem {
+  uint64_t kfull[4], kempty[4], vfull[4], vempty[4];
+  uint64_t qready[2], sfull[2], pfull[2], ofull[2];
+  uint32_t tmem_base;
+  int abort;
+};
+
+struct Args {
+  AttnArgs a;
+  int group, rows, row_tiles, key_tiles, slots;
+  int64_t units, out_rows;
+  float* part_o;
+  float2* part_ml;
+};
+
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* tm, int x, int y, int z,
+                                            uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(tm)), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+      : "memory");
+}
+// V as the B operand: the 64 values of a swizzled row run along N, rows along
+// K. Blocks of 64 values are SUB bytes apart, groups of 8 keys 1024.
+__device__ __forceinline__ uint64_t v_desc(uint32_t saddr, uint32_t block_bytes) {
+  uint64_t d = (uint64_t)((saddr & 0x3FFFFu) >> 4);
+  d |= (uint64_t)(block_bytes >> 4) << 16;
+  d |= (uint64_t)(1024 >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;
+  return d;
+}
+// A operand from TMEM
+__device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b,
+                                           uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b), "r"(idesc), "r"(accumulate));
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+      "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
+      "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]),
+      "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+template <int DP>
+__global__ void __launch_bounds__(kThreads, 1)
+    k_attn_prefix_tc(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                     const Args p) {
+  using C = Cfg<DP>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* sq = smem;                        // two halves of queries
+  uint8_t* sk = smem + 2 * C::TILE;          // ring of K tiles
+  uint8_t* sv = sk + C::STAGES * C::TILE;    // ring of V tiles
+  Smem* S = reinterpret_cast<Smem*>(smem + C::DATA);
+  const int wp = warp_id(), lane = lane_id();
+  const AttnArgs& a = p.a;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::STAGES; ++s) {
+      mbar_init(&S->kfull[s], 1), mbar_init(&S->kempty[s], 1);
+      mbar_init(&S->vfull[s], 1), mbar_init(&S->vempty[s], 1);
+    }
+    for (int w = 0; w < 2; ++w) {
+      mbar_init(&S->qready[w], 4), mbar_init(&S->sfull[w], 1);
+      mbar_init(&S->pfull[w], 4), mbar_init(&S->ofull[w], 1);
+    }
+    S->abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (wp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(&S->tmem_base)),
+                 "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = S->tmem_base;  // S of half w: columns 128 w; O: 256 + DP w
+  auto wait = [&](uint64_t* b, uint32_t parity) {
+    return mbar_wait_for(b, parity, kWaitNs, &S->abort);
+  };
+  // this CTA's run of units; f(tile, first key tile, last + 1) for each tile in it
+  const int64_t u0 = p.units * blockIdx.x / gridDim.x, u1 = p.units * (blockIdx.x + 1) / gridDim.x;
+  auto each_tile = [&](auto f) {
+    for (int64_t u = u0; u < u1;) {
+      const int tile = (int)(u / p.key_tiles), k0 = (int)(u - (int64_t)tile * p.key_tiles);
+      const int k1 = (int)min((int64_t)p.key_tiles, k0 + (u1 - u));
+      if (!f(tile, k0, k1)) return;
+      u += k1 - k0;
+    }
+  };
+  auto halves_of = [&](int tile) {
+    return p.rows - (tile % p.row_tiles) * 2 * kRows > kRows ? 2 : 1;
+  };
+
+  if (wp == 9) {
+    // ------------------------------------------------------------ TMA loads
+    if (lane == 0) {
+      int s = 0, issued = 0;
+      uint32_t ph = 0;
+      each_tile([&](int tile, int k0, int k1) {
+        const int kh = tile / p.row_tiles;
+        for (int k = k0; k < k1; ++k) {
+          if (!wait(&S->kempty[s], ph ^ 1u)) return false;
+          mbar_expect_tx(&S->kfull[s], C::TILE);
+          for (int d = 0; d < DP / 64; ++d)
+            tma_load_3d(sk + s * C::TILE + d * C::SUB, &tmK, d * 64, k * kKeys, kh, &S->kfull[s]);
+          if (!wait(&S->vempty[s], ph ^ 1u)) return false;
+          mbar_expect_tx(&S->vfull[s], C::TILE);
+          for (int d = 0; d < DP / 64; ++d)
+            tma_load_3d(sv + s * C::TILE + d * C::SUB, &tmV, d * 64, k * kKeys, kh, &S->vfull[s]);
+          ++issued;
+          if (++s == C::STAGES) s = 0, ph ^= 1u;
+        }
+        return true;
+      });
+      if (S->abort) {  // leave no copy in flight: wait for each stage's last one
+        for (int i = 0; i < C::STAGES && i < issued; ++i) {
+          s = s == 0 ? C::STAGES - 1 : s - 1;
+          if (s == C::STAGES - 1) ph ^= 1u;
+          mbar_wait_for(&S->kfull[s], ph, kWaitNs, nullptr);
+          mbar_wait_for(&S->vfull[s], ph, kWaitNs, nullptr);
+        }
+      }
+    }
+  } else if (wp == 8) {
+    // ------------------------------------------------------------ MMA issue
+    if (lane == 0) {
+      int ks = 0, vs = 0;
+      uint32_t kph = 0, vph = 0, qph = 0, pph[2] = {0, 0};
+      const uint32_t q0 = smem_u32(sq), k_0 = smem_u32(sk), v_0 = smem_u32(sv);
+      auto scores = [&](int w, int stage) {
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; ++kk) {
+          const uint32_t off = (kk >> 2) * C::SUB + (kk & 3) * 32;
+          mma_f16<false>(tmem + 128 * w, sw128_desc(q0 + w * C::TILE + off),
+                         sw128_desc(k_0 + stage * C::TILE + off), C::IDESC_S, kk != 0);
+        }
+        mma_commit<false>(&S->sfull[w]);
+      };
+      each_tile([&](int tile, int k0, int k1) {
+        const int halves = halves_of(tile);
+        if (!wait(&S->kfull[ks], kph)) return false;
+        for (int w = 0; w < halves; ++w) {
+          if (!wait(&S->qready[w], w == 0 ? qph & 1u : (qph >> 1) & 1u)) return false;
+          fence_after();
+          scores(w, ks);
+        }
+        qph ^= halves == 2 ? 3u : 1u;
+        mma_commit<false>(&S->kempty[ks]);
+        if (++ks == C::STAGES) ks = 0, kph ^= 1u;
+        for (int k = k0; k < k1; ++k) {
+          const bool more = k + 1 < k1;
+          if (!wait(&S->vfull[vs], vph)) return false;
+          if (more && !wait(&S->kfull[ks], kph)) return false;
+          for (int w = 0; w < halves; ++w) {
+            if (!wait(&S->pfull[w], pph[w])) return false;
+            pph[w] ^= 1u;
+            fence_after();
+#pragma unroll
+            for (int kk = 0; kk < kKeys / 16; ++kk)
+              mma_f16_ts(tmem + 256 + DP * w, tmem + 128 * w + kk * 8,
+                         v_desc(v_0 + vs * C::TILE + kk * 2048, C::SUB), C::IDESC_O,
+                         k != k0 || kk != 0);
+            // the tile's last arrival is ofull's: nothing arrives behind it
+            if (w == halves - 1) mma_commit<false>(&S->vempty[vs]);
+            if (more)
+              scores(w, ks);
+            else
+              mma_commit<false>(&S->ofull[w]);
+          }
+          if (++vs == C::STAGES) vs = 0, vph ^= 1u;
+          if (more) {
+            mma_commit<false>(&S->kempty[ks]);
+            if (++ks == C::STAGES) ks = 0, kph ^= 1u;
+          }
+        }
+        return true;
+      });
+    }
+  } else {
+    // ------------------------------------------------------------ softmax
+    const int w = wp >> 2, quad = wp & 3, tr = quad * 32 + lane;  // half, lane quadrant, row
+    const uint32_t lanes = (uint32_t)(quad * 32) << 16;
+    const uint32_t ts = tmem + lanes + 128 * w, to = tmem + lanes + 256 + DP * w;
+    const float turn = a.scale < 0.f ? -1.f : 1.f, rs = a.scale * turn * kLog2e;
+    const uint32_t flip = turn < 0.f ? 0x80008000u : 0u;
+    uint32_t sph = 0, oph = 0;
+    const int D = a.head_dim;
+    each_tile([&](int tile, int k0, int k1) {
+      if (w >= halves_of(tile)) return true;
+      const int kh = tile / p.row_tiles, r = (tile % p.row_tiles) * 2 * kRows + w * kRows + tr;
+      const bool real = r < p.rows;
+      const int bt = real ? r / p.group : 0, h = kh * p.group + (real ? r - bt * p.group : 0);
+      const int b = bt / (int)a.tokens, t = bt - b * (int)a.tokens;
+      // ---- this thread's query row, K-major with the 128-byte swizzle
+      {
+        const __nv_bfloat16* q =
+            static_cast<const __nv_bfloat16*>(a.q.p) + b * a.q.sb + t * a.q.st + h * a.q.sh;
+        uint8_t* row = sq + w * C::TILE + tr * 128;
+#pragma unroll
+        for (int c = 0; c < DP / 8; ++c) {
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (real && c * 8 < D) v = *reinterpret_cast<const uint4*>(q + c * 8);
+          v.x ^= flip, v.y ^= flip, v.z ^= flip, v.w ^= flip;
+          *reinterpret_cast<uint4*>(row + (c >> 3) * C::SUB + (((c & 7) ^ (tr & 7)) << 4)) = v;
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&S->qready[w]);
+      }
+      float m = -INFINITY, l = 0.f;  // fixed maximum (before rs), sum
+      int ok = 1;
+      for (int k = k0; k < k1; ++k) {
+        if (lane == 0) ok = wait(&S->sfull[w], sph);
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+        if (!ok) break;
+        sph ^= 1u;
+        fence_after();
+        uint32_t s[4][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld32(ts + 32 * c, s[c]);
+        tmem_wait_ld();
+        const int left = (int)a.prefix_cols - k * kKeys;  // keys of this tile
+        if (left < kKeys) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (c * 32 + i >= left) s[c][i] = 0xff800000u;  // -inf
+        }
+        float mx = m;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(s[c][i]));
+        const bool first = k == k0;
+        const bool grow = first || (mx - m) * rs > kGrow;
+        if (first) {
+          m = mx;
+        } else if (__any_sync(0xffffffffu, grow)) {
+          // the scores' completion covers every product before them: O is at rest
+          const float f = grow ? ex2((m - mx) * rs) : 1.f;
+          if (grow) m = mx;
+          l *= f;
+#pragma unroll
+          for (int c = 0; c < DP / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld32(to + 32 * c, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+            tmem_st32(to + 32 * c, o);
+          }
+        }
+        const float base = m == -INFINITY ? 0.f : m * rs;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t pk[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const int e = 2 * i;
+            const float x = ex2(fmaf(__uint_as_float(s[2 * c + (e >> 5)][e & 31]), rs, -base));
+            const float y = ex2(fmaf(__uint_as_float(s[2 * c + (e >> 5)][(e + 1) & 31]), rs, -base));
+            l += x + y;
+            pk[i] = pack_bf16x2(x, y);
+          }
+          tmem_st32(ts + 32 * c, pk);
+        }
+        tmem_wait_st();
+        fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&S->pfull[w]);
+      }
+      // ---- the run's result to its slot; slots behind the tile's last are empty
+      if (ok) {
+        if (lane == 0) ok = wait(&S->ofull[w], oph);
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+        oph ^= 1u;
+      }
+      fence_after();
+      const int64_t x0 = (int64_t)tile * p.key_tiles;
+      const int slot = (int)blockIdx.x - (int)(((x0 + 1) * gridDim.x - 1) / p.units);
+      const int64_t orow = ((int64_t)b * a.tokens + t) * a.q_heads + h;
+      if (real) {
+        const float mb = m == -INFINITY ? m : m * rs;
+        // a wait that ran out leaves a result that cannot be missed
+        p.part_ml[slot * p.out_rows + orow] =
+            ok ? make_float2(mb, l) : make_float2(0.f, __int_as_float(0x7fffffff));
+        if (k1 == p.key_tiles)
+          for (int e = slot + 1; e < p.slots; ++e)
+            p.part_ml[e * p.out_rows + orow] = make_float2(-INFINITY, 0.f);
+      }
+      if (!ok) return false;
+      float* out = p.part_o + (slot * p.out_rows + orow) * D;
+#pragma unroll
+      for (int c = 0; c < DP / 32; ++c) {
+        uint32_t o[32];
+        tmem_ld32(to + 32 * c, o);
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 32; i += 4)
+          if (real && c * 32 + i < D)
+            *reinterpret_cast<uint4*>(out + c * 32 + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+      }
+      fence_before();
+      return true;
+    });
+  }
+  // every warp arrives, so no copy, product or TMEM access is left when TMEM goes
+  fence_before();
+  __syncthreads();
+  fence_after();
+  if (wp == 8)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+}
+
+template <int DP>
+int launch(const Args& p, int ctas, cudaStream_t st) {
+  const AttnArgs& a = p.a;
+  CUtensorMap tk, tv;
+  const uint64_t dims[3] = {(uint64_t)a.head_dim, (uint64_t)a.prefix_cols, (uint64_t)a.kv_heads};
+  const uint32_t box[3] = {64, kKeys, 1};
+  if (int rc = encode_bf16_3d(&tk, a.kp, dims, box)) return rc;
+  if (int rc = encode_bf16_3d(&tv, a.vp, dims, box)) return rc;
+  const cudaError_t e = cudaFuncSetAttribute(
+      k_attn_prefix_tc<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<DP>::SMEM);
+  if (e != cudaSuccess) return (int)e;
+  k_attn_prefix_tc<DP><<<ctas, kThreads, Cfg<DP>::SMEM, st>>>(tk, tv, p);
+  return 0;
+}
+
+}  // namespace px
+}  // namespace
+
+constexpr int kMinUnits = 4;  // units of a CTA, at least (while the others suffice)
+
+PrefixTcPlan plan_prefix_tc(int64_t rows, int kv_heads, int64_t prefix_cols) {
+  const int64_t key_tiles = (prefix_cols + px::kKeys - 1) / px::kKeys;
+  const int64_t units = kv_heads * ((rows + 2 * px::kRows - 1) / (2 * px::kRows)) * key_tiles;
+  PrefixTcPlan p;
+  const int64_t most = (units + kMinUnits - 1) / kMinUnits;
+  p.ctas = (int)(most < 148 ? most : 148);
+  // a tile's key tiles lie in at most so many runs of units / ctas or more
+  const int64_t run = units / p.ctas;
+  const int64_t slots = (key_tiles - 1 + run - 1) / run + 1;
+  p.slots = (int)(slots < key_tiles ? slots : key_tiles);
+  return p;
+}
+
+int launch_prefix_tc(const AttnArgs& a, const PrefixTcPlan& plan, int64_t out_rows, float* part_o,
+                     float2* part_ml, cudaStream_t st) {
+  px::Args p{a, a.q_heads / a.kv_heads, 0, 0, 0, plan.slots, 0, out_rows, part_o, part_ml};
+  p.rows = (int)(a.batch * a.tokens * p.group);
+  p.row_tiles = (p.rows + 2 * px::kRows - 1) / (2 * px::kRows);
+  p.key_tiles = (int)((a.prefix_cols + px::kKeys - 1) / px::kKeys);
+  p.units = (int64_t)a.kv_heads * p.row_tiles * p.key_tiles;
+  return a.head_dim <= 64 ? px::launch<64>(p, plan.ctas, st) : px::launch<128>(p, plan.ctas, st);
+}
+
+}  // namespace mep

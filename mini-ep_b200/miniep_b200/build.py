@@ -25,7 +25,7 @@ OBJ = ROOT / "_build"
 
 SOURCES = ["mep_api.cu", "mep_router.cu", "mep_router_tc.cu", "mep_route.cu", "mep_move.cu",
            "mep_ffn.cu", "mep_noalloc.cu", "mep_norm.cu", "mep_kv.cu", "mep_attn.cu",
-           "mep_sample.cu"]
+           "mep_attn_tc.cu", "mep_sample.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-std=c++17", "-O3", "-lineinfo", "-Xcompiler", "-fPIC,-O2", "--expt-relaxed-constexpr"]
 

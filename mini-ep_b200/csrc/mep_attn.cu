@@ -106,6 +106,12 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
+__device__ __forceinline__ void store4(float* p, float a, float b, float c, float d) {
+  *reinterpret_cast<float4*>(p) = make_float4(a, b, c, d);
+}
+__device__ __forceinline__ void store4(__nv_bfloat16* p, float a, float b, float c, float d) {
+  *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16(a, b), pack_bf16(c, d));
+}
 __device__ __forceinline__ float quad_max(float x) {
   x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
   return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
@@ -161,7 +167,7 @@ struct Tile {
   // registers), rows 4 floats apart in the banks
   static constexpr int kQRow = DP + 4;
   static constexpr int kQBytes = kF32 ? kRows * kQRow * 4 : 0;
-  static constexpr int kJoin = KS ? 5 * 16 * (DP * 4 + 8) : 0;
+  static constexpr int kJoin = KS ? 5 * 16 * (DP * 4 + 8) : 64 * ((DP + 4) * 4 + 8);
   static constexpr int kBody = kStages * kStageBytes + kQBytes;
   static constexpr int kSmem = kBody > kJoin ? kBody : kJoin;
   // place of 16-byte chunk c of staged row r, so that the accesses of a warp
@@ -175,6 +181,17 @@ struct Tile {
     return kRow >= 128 ? c ^ (r & 7) : c ^ ((r >> 1) & 3);
   }
 };
+
+// x += y's values, in units of 2^base, times `times`. The load does not wait for
+// ml: an empty slot's values are unwritten and left out.
+__device__ __forceinline__ void add_part(float4& x, float2 ml, float base, float times,
+                                         const float* values) {
+  const float4 y = *reinterpret_cast<const float4*>(values);
+  if (ml.y != 0.f) {
+    const float f = ex2(ml.x - base) * times;
+    x.x += y.x * f, x.y += y.y * f, x.z += y.z * f, x.w += y.w * f;
+  }
+}
 
 template <typename QT, typename CT, int DP, bool KS, bool PREFIX>
 __global__ void __launch_bounds__(kThreads) k_attn_part(const PartArgs p) {
@@ -711,67 +728,84 @@ __global__ void __launch_bounds__(kThreads) k_attn_part(const PartArgs p) {
         mm = fmaxf(mm, (p.splits > 1 ? cluster.map_shared_rank(cm, c) : cm)[r].x);
       for (int c = 0; c < p.extra; ++c) mm = fmaxf(mm, p.part_ml[c * p.out_rows + orow].x);
       const float base = mm == -INFINITY ? 0.f : mm;
-      float x[4] = {};
-      auto add = [&](float2 ml, float4 y) {
-        const float f = ex2(ml.x - base);
-        ll += ml.y * f;
-        x[0] += y.x * f, x[1] += y.y * f, x[2] += y.z * f, x[3] += y.w * f;
-      };
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
       for (int c = 0; c < p.extra; ++c) {
         const int64_t slot = c * p.out_rows + orow;
-        const float2 ml = p.part_ml[slot];  // an empty slot's values are unwritten
-        if (ml.y != 0.f) add(ml, *reinterpret_cast<const float4*>(p.part_o + slot * D + d));
+        const float2 ml = p.part_ml[slot];
+        add_part(x, ml, base, 1.f, p.part_o + slot * D + d);
+        ll += ml.y * ex2(ml.x - base);
       }
       for (int c = 0; c < p.splits; ++c) {
-        const float2* fm = p.splits > 1 ? cluster.map_shared_rank(cm, c) : cm;
-        const float* fo = p.splits > 1 ? cluster.map_shared_rank(co, c) : co;
-        add(fm[r], *reinterpret_cast<const float4*>(fo + r * DP + d));
+        const float2 ml = (p.splits > 1 ? cluster.map_shared_rank(cm, c) : cm)[r];
+        add_part(x, ml, base, 1.f, (p.splits > 1 ? cluster.map_shared_rank(co, c) : co) + r * DP + d);
+        ll += ml.y * ex2(ml.x - base);
       }
       const float inv = ll == 0.f ? 0.f : 1.f / ll;
-      QT* out = static_cast<QT*>(a.out) + orow * D + d;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) out[e] = Elt<QT>::from_f(x[e] * inv);
+      store4(static_cast<QT*>(a.out) + orow * D + d, x.x * inv, x.y * inv, x.z * inv, x.w * inv);
     }
     if (p.splits > 1) cluster.sync();  // nobody leaves while its sums are read
-  } else {
+  } else if (!p.joined) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       if (row[u] >= rN) continue;
-      const int64_t orow = out_row(row[u]);
-      const int64_t slot = (p.extra + split) * p.out_rows + orow;
-      if (p.joined && p.extra) {
-        float mm = m[u];
-        for (int c = 0; c < p.extra; ++c) mm = fmaxf(mm, p.part_ml[c * p.out_rows + orow].x);
-        const float base = mm == -INFINITY ? 0.f : mm, f0 = ex2(m[u] - base);
-        l[u] *= f0;
-#pragma unroll
-        for (int i = 0; i < OT; ++i) o[i][2 * u] *= f0, o[i][2 * u + 1] *= f0;
-        for (int c = 0; c < p.extra; ++c) {
-          const float2 ml = p.part_ml[c * p.out_rows + orow];
-          if (ml.y == 0.f) continue;  // empty: its values are unwritten
-          const float f = ex2(ml.x - base);
-          l[u] += ml.y * f;
-          const float* y = p.part_o + (c * p.out_rows + orow) * D;
-#pragma unroll
-          for (int i = 0; i < OT; ++i)
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-              if (value_of(i, j) < D) o[i][2 * u + j] += y[value_of(i, j)] * f;
-        }
-      }
-      const float inv = l[u] == 0.f ? 0.f : 1.f / l[u];
+      const int64_t slot = (p.extra + split) * p.out_rows + out_row(row[u]);
 #pragma unroll
       for (int i = 0; i < OT; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int d = value_of(i, j);
-          if (d >= D) continue;
-          if (!p.joined)
-            p.part_o[slot * D + d] = o[i][2 * u + j];
-          else
-            static_cast<QT*>(a.out)[orow * D + d] = Elt<QT>::from_f(o[i][2 * u + j] * inv);
-        }
-      if (!p.joined && t4 == 0) p.part_ml[slot] = make_float2(m[u], l[u]);
+        for (int j = 0; j < 2; ++j)
+          if (value_of(i, j) < D) p.part_o[slot * D + value_of(i, j)] = o[i][2 * u + j];
+      if (t4 == 0) p.part_ml[slot] = make_float2(m[u], l[u]);
+    }
+  } else {
+    // ---- 64 rows to shared memory, then joined with the extra partial
+    // results and written four values a thread
+    __syncthreads();
+    float* co = reinterpret_cast<float*>(smem);  // [64][DP + 4]
+    float2* cm = reinterpret_cast<float2*>(smem + 64 * (DP + 4) * 4);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int r = wrow + g + 8 * u;
+#pragma unroll
+      for (int i = 0; i < OT; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) co[r * (DP + 4) + value_of(i, j)] = o[i][2 * u + j];
+      if (t4 == 0) cm[r] = make_float2(m[u], l[u]);
+    }
+    __syncthreads();
+    // a row's joint maximum and the inverse of its sum
+    if (threadIdx.x < nrow) {
+      const float2 own = cm[threadIdx.x];
+      const int64_t orow = out_row(r0 + threadIdx.x);
+      float mm = own.x;
+      for (int c = 0; c < p.extra; ++c) mm = fmaxf(mm, p.part_ml[c * p.out_rows + orow].x);
+      const float base = mm == -INFINITY ? 0.f : mm;
+      float ll = own.y * ex2(own.x - base);
+      for (int c = 0; c < p.extra; ++c) {
+        const float2 ml = p.part_ml[c * p.out_rows + orow];
+        ll += ml.y * ex2(ml.x - base);
+      }
+      const float inv = ll == 0.f ? 0.f : 1.f / ll;
+      cm[threadIdx.x] = make_float2(base, inv);
+      co[threadIdx.x * (DP + 4) + DP] = ex2(own.x - base) * inv;
+      *reinterpret_cast<int*>(&co[threadIdx.x * (DP + 4) + DP + 1]) = (int)orow;
+    }
+    __syncthreads();
+    const int quads = D >> 2;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < nrow * quads; i += kThreads) {
+      const int r = i / quads, d = (i - r * quads) * 4;
+      const float2 bi = cm[r];
+      const float* own = co + r * (DP + 4);
+      const int64_t orow = *reinterpret_cast<const int*>(own + DP + 1);
+      const float f0 = own[DP];
+      float4 x = *reinterpret_cast<const float4*>(own + d);
+      x.x *= f0, x.y *= f0, x.z *= f0, x.w *= f0;
+      for (int c = 0; c < p.extra; ++c) {
+        const int64_t slot = c * p.out_rows + orow;
+        add_part(x, p.part_ml[slot], bi.x, bi.y, p.part_o + slot * D + d);
+      }
+      store4(static_cast<QT*>(a.out) + orow * D + d, x.x, x.y, x.z, x.w);
     }
   }
 }

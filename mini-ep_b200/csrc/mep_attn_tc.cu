@@ -52,7 +52,7 @@ struct Cfg {
 
 struct Smem {
   uint64_t kfull[4], kempty[4], vfull[4], vempty[4];
-  uint64_t qready[2], sfull[2], pfull[2], ofull[2];
+  uint64_t qready[2], sfull[2], pfull[2][2], ofull[2];
   uint32_t tmem_base;
   int abort;
 };
@@ -104,6 +104,47 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
       "r"(r[30]), "r"(r[31])
       : "memory");
 }
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+      : "memory");
+}
+// two fp32 values an instruction
+__device__ __forceinline__ uint64_t pair(float x, float y) {
+  return (uint64_t)__float_as_uint(y) << 32 | __float_as_uint(x);
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& x, float& y) {
+  x = __uint_as_float((uint32_t)v), y = __uint_as_float((uint32_t)(v >> 32));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+// 2^x for x <= 2^7 by rounding to an integer n and a polynomial in the rest r:
+// the Taylor terms of 2^r up to r^4 leave 2^-14.5 of it at |r| = 1/2, against the
+// 2^-9 of the bf16 weights. Below 2^-126 the result is not zero but 2^-126.
+__device__ __forceinline__ float ex2_poly(float x) {
+  x = fmaxf(x, -126.f);
+  const float t = x + 12582912.f;  // 1.5 * 2^23: n in the low bits
+  const float r = x - (t - 12582912.f);
+  constexpr float l2 = 0.6931471805599453f;
+  const float y = fmaf(r, fmaf(r, fmaf(r, fmaf(r, l2 * l2 * l2 * l2 / 24, l2 * l2 * l2 / 6),
+                                       l2 * l2 / 2), l2), 1.f);
+  return __uint_as_float(__float_as_uint(y) + ((uint32_t)__float_as_int(t) << 23));
+}
 __device__ __forceinline__ void tmem_wait_st() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
@@ -129,7 +170,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int w = 0; w < 2; ++w) {
       mbar_init(&S->qready[w], 4), mbar_init(&S->sfull[w], 1);
-      mbar_init(&S->pfull[w], 4), mbar_init(&S->ofull[w], 1);
+      mbar_init(&S->pfull[w][0], 4), mbar_init(&S->pfull[w][1], 4);
+      mbar_init(&S->ofull[w], 1);
     }
     S->abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -223,14 +265,18 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!wait(&S->vfull[vs], vph)) return false;
           if (more && !wait(&S->kfull[ks], kph)) return false;
           for (int w = 0; w < halves; ++w) {
-            if (!wait(&S->pfull[w], pph[w])) return false;
-            pph[w] ^= 1u;
-            fence_after();
+            // the weights of 64 keys at a time
 #pragma unroll
-            for (int kk = 0; kk < kKeys / 16; ++kk)
-              mma_f16_ts(tmem + 256 + DP * w, tmem + 128 * w + kk * 8,
-                         v_desc(v_0 + vs * C::TILE + kk * 2048, C::SUB), C::IDESC_O,
-                         k != k0 || kk != 0);
+            for (int part = 0; part < 2; ++part) {
+              if (!wait(&S->pfull[w][part], pph[w])) return false;
+              fence_after();
+#pragma unroll
+              for (int kk = part * 4; kk < part * 4 + 4; ++kk)
+                mma_f16_ts(tmem + 256 + DP * w, tmem + 128 * w + kk * 8,
+                           v_desc(v_0 + vs * C::TILE + kk * 2048, C::SUB), C::IDESC_O,
+                           k != k0 || kk != 0);
+            }
+            pph[w] ^= 1u;
             // the tile's last arrival is ofull's: nothing arrives behind it
             if (w == halves - 1) mma_commit<false>(&S->vempty[vs]);
             if (more)
@@ -298,11 +344,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int i = 0; i < 32; ++i)
               if (c * 32 + i >= left) s[c][i] = 0xff800000u;  // -inf
         }
-        float mx = m;
+        // four chains of maxima at a time
+        float mx4[4] = {m, m, m, m};
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+        for (int i = 0; i < 32; ++i)
 #pragma unroll
-          for (int i = 0; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(s[c][i]));
+          for (int c = 0; c < 4; ++c) mx4[c] = fmaxf(mx4[c], __uint_as_float(s[c][i]));
+        const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
         const bool first = k == k0;
         const bool grow = first || (mx - m) * rs > kGrow;
         if (first) {
@@ -312,34 +360,48 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float f = grow ? ex2((m - mx) * rs) : 1.f;
           if (grow) m = mx;
           l *= f;
-#pragma unroll
-          for (int c = 0; c < DP / 32; ++c) {
-            uint32_t o[32];
-            tmem_ld32(to + 32 * c, o);
+#pragma unroll 1
+          for (int c = 0; c < DP; c += 8) {
+            uint32_t o[8];
+            tmem_ld8(to + c, o);
             tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-            tmem_st32(to + 32 * c, o);
+            for (int i = 0; i < 8; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+            tmem_st8(to + c, o);
           }
         }
         const float base = m == -INFINITY ? 0.f : m * rs;
+        const uint64_t rs2 = pair(rs, rs), nb2 = pair(-base, -base);
+        uint64_t sum[2] = {0, 0};  // (0.f, 0.f)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           uint32_t pk[32];
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
-            const int e = 2 * i;
-            const float x = ex2(fmaf(__uint_as_float(s[2 * c + (e >> 5)][e & 31]), rs, -base));
-            const float y = ex2(fmaf(__uint_as_float(s[2 * c + (e >> 5)][(e + 1) & 31]), rs, -base));
-            l += x + y;
+            const int e = (2 * i) & 31;
+            const uint32_t(&src)[32] = s[2 * c + (i >> 4)];
+            float x, y;
+            unpair(fma2((uint64_t)src[e + 1] << 32 | src[e], rs2, nb2), x, y);
+            // a quarter of the exponentials on the FMA pipe: the other unit
+            // does 16 a clock of an SM, and 256 x 128 of them take as long as
+            // the tile's products (64-wide heads: twice that)
+            if ((i & 3) == 3) {
+              x = ex2_poly(x), y = ex2_poly(y);
+            } else {
+              x = ex2(x), y = ex2(y);
+            }
+            sum[i & 1] = add2(sum[i & 1], pair(x, y));
             pk[i] = pack_bf16x2(x, y);
           }
           tmem_st32(ts + 32 * c, pk);
+          tmem_wait_st();
+          fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&S->pfull[w][c]);
         }
-        tmem_wait_st();
-        fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&S->pfull[w]);
+        float x, y;
+        unpair(add2(sum[0], sum[1]), x, y);
+        l += x + y;
       }
       // ---- the run's result to its slot; slots behind the tile's last are empty
       if (ok) {

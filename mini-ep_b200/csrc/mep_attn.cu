@@ -184,9 +184,13 @@ struct Tile {
 
 // x += y's values, in units of 2^base, times `times`. The load does not wait for
 // ml: an empty slot's values are unwritten and left out.
+// kGlobal: from an earlier launch, through the read-only path, so that the
+// loads of several values need not wait for the stores between them.
+template <bool kGlobal>
 __device__ __forceinline__ void add_part(float4& x, float2 ml, float base, float times,
                                          const float* values) {
-  const float4 y = *reinterpret_cast<const float4*>(values);
+  const float4 y = kGlobal ? __ldg(reinterpret_cast<const float4*>(values))
+                           : *reinterpret_cast<const float4*>(values);
   if (ml.y != 0.f) {
     const float f = ex2(ml.x - base) * times;
     x.x += y.x * f, x.y += y.y * f, x.z += y.z * f, x.w += y.w * f;
@@ -726,19 +730,19 @@ __global__ void __launch_bounds__(kThreads) k_attn_part(const PartArgs p) {
       float mm = -INFINITY, ll = 0.f;
       for (int c = 0; c < p.splits; ++c)
         mm = fmaxf(mm, (p.splits > 1 ? cluster.map_shared_rank(cm, c) : cm)[r].x);
-      for (int c = 0; c < p.extra; ++c) mm = fmaxf(mm, p.part_ml[c * p.out_rows + orow].x);
+      for (int c = 0; c < p.extra; ++c) mm = fmaxf(mm, __ldg(p.part_ml + c * p.out_rows + orow).x);
       const float base = mm == -INFINITY ? 0.f : mm;
       float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
       for (int c = 0; c < p.extra; ++c) {
         const int64_t slot = c * p.out_rows + orow;
-        const float2 ml = p.part_ml[slot];
-        add_part(x, ml, base, 1.f, p.part_o + slot * D + d);
+        const float2 ml = __ldg(p.part_ml + slot);
+        add_part<true>(x, ml, base, 1.f, p.part_o + slot * D + d);
         ll += ml.y * ex2(ml.x - base);
       }
       for (int c = 0; c < p.splits; ++c) {
         const float2 ml = (p.splits > 1 ? cluster.map_shared_rank(cm, c) : cm)[r];
-        add_part(x, ml, base, 1.f, (p.splits > 1 ? cluster.map_shared_rank(co, c) : co) + r * DP + d);
+        add_part<false>(x, ml, base, 1.f, (p.splits > 1 ? cluster.map_shared_rank(co, c) : co) + r * DP + d);
         ll += ml.y * ex2(ml.x - base);
       }
       const float inv = ll == 0.f ? 0.f : 1.f / ll;
@@ -778,11 +782,11 @@ __global__ void __launch_bounds__(kThreads) k_attn_part(const PartArgs p) {
       const float2 own = cm[threadIdx.x];
       const int64_t orow = out_row(r0 + threadIdx.x);
       float mm = own.x;
-      for (int c = 0; c < p.extra; ++c) mm = fmaxf(mm, p.part_ml[c * p.out_rows + orow].x);
+      for (int c = 0; c < p.extra; ++c) mm = fmaxf(mm, __ldg(p.part_ml + c * p.out_rows + orow).x);
       const float base = mm == -INFINITY ? 0.f : mm;
       float ll = own.y * ex2(own.x - base);
       for (int c = 0; c < p.extra; ++c) {
-        const float2 ml = p.part_ml[c * p.out_rows + orow];
+        const float2 ml = __ldg(p.part_ml + c * p.out_rows + orow);
         ll += ml.y * ex2(ml.x - base);
       }
       const float inv = ll == 0.f ? 0.f : 1.f / ll;
@@ -792,7 +796,7 @@ __global__ void __launch_bounds__(kThreads) k_attn_part(const PartArgs p) {
     }
     __syncthreads();
     const int quads = D >> 2;
-#pragma unroll 4
+#pragma unroll 8
     for (int i = threadIdx.x; i < nrow * quads; i += kThreads) {
       const int r = i / quads, d = (i - r * quads) * 4;
       const float2 bi = cm[r];
@@ -803,7 +807,7 @@ __global__ void __launch_bounds__(kThreads) k_attn_part(const PartArgs p) {
       x.x *= f0, x.y *= f0, x.z *= f0, x.w *= f0;
       for (int c = 0; c < p.extra; ++c) {
         const int64_t slot = c * p.out_rows + orow;
-        add_part(x, p.part_ml[slot], bi.x, bi.y, p.part_o + slot * D + d);
+        add_part<true>(x, __ldg(p.part_ml + slot), bi.x, bi.y, p.part_o + slot * D + d);
       }
       store4(static_cast<QT*>(a.out) + orow * D + d, x.x, x.y, x.z, x.w);
     }

@@ -52,7 +52,7 @@ struct Cfg {
 
 struct Smem {
   uint64_t kfull[4], kempty[4], vfull[4], vempty[4];
-  uint64_t qready[2], sfull[2], pfull[2][2], ofull[2];
+  uint64_t qready[2], sfull[2], pfull[2][2], ofull[2], qfree[2];
   uint32_t tmem_base;
   int abort;
 };
@@ -116,6 +116,18 @@ __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8])
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
       : "memory");
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void bulk_wait_read() {
+  asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+}
 // two fp32 values an instruction
 __device__ __forceinline__ uint64_t pair(float x, float y) {
   return (uint64_t)__float_as_uint(y) << 32 | __float_as_uint(x);
@@ -132,18 +144,6 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t d;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
-}
-// 2^x for x <= 2^7 by rounding to an integer n and a polynomial in the rest r:
-// the Taylor terms of 2^r up to r^4 leave 2^-14.5 of it at |r| = 1/2, against the
-// 2^-9 of the bf16 weights. Below 2^-126 the result is not zero but 2^-126.
-__device__ __forceinline__ float ex2_poly(float x) {
-  x = fmaxf(x, -126.f);
-  const float t = x + 12582912.f;  // 1.5 * 2^23: n in the low bits
-  const float r = x - (t - 12582912.f);
-  constexpr float l2 = 0.6931471805599453f;
-  const float y = fmaf(r, fmaf(r, fmaf(r, fmaf(r, l2 * l2 * l2 * l2 / 24, l2 * l2 * l2 / 6),
-                                       l2 * l2 / 2), l2), 1.f);
-  return __uint_as_float(__float_as_uint(y) + ((uint32_t)__float_as_int(t) << 23));
 }
 __device__ __forceinline__ void tmem_wait_st() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -171,7 +171,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int w = 0; w < 2; ++w) {
       mbar_init(&S->qready[w], 4), mbar_init(&S->sfull[w], 1);
       mbar_init(&S->pfull[w][0], 4), mbar_init(&S->pfull[w][1], 4);
-      mbar_init(&S->ofull[w], 1);
+      mbar_init(&S->ofull[w], 1), mbar_init(&S->qfree[w], 4);
     }
     S->abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -300,7 +300,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t ts = tmem + lanes + 128 * w, to = tmem + lanes + 256 + DP * w;
     const float turn = a.scale < 0.f ? -1.f : 1.f, rs = a.scale * turn * kLog2e;
     const uint32_t flip = turn < 0.f ? 0x80008000u : 0u;
-    uint32_t sph = 0, oph = 0;
+    uint32_t sph = 0, oph = 0, fph = 1;
     const int D = a.head_dim;
     each_tile([&](int tile, int k0, int k1) {
       if (w >= halves_of(tile)) return true;
@@ -308,8 +308,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool real = r < p.rows;
       const int bt = real ? r / p.group : 0, h = kh * p.group + (real ? r - bt * p.group : 0);
       const int b = bt / (int)a.tokens, t = bt - b * (int)a.tokens;
-      // ---- this thread's query row, K-major with the 128-byte swizzle
-      {
+      // ---- this thread's query row, K-major with the 128-byte swizzle, once the
+      // half's four warps have written the last tile's results out of the buffer
+      int ok = 1;
+      if (lane == 0) ok = wait(&S->qfree[w], fph);
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+      fph ^= 1u;
+      if (ok) {
         const __nv_bfloat16* q =
             static_cast<const __nv_bfloat16*>(a.q.p) + b * a.q.sb + t * a.q.st + h * a.q.sh;
         uint8_t* row = sq + w * C::TILE + tr * 128;
@@ -325,8 +330,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive(&S->qready[w]);
       }
       float m = -INFINITY, l = 0.f;  // fixed maximum (before rs), sum
-      int ok = 1;
-      for (int k = k0; k < k1; ++k) {
+      for (int k = k0; ok && k < k1; ++k) {
         if (lane == 0) ok = wait(&S->sfull[w], sph);
         ok = __shfl_sync(0xffffffffu, ok, 0);
         if (!ok) break;
@@ -382,14 +386,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t(&src)[32] = s[2 * c + (i >> 4)];
             float x, y;
             unpair(fma2((uint64_t)src[e + 1] << 32 | src[e], rs2, nb2), x, y);
-            // a quarter of the exponentials on the FMA pipe: the other unit
-            // does 16 a clock of an SM, and 256 x 128 of them take as long as
-            // the tile's products (64-wide heads: twice that)
-            if ((i & 3) == 3) {
-              x = ex2_poly(x), y = ex2_poly(y);
-            } else {
-              x = ex2(x), y = ex2(y);
-            }
+            x = ex2(x), y = ex2(y);
             sum[i & 1] = add2(sum[i & 1], pair(x, y));
             pk[i] = pack_bf16x2(x, y);
           }
@@ -423,20 +420,37 @@ __global__ void __launch_bounds__(kThreads, 1)
             p.part_ml[e * p.out_rows + orow] = make_float2(-INFINITY, 0.f);
       }
       if (!ok) return false;
+      // O through the half's query buffer, which nothing reads any more: W
+      // values of each row at a time, a bulk store a row
+      constexpr int W = DP / 4, STRIDE = W * 4 + 16;  // 16: rows in other banks
+      static_assert(kRows * STRIDE <= C::TILE, "O passes fit the query buffer");
+      uint8_t* row = sq + w * C::TILE + tr * STRIDE;
       float* out = p.part_o + (slot * p.out_rows + orow) * D;
-#pragma unroll
-      for (int c = 0; c < DP / 32; ++c) {
-        uint32_t o[32];
-        tmem_ld32(to + 32 * c, o);
+#pragma unroll 1
+      for (int c = 0; c < DP; c += W) {
+        uint32_t o[W];
+        __syncwarp();  // the warp's loads are collective; rows past the last store nothing
+        if constexpr (W == 32)
+          tmem_ld32(to + c, o);
+        else
+          tmem_ld16(to + c, o);
         tmem_wait_ld();
+        bulk_wait_read();  // the last pass has left the buffer
 #pragma unroll
-        for (int i = 0; i < 32; i += 4)
-          if (real && c * 32 + i < D)
-            *reinterpret_cast<uint4*>(out + c * 32 + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+        for (int i = 0; i < W; i += 4)
+          *reinterpret_cast<uint4*>(row + i * 4) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        const int n = min(W, D - c);
+        if (real && n > 0) bulk_store_s2g(out + c, row, n * 4);
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
       }
+      bulk_wait_read();
       fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&S->qfree[w]);
       return true;
     });
+    asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
   // every warp arrives, so no copy, product or TMEM access is left when TMEM goes
   fence_before();

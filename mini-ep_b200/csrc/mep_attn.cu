@@ -795,21 +795,36 @@ __global__ void __launch_bounds__(kThreads) k_attn_part(const PartArgs p) {
       *reinterpret_cast<int*>(&co[threadIdx.x * (DP + 4) + DP + 1]) = (int)orow;
     }
     __syncthreads();
+    // kBatch pieces of four values a thread at a time, their loads together
     const int quads = D >> 2;
-#pragma unroll 8
-    for (int i = threadIdx.x; i < nrow * quads; i += kThreads) {
-      const int r = i / quads, d = (i - r * quads) * 4;
-      const float2 bi = cm[r];
-      const float* own = co + r * (DP + 4);
-      const int64_t orow = *reinterpret_cast<const int*>(own + DP + 1);
-      const float f0 = own[DP];
-      float4 x = *reinterpret_cast<const float4*>(own + d);
-      x.x *= f0, x.y *= f0, x.z *= f0, x.w *= f0;
-      for (int c = 0; c < p.extra; ++c) {
-        const int64_t slot = c * p.out_rows + orow;
-        add_part<true>(x, __ldg(p.part_ml + slot), bi.x, bi.y, p.part_o + slot * D + d);
+    constexpr int kBatch = 8;
+    for (int i0 = threadIdx.x; i0 < nrow * quads; i0 += kBatch * kThreads) {
+      float4 x[kBatch];
+      int64_t orow[kBatch];
+      int mrow[kBatch];
+      float2 bi[kBatch];
+#pragma unroll
+      for (int e = 0; e < kBatch; ++e) {
+        const int i = min(i0 + e * kThreads, nrow * quads - 1), r = i / quads;
+        const float* own = co + r * (DP + 4);
+        bi[e] = cm[r];
+        orow[e] = *reinterpret_cast<const int*>(own + DP + 1);
+        mrow[e] = (int)orow[e];
+        x[e] = *reinterpret_cast<const float4*>(own + (i - r * quads) * 4);
+        x[e].x *= own[DP], x[e].y *= own[DP], x[e].z *= own[DP], x[e].w *= own[DP];
+        orow[e] = orow[e] * D + (i - r * quads) * 4;
       }
-      store4(static_cast<QT*>(a.out) + orow * D + d, x.x, x.y, x.z, x.w);
+      for (int c = 0; c < p.extra; ++c) {
+        const float* po = p.part_o + c * p.out_rows * D;
+        const float2* pm = p.part_ml + c * p.out_rows;
+#pragma unroll
+        for (int e = 0; e < kBatch; ++e)
+          add_part<true>(x[e], __ldg(pm + mrow[e]), bi[e].x, bi[e].y, po + orow[e]);
+      }
+#pragma unroll
+      for (int e = 0; e < kBatch; ++e)
+        if (i0 + e * kThreads < nrow * quads)
+          store4(static_cast<QT*>(a.out) + orow[e], x[e].x, x[e].y, x[e].z, x[e].w);
     }
   }
 }

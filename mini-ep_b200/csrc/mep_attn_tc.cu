@@ -5,14 +5,15 @@
 // exponentials, not by the prefix's bytes.
 //
 // A CTA has 256 rows (two halves of 128, the MMA's M) and walks tiles of 128
-// keys: S = Q K^T into TMEM, a thread a row takes the running maximum and the
-// exponentials, P goes back to TMEM over S as bf16 and is the A operand of
-// O += P V, which stays in TMEM. The halves alternate: while one's warps work
-// on exponentials, the tensor cores run the other's products. Q lies in shared
-// memory, K and V come by TMA through rings (a 3D tensor map, so that the last
-// tile's missing keys read as zeros). O is rescaled only when a row's maximum
-// has grown by more than 2^8 since it was last fixed: weights up to 2^8 are
-// as exact in bf16 and fp32 as weights up to 1.
+// keys in steps of 64: S = Q K^T into TMEM, a thread a row takes the running
+// maximum and the exponentials, P goes back to TMEM over S as bf16 and is the A
+// operand of O += P V, which stays in TMEM. Each half has two S buffers, so
+// that the next step's scores are there when a step's exponentials are done:
+// with one of 128 keys the products' latency (1900 of 4100 clocks a tile) lay
+// open. Q lies in shared memory, K and V come by TMA through rings (a 3D
+// tensor map, so that the last tile's missing keys read as zeros). O is
+// rescaled only when a row's maximum has grown by more than 2^8 since it was
+// last fixed: weights up to 2^8 are as exact in bf16 and fp32 as weights up to 1.
 //
 // Persistent: the (head, 256-row tile, key tile) units are dealt to the CTAs in
 // equal runs, so a tile's keys may be cut between CTAs. A run's result is a
@@ -33,7 +34,8 @@ using namespace ::mep::tc;
 
 constexpr int kRows = 128;   // rows of a half
 constexpr int kKeys = 128;   // keys of a tile
-constexpr int kThreads = 320;  // two softmax warpgroups, an MMA and a TMA warp
+constexpr int kStep = 64;    // keys of a step
+constexpr int kThreads = 352;  // two softmax warpgroups, an MMA warp for each, a TMA warp
 constexpr unsigned long long kWaitNs = 2000000000ull;
 constexpr float kGrow = 8.f;
 
@@ -46,13 +48,13 @@ struct Cfg {
   static constexpr int SMEM = DATA + 1024 + 1024;   // data | barriers | alignment slack
   // kind::f16, fp32 accumulators, bf16 operands, M = 128
   static constexpr uint32_t BASE = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(kRows >> 4) << 24);
-  static constexpr uint32_t IDESC_S = BASE | ((uint32_t)(kKeys >> 3) << 17);
+  static constexpr uint32_t IDESC_S = BASE | ((uint32_t)(kStep >> 3) << 17);
   static constexpr uint32_t IDESC_O = BASE | ((uint32_t)(DP >> 3) << 17) | (1u << 16);  // V: N-major
 };
 
 struct Smem {
   uint64_t kfull[4], kempty[4], vfull[4], vempty[4];
-  uint64_t qready[2], sfull[2], pfull[2][2], ofull[2], qfree[2];
+  uint64_t qready[2], qfree[2], sfull[2][2], pfull[2][2], odone[2], ofull[2];
   uint32_t tmem_base;
   int abort;
 };
@@ -83,25 +85,47 @@ __device__ __forceinline__ uint64_t v_desc(uint32_t saddr, uint32_t block_bytes)
   d |= (uint64_t)2 << 61;
   return d;
 }
-// A operand from TMEM
-__device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b,
-                                           uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(p));
+  return p != 0;
+}
+// Products from ready descriptors. ACC: 0 overwrite, 1 accumulate, 2 as `acc` says.
+template <int ACC>
+__device__ __forceinline__ void mma_ss(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(b), "r"(idesc), "r"(accumulate));
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a), "l"(b), "r"(idesc), "n"(ACC));
 }
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+// A operand from TMEM
+template <int ACC>
+__device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b,
+                                       uint32_t idesc, uint32_t acc) {
+  if (ACC == 2)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(b), "r"(idesc), "r"(acc));
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(b), "r"(idesc), "n"(ACC));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
-      "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
-      "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]),
-      "r"(r[30]), "r"(r[31])
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
 __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
@@ -124,9 +148,6 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
         "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
         "=r"(r[14]), "=r"(r[15])
       : "r"(taddr));
-}
-__device__ __forceinline__ void bulk_wait_read() {
-  asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
 }
 // two fp32 values an instruction
 __device__ __forceinline__ uint64_t pair(float x, float y) {
@@ -165,13 +186,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   const AttnArgs& a = p.a;
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::STAGES; ++s) {
-      mbar_init(&S->kfull[s], 1), mbar_init(&S->kempty[s], 1);
-      mbar_init(&S->vfull[s], 1), mbar_init(&S->vempty[s], 1);
+      mbar_init(&S->kfull[s], 1), mbar_init(&S->kempty[s], 2);
+      mbar_init(&S->vfull[s], 1), mbar_init(&S->vempty[s], 2);
     }
     for (int w = 0; w < 2; ++w) {
-      mbar_init(&S->qready[w], 4), mbar_init(&S->sfull[w], 1);
-      mbar_init(&S->pfull[w][0], 4), mbar_init(&S->pfull[w][1], 4);
-      mbar_init(&S->ofull[w], 1), mbar_init(&S->qfree[w], 4);
+      mbar_init(&S->qready[w], 4), mbar_init(&S->qfree[w], 4), mbar_init(&S->odone[w], 1);
+      mbar_init(&S->ofull[w], 1);
+      for (int i = 0; i < 2; ++i) mbar_init(&S->sfull[w][i], 1), mbar_init(&S->pfull[w][i], 4);
     }
     S->abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -186,7 +207,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   fence_before();
   __syncthreads();
   fence_after();
-  const uint32_t tmem = S->tmem_base;  // S of half w: columns 128 w; O: 256 + DP w
+  // S of half w, buffer i: columns 128 w + 64 i; O: 256 + DP w
+  const uint32_t tmem = S->tmem_base;
   auto wait = [&](uint64_t* b, uint32_t parity) {
     return mbar_wait_for(b, parity, kWaitNs, &S->abort);
   };
@@ -200,11 +222,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       u += k1 - k0;
     }
   };
+  // steps of key tiles [k0, k1): the last tile's second one may hold no key
+  auto steps_of = [&](int k0, int k1) {
+    return min(2 * (k1 - k0), ((int)a.prefix_cols - k0 * kKeys + kStep - 1) / kStep);
+  };
   auto halves_of = [&](int tile) {
     return p.rows - (tile % p.row_tiles) * 2 * kRows > kRows ? 2 : 1;
   };
 
-  if (wp == 9) {
+  if (wp == 10) {
     // ------------------------------------------------------------ TMA loads
     if (lane == 0) {
       int s = 0, issued = 0;
@@ -234,65 +260,87 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
     }
-  } else if (wp == 8) {
+  } else if (wp >= 8) {
     // ------------------------------------------------------------ MMA issue
-    if (lane == 0) {
-      int ks = 0, vs = 0;
-      uint32_t kph = 0, vph = 0, qph = 0, pph[2] = {0, 0};
-      const uint32_t q0 = smem_u32(sq), k_0 = smem_u32(sk), v_0 = smem_u32(sv);
-      auto scores = [&](int w, int stage) {
-#pragma unroll
-        for (int kk = 0; kk < DP / 16; ++kk) {
-          const uint32_t off = (kk >> 2) * C::SUB + (kk & 3) * 32;
-          mma_f16<false>(tmem + 128 * w, sw128_desc(q0 + w * C::TILE + off),
-                         sw128_desc(k_0 + stage * C::TILE + off), C::IDESC_S, kk != 0);
-        }
-        mma_commit<false>(&S->sfull[w]);
-      };
-      each_tile([&](int tile, int k0, int k1) {
-        const int halves = halves_of(tile);
-        if (!wait(&S->kfull[ks], kph)) return false;
-        for (int w = 0; w < halves; ++w) {
-          if (!wait(&S->qready[w], w == 0 ? qph & 1u : (qph >> 1) & 1u)) return false;
-          fence_after();
-          scores(w, ks);
-        }
-        qph ^= halves == 2 ? 3u : 1u;
-        mma_commit<false>(&S->kempty[ks]);
-        if (++ks == C::STAGES) ks = 0, kph ^= 1u;
+    // A warp for each half, so that one's waits do not hold up the other's
+    // products. The whole warp walks the steps, its elected lane issues: with
+    // operands that are the same in every lane an instruction takes the issuer
+    // some 50 clocks; from a branch of one lane it took 80, more than it ran.
+    const int w = wp - 8;
+    int ks = 0, vs = 0;
+    uint32_t kph = 0, vph = 0, qph = 0, pph[2] = {0, 0};
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+    // descriptors of the first block of each buffer; addresses count 16 bytes
+    const uint64_t qw = sw128_desc(smem_u32(sq + w * C::TILE)), kd = sw128_desc(smem_u32(sk));
+    const uint64_t vd = v_desc(smem_u32(sv), C::SUB);
+    auto wait_all = [&](uint64_t* b, uint32_t parity) {
+      return __all_sync(0xffffffffu, wait(b, parity)) != 0;
+    };
+    each_tile([&](int tile, int k0, int k1) {
+      const bool idle = w >= halves_of(tile);
+      const int steps = steps_of(k0, k1);
+      auto next_k = [&] { if (++ks == C::STAGES) ks = 0, kph ^= 1u; };
+      auto next_v = [&] { if (++vs == C::STAGES) vs = 0, vph ^= 1u; };
+      if (idle) {  // no such rows: only release the tiles
         for (int k = k0; k < k1; ++k) {
-          const bool more = k + 1 < k1;
-          if (!wait(&S->vfull[vs], vph)) return false;
-          if (more && !wait(&S->kfull[ks], kph)) return false;
-          for (int w = 0; w < halves; ++w) {
-            // the weights of 64 keys at a time
-#pragma unroll
-            for (int part = 0; part < 2; ++part) {
-              if (!wait(&S->pfull[w][part], pph[w])) return false;
-              fence_after();
-#pragma unroll
-              for (int kk = part * 4; kk < part * 4 + 4; ++kk)
-                mma_f16_ts(tmem + 256 + DP * w, tmem + 128 * w + kk * 8,
-                           v_desc(v_0 + vs * C::TILE + kk * 2048, C::SUB), C::IDESC_O,
-                           k != k0 || kk != 0);
-            }
-            pph[w] ^= 1u;
-            // the tile's last arrival is ofull's: nothing arrives behind it
-            if (w == halves - 1) mma_commit<false>(&S->vempty[vs]);
-            if (more)
-              scores(w, ks);
-            else
-              mma_commit<false>(&S->ofull[w]);
-          }
-          if (++vs == C::STAGES) vs = 0, vph ^= 1u;
-          if (more) {
-            mma_commit<false>(&S->kempty[ks]);
-            if (++ks == C::STAGES) ks = 0, kph ^= 1u;
-          }
+          if (!wait_all(&S->kfull[ks], kph)) return false;
+          if (lane == 0) mbar_arrive(&S->kempty[ks]);
+          next_k();
+          if (!wait_all(&S->vfull[vs], vph)) return false;
+          if (lane == 0) mbar_arrive(&S->vempty[vs]);
+          next_v();
         }
         return true;
-      });
-    }
+      }
+      // the scores of step t, from the K tile in stage ks
+      auto scores = [&](int t) {
+        const uint64_t kw = kd + (uint32_t)(ks * (C::TILE >> 4) + (t & 1) * (kStep * 128 >> 4));
+        const uint32_t to = tm + 128 * w + 64 * (t & 1);
+        const bool k_used = (t & 1) || t + 1 == steps;
+        if (elect_one()) {
+          mma_ss<0>(to, qw, kw, C::IDESC_S);
+#pragma unroll
+          for (int kk = 1; kk < DP / 16; ++kk) {
+            const uint32_t off = (kk >> 2) * (C::SUB >> 4) + (kk & 3) * 2;
+            mma_ss<1>(to, qw + off, kw + off, C::IDESC_S);
+          }
+          mma_commit<false>(&S->sfull[w][t & 1]);
+          if (k_used) mma_commit<false>(&S->kempty[ks]);
+        }
+        __syncwarp();
+        if (k_used) next_k();
+      };
+      if (!wait_all(&S->kfull[ks], kph) || !wait_all(&S->qready[w], qph)) return false;
+      qph ^= 1u;
+      fence_after();
+      scores(0);
+      if (steps > 1) scores(1);
+      for (int t = 0; t < steps; ++t) {
+        const int i = t & 1;
+        if (i == 0 && !wait_all(&S->vfull[vs], vph)) return false;
+        if (i == 0 && t + 2 < steps && !wait_all(&S->kfull[ks], kph)) return false;
+        if (!wait_all(&S->pfull[w][i], pph[i])) return false;
+        pph[i] ^= 1u;
+        fence_after();
+        const uint32_t po = tm + 256 + DP * w, pt = tm + 128 * w + 64 * i;
+        const uint64_t vw = vd + (uint32_t)(vs * (C::TILE >> 4) + i * (kStep * 128 >> 4));
+        const bool v_used = i || t + 1 == steps;
+        if (elect_one()) {
+          mma_ts<2>(po, pt, vw, C::IDESC_O, t != 0);
+#pragma unroll
+          for (int kk = 1; kk < kStep / 16; ++kk)
+            mma_ts<1>(po, pt + kk * 8, vw + kk * (2048 >> 4), C::IDESC_O, 1);
+          // before ofull: the tile's last arrival is the one waited for
+          if (v_used) mma_commit<false>(&S->vempty[vs]);
+          mma_commit<false>(&S->odone[w]);
+          if (t + 1 == steps) mma_commit<false>(&S->ofull[w]);
+        }
+        __syncwarp();
+        if (v_used) next_v();
+        if (t + 2 < steps) scores(t + 2);
+      }
+      return true;
+    });
   } else {
     // ------------------------------------------------------------ softmax
     const int w = wp >> 2, quad = wp & 3, tr = quad * 32 + lane;  // half, lane quadrant, row
@@ -300,7 +348,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t ts = tmem + lanes + 128 * w, to = tmem + lanes + 256 + DP * w;
     const float turn = a.scale < 0.f ? -1.f : 1.f, rs = a.scale * turn * kLog2e;
     const uint32_t flip = turn < 0.f ? 0x80008000u : 0u;
-    uint32_t sph = 0, oph = 0, fph = 1;
+    // dph: parity of the last step's product. Its wait in step t may lag by one
+    // phase only: the scores of step t came behind the product of step t - 2.
+    uint32_t sph[2] = {0, 0}, dph = 1, oph = 0, fph = 1;
     const int D = a.head_dim;
     each_tile([&](int tile, int k0, int k1) {
       if (w >= halves_of(tile)) return true;
@@ -318,49 +368,57 @@ __global__ void __launch_bounds__(kThreads, 1)
         const __nv_bfloat16* q =
             static_cast<const __nv_bfloat16*>(a.q.p) + b * a.q.sb + t * a.q.st + h * a.q.sh;
         uint8_t* row = sq + w * C::TILE + tr * 128;
+        uint4 v[DP / 8];  // all loads before the first store
+#pragma unroll
+        for (int c = 0; c < DP / 8; ++c)
+          v[c] = real && c * 8 < D ? *reinterpret_cast<const uint4*>(q + c * 8)
+                                   : make_uint4(0, 0, 0, 0);
 #pragma unroll
         for (int c = 0; c < DP / 8; ++c) {
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (real && c * 8 < D) v = *reinterpret_cast<const uint4*>(q + c * 8);
-          v.x ^= flip, v.y ^= flip, v.z ^= flip, v.w ^= flip;
-          *reinterpret_cast<uint4*>(row + (c >> 3) * C::SUB + (((c & 7) ^ (tr & 7)) << 4)) = v;
+          v[c].x ^= flip, v[c].y ^= flip, v[c].z ^= flip, v[c].w ^= flip;
+          *reinterpret_cast<uint4*>(row + (c >> 3) * C::SUB + (((c & 7) ^ (tr & 7)) << 4)) = v[c];
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) mbar_arrive(&S->qready[w]);
       }
       float m = -INFINITY, l = 0.f;  // fixed maximum (before rs), sum
-      for (int k = k0; ok && k < k1; ++k) {
-        if (lane == 0) ok = wait(&S->sfull[w], sph);
+      const int steps = steps_of(k0, k1);
+      for (int t = 0; ok && t < steps; ++t) {
+        const int i = t & 1;
+        if (lane == 0) ok = wait(&S->sfull[w][i], sph[i]);
         ok = __shfl_sync(0xffffffffu, ok, 0);
         if (!ok) break;
-        sph ^= 1u;
+        sph[i] ^= 1u;
         fence_after();
-        uint32_t s[4][32];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32(ts + 32 * c, s[c]);
+        uint32_t s[2][32];
+        tmem_ld32(ts + 64 * i, s[0]);
+        tmem_ld32(ts + 64 * i + 32, s[1]);
         tmem_wait_ld();
-        const int left = (int)a.prefix_cols - k * kKeys;  // keys of this tile
-        if (left < kKeys) {
+        const int left = (int)a.prefix_cols - k0 * kKeys - t * kStep;  // keys of this step
+        if (left < kStep) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (c * 32 + e >= left) s[c][e] = 0xff800000u;  // -inf
+        }
+        float mx4[4] = {m, m, m, m};  // four chains of maxima at a time
+#pragma unroll
+        for (int e = 0; e < 32; e += 2)
 #pragma unroll
           for (int c = 0; c < 4; ++c)
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (c * 32 + i >= left) s[c][i] = 0xff800000u;  // -inf
-        }
-        // four chains of maxima at a time
-        float mx4[4] = {m, m, m, m};
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) mx4[c] = fmaxf(mx4[c], __uint_as_float(s[c][i]));
+            mx4[c] = fmaxf(mx4[c], __uint_as_float(s[c >> 1][e + (c & 1)]));
         const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
-        const bool first = k == k0;
-        const bool grow = first || (mx - m) * rs > kGrow;
-        if (first) {
+        const bool grow = t == 0 || (mx - m) * rs > kGrow;
+        if (t == 0) {
           m = mx;
         } else if (__any_sync(0xffffffffu, grow)) {
-          // the scores' completion covers every product before them: O is at rest
+          // the last step's product has to be done before O is touched
+          if (lane == 0) ok = wait(&S->odone[w], dph);
+          ok = __shfl_sync(0xffffffffu, ok, 0);
+          if (!ok) break;
+          fence_after();
           const float f = grow ? ex2((m - mx) * rs) : 1.f;
           if (grow) m = mx;
           l *= f;
@@ -370,7 +428,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             tmem_ld8(to + c, o);
             tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 8; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+            for (int e = 0; e < 8; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
             tmem_st8(to + c, o);
           }
         }
@@ -379,23 +437,22 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint64_t sum[2] = {0, 0};  // (0.f, 0.f)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          uint32_t pk[32];
+          uint32_t pk[16];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const int e = (2 * i) & 31;
-            const uint32_t(&src)[32] = s[2 * c + (i >> 4)];
+          for (int e = 0; e < 16; ++e) {
             float x, y;
-            unpair(fma2((uint64_t)src[e + 1] << 32 | src[e], rs2, nb2), x, y);
+            unpair(fma2((uint64_t)s[c][2 * e + 1] << 32 | s[c][2 * e], rs2, nb2), x, y);
             x = ex2(x), y = ex2(y);
-            sum[i & 1] = add2(sum[i & 1], pair(x, y));
-            pk[i] = pack_bf16x2(x, y);
+            sum[e & 1] = add2(sum[e & 1], pair(x, y));
+            pk[e] = pack_bf16x2(x, y);
           }
-          tmem_st32(ts + 32 * c, pk);
-          tmem_wait_st();
-          fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&S->pfull[w][c]);
+          tmem_st16(ts + 64 * i + 16 * c, pk);
         }
+        tmem_wait_st();
+        fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&S->pfull[w][i]);
+        dph ^= 1u;
         float x, y;
         unpair(add2(sum[0], sum[1]), x, y);
         l += x + y;
@@ -420,37 +477,41 @@ __global__ void __launch_bounds__(kThreads, 1)
             p.part_ml[e * p.out_rows + orow] = make_float2(-INFINITY, 0.f);
       }
       if (!ok) return false;
-      // O through the half's query buffer, which nothing reads any more: W
-      // values of each row at a time, a bulk store a row
-      constexpr int W = DP / 4, STRIDE = W * 4 + 16;  // 16: rows in other banks
+      // O through the half's query buffer, which no product reads any more: W
+      // values of the warp's 32 rows at a time, written out a row at a time
+      constexpr int W = DP / 4, STRIDE = W * 4 + 16, PER = W / 4;  // 16: rows in other banks
       static_assert(kRows * STRIDE <= C::TILE, "O passes fit the query buffer");
-      uint8_t* row = sq + w * C::TILE + tr * STRIDE;
-      float* out = p.part_o + (slot * p.out_rows + orow) * D;
+      uint8_t* mine = sq + w * C::TILE + quad * 32 * STRIDE;
+      const int at = real ? (int)orow : -1;
 #pragma unroll 1
       for (int c = 0; c < DP; c += W) {
         uint32_t o[W];
-        __syncwarp();  // the warp's loads are collective; rows past the last store nothing
         if constexpr (W == 32)
           tmem_ld32(to + c, o);
         else
           tmem_ld16(to + c, o);
         tmem_wait_ld();
-        bulk_wait_read();  // the last pass has left the buffer
 #pragma unroll
-        for (int i = 0; i < W; i += 4)
-          *reinterpret_cast<uint4*>(row + i * 4) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        const int n = min(W, D - c);
-        if (real && n > 0) bulk_store_s2g(out + c, row, n * 4);
-        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        for (int e = 0; e < W; e += 4)
+          *reinterpret_cast<uint4*>(mine + lane * STRIDE + e * 4) =
+              make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+        __syncwarp();
+        const int piece = lane % PER, d = c + piece * 4;
+#pragma unroll
+        for (int e = 0; e < PER; ++e) {
+          const int r = e * (32 / PER) + lane / PER;
+          const int to_row = __shfl_sync(0xffffffffu, at, r);
+          const uint4 v = *reinterpret_cast<const uint4*>(mine + r * STRIDE + piece * 16);
+          if (to_row >= 0 && d < D)
+            *reinterpret_cast<uint4*>(p.part_o + (slot * p.out_rows + to_row) * D + d) = v;
+        }
+        __syncwarp();
       }
-      bulk_wait_read();
       fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&S->qfree[w]);
       return true;
     });
-    asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
   // every warp arrives, so no copy, product or TMEM access is left when TMEM goes
   fence_before();

@@ -4,7 +4,7 @@
  * Drop-in compute path behind mini-EP's MoE-backend contract
  * (kanwarpal-brar/mini-ep, miniep/ep.py and miniep/modeling.py). The reference
  * is Python; its FFI for this path would be ctypes, so every entry point takes
- * plain pointers and sizes only:
+ * plain pointers and sizes only (two take them in a struct of 8-byte fields):
  *   - tensor arguments are DEVICE pointers (contiguous, row-major) unless the
  *     comment says "host";
  *   - `stream` is a cudaStream_t passed as void*; all GPU work is enqueued on
@@ -324,15 +324,31 @@ int mep_dest_ranks_noalloc(int num_experts, int world, const int64_t* table,
  * cos / sin: (table_rows, head_dim), fp32 or the model dtype (table_dtype).
  * A position outside the tables gives NaN rows.
  */
-int mep_norm_rope_store(int dtype, int cache_dtype, int64_t batch, int64_t tokens, int q_heads,
-                        int kv_heads, int head_dim, const void* q, int64_t q_sb, int64_t q_st,
-                        int64_t q_sh, const void* k, int64_t k_sb, int64_t k_st, int64_t k_sh,
-                        const void* v, int64_t v_sb, int64_t v_st, int64_t v_sh,
-                        const void* q_norm, const void* k_norm, float eps, const void* cos,
-                        const void* sin, int table_dtype, int64_t table_rows,
-                        const int64_t* positions, int64_t p_sb, int64_t p_st, void* q_out,
-                        void* k_cache, void* v_cache, float* k_scale, float* v_scale,
-                        int64_t capacity, int64_t col, const int64_t* col_dev, void* stream);
+typedef struct mep_store_args {
+  int64_t dtype, cache_dtype, batch, tokens, q_heads, kv_heads, head_dim;
+  const void* q; /* strides of batch, token and head */
+  int64_t q_sb, q_st, q_sh;
+  const void* k;
+  int64_t k_sb, k_st, k_sh;
+  const void* v;
+  int64_t v_sb, v_st, v_sh;
+  const void* q_norm;
+  const void* k_norm;
+  double eps;
+  const void* cos;
+  const void* sin;
+  int64_t table_dtype, table_rows;
+  const int64_t* positions; /* strides of batch and token (0: broadcast) */
+  int64_t p_sb, p_st;
+  void* q_out;
+  void* k_cache;
+  void* v_cache;
+  float* k_scale;
+  float* v_scale;
+  int64_t capacity, col;
+  const int64_t* col_dev;
+} mep_store_args;
+int mep_norm_rope_store(const mep_store_args* args, void* stream);
 
 /*
  * Columns [start, start + columns) of a quantised layer in the model dtype:
@@ -354,14 +370,27 @@ int mep_kv_read(int dtype, int64_t batch, int kv_heads, int head_dim, const void
  * contiguous. workspace: mep_cache_attention_workspace bytes, the caller's, in
  * use until the call's work on `stream` is done.
  */
-int mep_cache_attention(int dtype, int cache_dtype, int64_t batch, int64_t tokens, int q_heads,
-                        int kv_heads, int head_dim, const void* q, int64_t q_sb, int64_t q_st,
-                        int64_t q_sh, const void* k_cache, const void* v_cache,
-                        const float* k_scale, const float* v_scale, int64_t capacity,
-                        const int64_t* lengths, int64_t prompt_cols, int64_t col,
-                        const int64_t* col_dev, const void* k_prefix, const void* v_prefix,
-                        int64_t prefix_cols, float scale, void* out, void* workspace,
-                        int64_t workspace_bytes, void* stream);
+typedef struct mep_attention_args {
+  int64_t dtype, cache_dtype, batch, tokens, q_heads, kv_heads, head_dim;
+  const void* q;
+  int64_t q_sb, q_st, q_sh;
+  const void* k_cache;
+  const void* v_cache;
+  const float* k_scale;
+  const float* v_scale;
+  int64_t capacity;
+  const int64_t* lengths;
+  int64_t prompt_cols, col;
+  const int64_t* col_dev;
+  const void* k_prefix;
+  const void* v_prefix;
+  int64_t prefix_cols;
+  double scale;
+  void* out;
+  void* workspace;
+  int64_t workspace_bytes;
+} mep_attention_args;
+int mep_cache_attention(const mep_attention_args* args, void* stream);
 /* Workspace of such a call (host arithmetic only). col: as given to the call,
  * or -1 when it is read on the device. */
 int mep_cache_attention_workspace(int dtype, int cache_dtype, int64_t batch, int64_t tokens,

@@ -906,9 +906,8 @@ template <typename QT, typename CT, int DP, bool KS, bool PREFIX>
 int run_part(const PartArgs& p, int64_t mats, cudaStream_t st) {
   using X = Tile<QT, CT, DP, KS>;
   auto* k = k_attn_part<QT, CT, DP, KS, PREFIX>;
-  const cudaError_t e =
-      cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, X::kSmem);
-  if (e != cudaSuccess) return (int)e;
+  static SmemLimit limit;
+  if (const int e = limit.raise(reinterpret_cast<const void*>(k), X::kSmem)) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(mats * p.row_tiles * p.splits), (unsigned)p.a.kv_heads);
   cfg.blockDim = dim3(kThreads);
@@ -980,47 +979,47 @@ extern "C" int mep_cache_attention_workspace(int dtype, int cache_dtype, int64_t
   return MEP_OK;
 }
 
-extern "C" int mep_cache_attention(int dtype, int cache_dtype, int64_t batch, int64_t tokens,
-                                   int q_heads, int kv_heads, int head_dim, const void* q,
-                                   int64_t q_sb, int64_t q_st, int64_t q_sh, const void* k_cache,
-                                   const void* v_cache, const float* k_scale, const float* v_scale,
-                                   int64_t capacity, const int64_t* lengths, int64_t prompt_cols,
-                                   int64_t col, const int64_t* col_dev, const void* k_prefix,
-                                   const void* v_prefix, int64_t prefix_cols, float scale,
-                                   void* out, void* workspace, int64_t workspace_bytes,
-                                   void* stream) {
+extern "C" int mep_cache_attention(const mep_attention_args* x, void* stream) {
   const char* op = "mep_cache_attention";
-  if (const char* why = bad_heads(dtype, cache_dtype, batch, tokens, q_heads, kv_heads, head_dim))
+  if (!x) return serve_invalid(op, "null arguments");
+  if (const char* why = bad_heads(x->dtype, x->cache_dtype, x->batch, x->tokens, x->q_heads,
+                                  x->kv_heads, x->head_dim))
     return serve_invalid(op, why);
-  if (capacity < 0 || prefix_cols < 0 || prompt_cols < 0)
+  if (x->capacity < 0 || x->prefix_cols < 0 || x->prompt_cols < 0)
     return serve_invalid(op, "negative columns");
-  if (capacity > 0x7fffffff - 1024 || prefix_cols > 0x7fffffff - 1024)
+  if (x->capacity > 0x7fffffff - 1024 || x->prefix_cols > 0x7fffffff - 1024)
     return serve_invalid(op, "columns up to 2^31 - 1025");
-  if (!col_dev && (col < 0 || col + tokens > capacity))
+  if (!x->col_dev && (x->col < 0 || x->col > x->capacity - x->tokens))
     return serve_invalid(op, "columns [col, col + tokens) do not fit the cache");
-  if (batch == 0 || tokens == 0) return MEP_OK;
-  AttnArgs a{batch, tokens, q_heads, kv_heads, head_dim, {q, q_sb, q_st, q_sh},
-             {k_cache, v_cache, k_scale, v_scale, capacity}, lengths, prompt_cols, col, col_dev,
-             k_prefix, v_prefix, prefix_cols, scale, out};
-  if (!q || !k_cache || !v_cache || !out) return serve_invalid(op, "null tensor");
-  if (prefix_cols > 0 && (!k_prefix || !v_prefix)) return serve_invalid(op, "null prefix");
-  if (cache_dtype == MEP_E4M3 && (!k_scale || !v_scale))
+  if (x->batch == 0 || x->tokens == 0) return MEP_OK;
+  const AttnArgs a{x->batch, x->tokens, (int)x->q_heads, (int)x->kv_heads, (int)x->head_dim,
+                   {x->q, x->q_sb, x->q_st, x->q_sh},
+                   {x->k_cache, x->v_cache, x->k_scale, x->v_scale, x->capacity}, x->lengths,
+                   x->prompt_cols, x->col, x->col_dev, x->k_prefix, x->v_prefix, x->prefix_cols,
+                   (float)x->scale, x->out};
+  if (!x->q || !x->k_cache || !x->v_cache || !x->out) return serve_invalid(op, "null tensor");
+  if (x->prefix_cols > 0 && (!x->k_prefix || !x->v_prefix))
+    return serve_invalid(op, "null prefix");
+  if (x->cache_dtype == MEP_E4M3 && (!x->k_scale || !x->v_scale))
     return serve_invalid(op, "a quantised cache needs k_scale and v_scale");
-  if (bad_strides(a.q, dtype == MEP_BF16 ? 2 : 4) || !aligned16(k_cache) || !aligned16(v_cache) ||
-      !aligned16(k_prefix) || !aligned16(v_prefix) || !aligned16(out))
+  if (bad_strides(a.q, x->dtype == MEP_BF16 ? 2 : 4) || !aligned16(x->k_cache) ||
+      !aligned16(x->v_cache) || !aligned16(x->k_prefix) || !aligned16(x->v_prefix) ||
+      !aligned16(x->out))
     return serve_invalid(op, "tensors and row strides must be multiples of 16 bytes");
-  const Plan pl = plan_for(dtype, batch, tokens, q_heads, kv_heads, head_dim, capacity,
-                           col_dev ? -1 : col, prefix_cols);
-  if (pl.bytes > 0 && (!workspace || workspace_bytes < pl.bytes || !aligned16(workspace)))
+  const Plan pl = plan_for((int)x->dtype, x->batch, x->tokens, a.q_heads, a.kv_heads, a.head_dim,
+                           x->capacity, x->col_dev ? -1 : x->col, x->prefix_cols);
+  if (pl.bytes > 0 &&
+      (!x->workspace || x->workspace_bytes < pl.bytes || !aligned16(x->workspace)))
     return serve_invalid(op, "workspace of " + std::to_string(pl.bytes) + " bytes needed");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool e4m3 = x->cache_dtype == MEP_E4M3;
   int rc;
-  if (dtype == MEP_BF16)
-    rc = cache_dtype == MEP_E4M3 ? run_attention<__nv_bfloat16, uint8_t>(a, pl, workspace, st)
-                                 : run_attention<__nv_bfloat16, __nv_bfloat16>(a, pl, workspace, st);
+  if (x->dtype == MEP_BF16)
+    rc = e4m3 ? run_attention<__nv_bfloat16, uint8_t>(a, pl, x->workspace, st)
+              : run_attention<__nv_bfloat16, __nv_bfloat16>(a, pl, x->workspace, st);
   else
-    rc = cache_dtype == MEP_E4M3 ? run_attention<float, uint8_t>(a, pl, workspace, st)
-                                 : run_attention<float, float>(a, pl, workspace, st);
+    rc = e4m3 ? run_attention<float, uint8_t>(a, pl, x->workspace, st)
+              : run_attention<float, float>(a, pl, x->workspace, st);
   if (rc < 0) return serve_invalid(op, "tensor map error " + std::to_string(rc));
   if (rc) return serve_cuda(op, (cudaError_t)rc);
   return serve_launched(op);

@@ -529,9 +529,9 @@ int launch(const Args& p, int ctas, cudaStream_t st) {
   const uint32_t box[3] = {64, kKeys, 1};
   if (int rc = encode_bf16_3d(&tk, a.kp, dims, box)) return rc;
   if (int rc = encode_bf16_3d(&tv, a.vp, dims, box)) return rc;
-  const cudaError_t e = cudaFuncSetAttribute(
-      k_attn_prefix_tc<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<DP>::SMEM);
-  if (e != cudaSuccess) return (int)e;
+  static SmemLimit limit;
+  if (const int e = limit.raise(reinterpret_cast<const void*>(k_attn_prefix_tc<DP>), Cfg<DP>::SMEM))
+    return e;
   k_attn_prefix_tc<DP><<<ctas, kThreads, Cfg<DP>::SMEM, st>>>(tk, tv, p);
   return 0;
 }

@@ -300,45 +300,42 @@ __global__ void __launch_bounds__(256) k_kv_read(CacheView c, int D, int64_t sta
 
 using namespace mep;
 
-extern "C" int mep_norm_rope_store(
-    int dtype, int cache_dtype, int64_t batch, int64_t tokens, int q_heads, int kv_heads,
-    int head_dim, const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* k,
-    int64_t k_sb, int64_t k_st, int64_t k_sh, const void* v, int64_t v_sb, int64_t v_st,
-    int64_t v_sh, const void* q_norm, const void* k_norm, float eps, const void* cos,
-    const void* sin, int table_dtype, int64_t table_rows, const int64_t* positions, int64_t p_sb,
-    int64_t p_st, void* q_out, void* k_cache, void* v_cache, float* k_scale, float* v_scale,
-    int64_t capacity, int64_t col, const int64_t* col_dev, void* stream) {
+extern "C" int mep_norm_rope_store(const mep_store_args* x, void* stream) {
   const char* op = "mep_norm_rope_store";
-  if (const char* why = bad_heads(dtype, cache_dtype, batch, tokens, q_heads, kv_heads, head_dim))
+  if (!x) return serve_invalid(op, "null arguments");
+  if (const char* why = bad_heads(x->dtype, x->cache_dtype, x->batch, x->tokens, x->q_heads,
+                                  x->kv_heads, x->head_dim))
     return serve_invalid(op, why);
-  if (table_dtype != MEP_F32 && table_dtype != dtype)
+  if (x->table_dtype != MEP_F32 && x->table_dtype != x->dtype)
     return serve_invalid(op, "the rotation tables must be fp32 or in the model dtype");
-  if (capacity < 0) return serve_invalid(op, "negative capacity");
-  if (!col_dev && (col < 0 || col + tokens > capacity))
+  if (x->capacity < 0) return serve_invalid(op, "negative capacity");
+  if (!x->col_dev && (x->col < 0 || x->col > x->capacity - x->tokens))
     return serve_invalid(op, "columns [col, col + tokens) do not fit the cache");
-  if (batch == 0 || tokens == 0) return MEP_OK;
-  StoreArgs a{batch, tokens, q_heads, kv_heads, head_dim, {q, q_sb, q_st, q_sh},
-              {k, k_sb, k_st, k_sh}, {v, v_sb, v_st, v_sh}, q_norm, k_norm, eps, cos, sin,
-              table_rows, positions, p_sb, p_st, q_out, k_cache, v_cache, k_scale, v_scale,
-              capacity, col, col_dev};
-  if (!q || !k || !v || !cos || !sin || !positions || !q_out || !k_cache || !v_cache)
+  if (x->batch == 0 || x->tokens == 0) return MEP_OK;
+  const StoreArgs a{x->batch, x->tokens, (int)x->q_heads, (int)x->kv_heads, (int)x->head_dim,
+                    {x->q, x->q_sb, x->q_st, x->q_sh}, {x->k, x->k_sb, x->k_st, x->k_sh},
+                    {x->v, x->v_sb, x->v_st, x->v_sh}, x->q_norm, x->k_norm, (float)x->eps, x->cos,
+                    x->sin, x->table_rows, x->positions, x->p_sb, x->p_st, x->q_out, x->k_cache,
+                    x->v_cache, x->k_scale, x->v_scale, x->capacity, x->col, x->col_dev};
+  if (!x->q || !x->k || !x->v || !x->cos || !x->sin || !x->positions || !x->q_out ||
+      !x->k_cache || !x->v_cache)
     return serve_invalid(op, "null tensor");
-  if (cache_dtype == MEP_E4M3 && (!k_scale || !v_scale))
+  if (x->cache_dtype == MEP_E4M3 && (!x->k_scale || !x->v_scale))
     return serve_invalid(op, "a quantised cache needs k_scale and v_scale");
-  const int elt = dtype == MEP_BF16 ? 2 : 4;
-  if (bad_strides(a.q, elt) || bad_strides(a.k, elt) || bad_strides(a.v, elt) || !aligned16(cos) ||
-      !aligned16(sin) || !aligned16(q_norm) || !aligned16(k_norm) || !aligned16(q_out) ||
-      !aligned16(k_cache) || !aligned16(v_cache))
+  const int elt = x->dtype == MEP_BF16 ? 2 : 4;
+  if (bad_strides(a.q, elt) || bad_strides(a.k, elt) || bad_strides(a.v, elt) ||
+      !aligned16(x->cos) || !aligned16(x->sin) || !aligned16(x->q_norm) || !aligned16(x->k_norm) ||
+      !aligned16(x->q_out) || !aligned16(x->k_cache) || !aligned16(x->v_cache))
     return serve_invalid(op, "tensors and row strides must be multiples of 16 bytes");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int tf = table_dtype == MEP_F32;
-  if (dtype == MEP_BF16) {
-    if (cache_dtype == MEP_E4M3)
+  const int tf = x->table_dtype == MEP_F32;
+  if (x->dtype == MEP_BF16) {
+    if (x->cache_dtype == MEP_E4M3)
       launch_store<__nv_bfloat16, __nv_fp8_storage_t>(a, tf, st);
     else
       launch_store<__nv_bfloat16, __nv_bfloat16>(a, tf, st);
   } else {
-    if (cache_dtype == MEP_E4M3)
+    if (x->cache_dtype == MEP_E4M3)
       launch_store<float, __nv_fp8_storage_t>(a, tf, st);
     else
       launch_store<float, float>(a, tf, st);

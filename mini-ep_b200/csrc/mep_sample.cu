@@ -677,8 +677,9 @@ int launch_sample(const SampleArgs& a, int64_t rows, cudaStream_t st) {
   const bool cached = per <= kMostSliceBytes;
   const int smem = kSharedBytes + (cached ? (int)per : 0);
   auto* k = cached ? k_sample<T, true> : k_sample<T, false>;
-  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return (int)e;
+  static SmemLimit limits[2];
+  const int most = cached ? kSharedBytes + (int)kMostSliceBytes : kSharedBytes;
+  if (const int e = limits[cached].raise(reinterpret_cast<const void*>(k), most)) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(rows * nc));
   cfg.blockDim = dim3(kNT);

@@ -2,6 +2,7 @@
 // the layout of a layer's key/value cache, argument errors and launch checks.
 #pragma once
 
+#include <atomic>
 #include <cstdint>
 #include <string>
 
@@ -29,6 +30,24 @@ inline int serve_launched(const char* op) {
   set_global_error(std::string(op) + ": kernel launch: " + cudaGetErrorString(e));
   return MEP_ERR_CUDA;
 }
+// Dynamic shared memory limit of a kernel, raised once on each device.
+class SmemLimit {
+ public:
+  int raise(const void* kernel, int bytes) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return (int)e;
+    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+    if (done_.load(std::memory_order_acquire) & bit) return 0;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return (int)e;
+    done_.fetch_or(bit, std::memory_order_release);
+    return 0;
+  }
+
+ private:
+  std::atomic<uint64_t> done_{0};
+};
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // One layer of a key/value cache: (batch, kv_heads, capacity, head_dim), rows
@@ -50,8 +69,8 @@ struct HeadsView {
 };
 
 // Checks shared by the entry points that take heads; null when they hold.
-inline const char* bad_heads(int dtype, int cache_dtype, int64_t batch, int64_t tokens, int q_heads,
-                             int kv_heads, int head_dim) {
+inline const char* bad_heads(int64_t dtype, int64_t cache_dtype, int64_t batch, int64_t tokens,
+                             int64_t q_heads, int64_t kv_heads, int64_t head_dim) {
   if (dtype != MEP_F32 && dtype != MEP_BF16) return "dtype must be MEP_F32 or MEP_BF16";
   if (cache_dtype != dtype && cache_dtype != MEP_E4M3)
     return "the cache must be in the model dtype or in MEP_E4M3";

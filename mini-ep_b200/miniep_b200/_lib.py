@@ -6,6 +6,7 @@ entry point raises. Build it with ``python -m miniep_b200.build``.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 import threading
 from pathlib import Path
 
@@ -27,6 +28,12 @@ TL_MARKS = {"barrier_end": 0, "counts_sent": 7, "layout": 8, "data_in": 11, "res
 _P = C.c_void_p
 _I64 = C.c_int64
 _I = C.c_int
+
+# mep_store_args and mep_attention_args of include/miniep_b200.h: 8-byte fields
+# (q integers and pointers, 0 for NULL; d doubles), packed per call: passing
+# forty arguments one by one took ctypes 8 us
+STORE_ARGS = struct.Struct("@7q 4q 4q 4q 2q d 4q 3q q 4q 3q")
+ATTENTION_ARGS = struct.Struct("@7q 4q 5q 4q 3q d 3q")
 
 # name -> argtypes (every function returns int unless listed in _RESTYPES)
 SIGNATURES = {
@@ -57,12 +64,9 @@ SIGNATURES = {
     "mep_debug_wait": [_P, C.c_uint32, _I64, _P],
     "mep_barrier": [_P, _P],
     "mep_read_timeline": [_P, _P, _P],
-    "mep_norm_rope_store": [_I, _I, _I64, _I64, _I, _I, _I] + [_P, _I64, _I64, _I64] * 3 +
-                           [_P, _P, C.c_float, _P, _P, _I, _I64, _P, _I64, _I64, _P, _P, _P, _P,
-                            _P, _I64, _I64, _P, _P],
+    "mep_norm_rope_store": [C.c_char_p, _P],  # packed structs: STORE_ARGS, ATTENTION_ARGS
     "mep_kv_read": [_I, _I64, _I, _I, _P, _P, _P, _P, _I64, _I64, _I64, _P, _P, _P],
-    "mep_cache_attention": [_I, _I, _I64, _I64, _I, _I, _I, _P, _I64, _I64, _I64, _P, _P, _P, _P,
-                            _I64, _P, _I64, _I64, _P, _P, _P, _I64, C.c_float, _P, _P, _I64, _P],
+    "mep_cache_attention": [C.c_char_p, _P],
     "mep_cache_attention_workspace": [_I, _I, _I64, _I64, _I, _I, _I, _I64, _I64, _I64,
                                       C.POINTER(_I64)],
     "mep_sample": [_I, _P, _I64, _I64, _I64, _P, _P, _P, _P, _P, C.c_float, C.c_int32, C.c_float,

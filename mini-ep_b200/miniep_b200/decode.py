@@ -35,29 +35,36 @@ def _need(cond: bool, msg: str):
 
 
 def _tensor(t, name: str, device, dtype=None):
+    """Refuses what is not a CUDA tensor on `device` (None: any) of `dtype`."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise MEPError(f"{name} must be a CUDA tensor")
-    if device is not None and t.device != device:
+    if device is not None and t.get_device() != device.index:
         raise MEPError(f"{name} is on {t.device}, expected {device}")
-    if dtype is not None and t.dtype != dtype:
+    if dtype is not None and t.dtype is not dtype:
         raise MEPError(f"{name} must be {dtype}, not {t.dtype}")
     if t.requires_grad and torch.is_grad_enabled():
         raise MEPError(f"{name} requires grad: this operator has no backward pass")
 
 
 def _rows(t):
-    """`t` itself where the kernels' 16-byte accesses fit its strides, else a copy."""
-    unit = 16 // t.element_size()
-    st = t.stride()
-    if st[-1] == 1 and t.data_ptr() % 16 == 0 and not any(s % unit for s in st[:-1]):
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
+    """`t` (batch, tokens, heads, head_dim) itself where the kernels' 16-byte
+    accesses fit its strides, else a copy; its address and strides."""
+    b, n, h, one = t.stride()
+    p = t.data_ptr()
+    if one != 1 or (p | (b | n | h) * t.element_size()) & 15:
+        t = t.clone(memory_format=torch.contiguous_format)
+        b, n, h, _ = t.stride()
+        p = t.data_ptr()
+    return t, p, b, n, h
 
 
 def _flat(t):
     """Contiguous and on a 16-byte boundary."""
     t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+    return t if t.data_ptr() & 15 == 0 else t.clone()
+
+
+_stream_of = torch._C._cuda_getCurrentRawStream
 
 
 class _on:
@@ -70,7 +77,7 @@ class _on:
         self.before = torch.cuda.current_device()
         if self.before != self.index:
             torch.cuda.set_device(self.index)
-        return torch._C._cuda_getCurrentRawStream(self.index)
+        return _stream_of(self.index)
 
     def __exit__(self, *exc):
         if self.before != self.index:
@@ -112,10 +119,9 @@ class KVCache:
         # every layer starts on a 16-byte boundary too: a row is a multiple of
         # 16 bytes (head_dim is one of 16), and scales are read one at a time
         step = [t[0].numel() * t.element_size() if self.layers else 0 for t in parts]
-        at = [t.data_ptr() for t in parts] + [None] * (4 - len(parts))
-        self._ptrs = [tuple(None if p is None else p + l * d
-                            for p, d in zip(at, step + [0] * (4 - len(parts))))
-                      for l in range(self.layers)]
+        at = [t.data_ptr() for t in parts] + [0] * (4 - len(parts))
+        step += [0] * (4 - len(parts))
+        self._ptrs = [tuple(p + l * d for p, d in zip(at, step)) for l in range(self.layers)]
 
     @classmethod
     def empty(cls, layers: int, batch: int, kv_heads: int, capacity: int, head_dim: int,
@@ -183,22 +189,20 @@ class SharedPrefix:
 
 
 def _column(col, device):
-    """(host column or -1, device pointer or None)."""
+    """(host column or -1, device pointer or 0)."""
     if isinstance(col, torch.Tensor):
         _tensor(col, "col", device, torch.int64)
         _need(col.numel() == 1, "col must hold one column")
         return -1, col.data_ptr()
-    return int(col), None
+    return int(col), 0
 
 
 def _heads(q, cache: KVCache):
     _tensor(q, "q", cache.device, cache.dtype)
-    _need(q.dim() == 4, "q must be (batch, tokens, heads, head_dim)")
-    B, T, Hq, D = q.shape
-    _need(B == cache.batch and D == cache.head_dim,
-          f"q {tuple(q.shape)} does not fit a cache of batch {cache.batch}, "
-          f"head_dim {cache.head_dim}")
-    return B, T, Hq, D
+    if q.dim() != 4 or q.shape[0] != cache.batch or q.shape[3] != cache.head_dim:
+        raise MEPError(f"q {tuple(q.shape)} must be (batch, tokens, heads, head_dim) and fit a "
+                       f"cache of batch {cache.batch}, head_dim {cache.head_dim}")
+    return q.shape
 
 
 def norm_rope_store(q, k, v, cos, sin, positions, cache: KVCache, layer: int, col, *,
@@ -211,40 +215,44 @@ def norm_rope_store(q, k, v, cos, sin, positions, cache: KVCache, layer: int, co
     or a one-element int64 device tensor (columns outside the cache are then
     not written). Returns the rotated q, (B, T, Hq, D) contiguous."""
     B, T, Hq, D = _heads(q, cache)
-    dev, dt = cache.device, cache.dtype
-    Hk = cache.kv_heads
-    for name, t in (("k", k), ("v", v)):
-        _tensor(t, name, dev, dt)
-        _need(t.shape == (B, T, Hk, D), f"{name} must be {(B, T, Hk, D)}, not {tuple(t.shape)}")
+    dev, dt, Hk = cache.device, cache.dtype, cache.kv_heads
+    _tensor(k, "k", dev, dt)
+    _tensor(v, "v", dev, dt)
+    if k.shape != (B, T, Hk, D) or v.shape != (B, T, Hk, D):
+        raise MEPError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must be {(B, T, Hk, D)}")
     _tensor(cos, "cos", dev)
     _tensor(sin, "sin", dev, cos.dtype)
-    _need(cos.dtype in (torch.float32, dt), f"cos and sin must be fp32 or {dt}")
-    _need(cos.dim() == 2 and cos.shape[1] == D and cos.shape == sin.shape,
-          f"cos and sin must both be (rows, {D})")
+    _need(cos.dtype is torch.float32 or cos.dtype is dt, f"cos and sin must be fp32 or {dt}")
+    rows = cos.shape[0] if cos.dim() == 2 else -1
+    _need(cos.shape == (rows, D) and sin.shape == (rows, D), f"cos and sin must be (rows, {D})")
     _tensor(positions, "positions", dev, torch.int64)
+    pb, pt = positions.stride() if positions.dim() == 2 else (0, 0)
     if positions.shape != (B, T):
-        _need(positions.dim() == 2 and positions.shape[0] == 1 and positions.shape[1] == T,
-              f"positions must be {(B, T)}, not {tuple(positions.shape)}")
-        positions = positions.expand(B, T)
-    for name, t in (("q_norm", q_norm), ("k_norm", k_norm)):
-        if t is not None:
-            _tensor(t, name, dev, dt)
-            _need(t.shape == (D,), f"{name} must be ({D},)")
-    host, devcol = _column(col, dev)
-    kp, vp, ksp, vsp = cache.layer(layer)
-    q, k, v, cos, sin = _rows(q), _rows(k), _rows(v), _flat(cos), _flat(sin)
-    q_norm = None if q_norm is None else _flat(q_norm)
-    k_norm = None if k_norm is None else _flat(k_norm)
-    out = torch.empty((B, T, Hq, D), dtype=dt, device=dev)
-    qs, ks, vs, ps = q.stride(), k.stride(), v.stride(), positions.stride()
+        _need(positions.shape == (1, T), f"positions must be {(B, T)}, not {tuple(positions.shape)}")
+        pb = 0
+    qn = kn = 0
+    if q_norm is not None:
+        _tensor(q_norm, "q_norm", dev, dt)
+        _need(q_norm.shape == (D,), f"q_norm must be ({D},)")
+        q_norm = _flat(q_norm)
+        qn = q_norm.data_ptr()
+    if k_norm is not None:
+        _tensor(k_norm, "k_norm", dev, dt)
+        _need(k_norm.shape == (D,), f"k_norm must be ({D},)")
+        k_norm = _flat(k_norm)
+        kn = k_norm.data_ptr()
+    cos, sin = _flat(cos), _flat(sin)
+    q, *qs = _rows(q)
+    k, *ks = _rows(k)
+    v, *vs = _rows(v)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    args = _lib.STORE_ARGS.pack(
+        _DTYPES[dt], cache._code, B, T, Hq, Hk, D, *qs, *ks, *vs, qn, kn, eps, cos.data_ptr(),
+        sin.data_ptr(), _DTYPES[cos.dtype], rows, positions.data_ptr(), pb, pt, out.data_ptr(),
+        *cache.layer(layer), cache.capacity, *_column(col, dev))
     with _on(dev) as stream:
-        check(_lib.lib().mep_norm_rope_store(
-            _DTYPES[dt], cache._code, B, T, Hq, Hk, D, q.data_ptr(), qs[0], qs[1], qs[2],
-            k.data_ptr(), ks[0], ks[1], ks[2], v.data_ptr(), vs[0], vs[1], vs[2],
-            None if q_norm is None else q_norm.data_ptr(),
-            None if k_norm is None else k_norm.data_ptr(), eps, cos.data_ptr(), sin.data_ptr(),
-            _DTYPES[cos.dtype], cos.shape[0], positions.data_ptr(), ps[0], ps[1], out.data_ptr(),
-            kp, vp, ksp, vsp, cache.capacity, host, devcol, stream), None, "norm_rope_store")
+        rc = _lib.lib().mep_norm_rope_store(args, stream)
+    check(rc, None, "norm_rope_store")
     return out
 
 
@@ -265,34 +273,33 @@ def cache_attention(q, cache: KVCache, layer: int, col, scale: float, *, lengths
     one-element int64 device tensor. Returns (B, T, Hq, D) contiguous; zeros
     for a query that sees nothing."""
     B, T, Hq, D = _heads(q, cache)
-    dev, dt = cache.device, cache.dtype
+    dev, dt, Hk = cache.device, cache.dtype, cache.kv_heads
+    lens = 0
     if lengths is not None:
         _tensor(lengths, "lengths", dev, torch.int64)
         _need(lengths.shape == (B,), f"lengths must be ({B},), not {tuple(lengths.shape)}")
         lengths = lengths.contiguous()
-    P, pk, pv = 0, None, None
+        lens = lengths.data_ptr()
+    P = pk = pv = 0
     if prefix is not None:
-        _need(prefix.k.device == dev and prefix.k.dtype == dt,
-              f"the prefix must be {dt} on {dev}")
-        _need(prefix.kv_heads == cache.kv_heads and prefix.head_dim == D,
+        if prefix.k.dtype is not dt or prefix.k.get_device() != dev.index:
+            raise MEPError(f"the prefix must be {dt} on {dev}")
+        _need(prefix.kv_heads == Hk and prefix.head_dim == D,
               "the prefix and the cache have different heads")
         _need(0 <= layer < prefix.layers, f"layer {layer} outside the prefix's {prefix.layers}")
         P, (pk, pv) = prefix.columns, prefix._ptrs[layer]
     host, devcol = _column(col, dev)
-    kp, vp, ksp, vsp = cache.layer(layer)
-    q = _rows(q)
-    dc = _DTYPES[dt]
-    nbytes = _attention_workspace(dc, cache._code, B, T, Hq, cache.kv_heads, D, cache.capacity,
-                                  host, P)
-    out = torch.empty((B, T, Hq, D), dtype=dt, device=dev)
+    dc, code = _DTYPES[dt], cache._code
+    nbytes = _attention_workspace(dc, code, B, T, Hq, Hk, D, cache.capacity, host, P)
+    q, *qs = _rows(q)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    qs = q.stride()
+    args = _lib.ATTENTION_ARGS.pack(
+        dc, code, B, T, Hq, Hk, D, *qs, *cache.layer(layer), cache.capacity, lens, prompt_cols,
+        host, devcol, pk, pv, P, scale, out.data_ptr(), 0 if ws is None else ws.data_ptr(), nbytes)
     with _on(dev) as stream:
-        check(_lib.lib().mep_cache_attention(
-            dc, cache._code, B, T, Hq, cache.kv_heads, D, q.data_ptr(), qs[0], qs[1], qs[2], kp,
-            vp, ksp, vsp, cache.capacity, None if lengths is None else lengths.data_ptr(),
-            prompt_cols, host, devcol, pk, pv, P, scale, out.data_ptr(),
-            None if ws is None else ws.data_ptr(), nbytes, stream), None, "cache_attention")
+        rc = _lib.lib().mep_cache_attention(args, stream)
+    check(rc, None, "cache_attention")
     return out
 
 

@@ -1,6 +1,8 @@
 """Decode-step operators without a GPU: what they refuse on the host, and the
 library's own argument checks (all made before any CUDA call)."""
 import ctypes as C
+import re
+from pathlib import Path
 
 import pytest
 import torch
@@ -29,6 +31,17 @@ def test_host_tensors_are_refused():
         M.sample_tokens([1.0], torch.zeros(2))
 
 
+def _store(lib, heads, cap=8, col=0):
+    """mep_norm_rope_store with null tensors."""
+    return lib.mep_norm_rope_store(_lib.STORE_ARGS.pack(
+        *heads, *[0] * 12, 0, 0, 1e-6, 0, 0, 0, 8, 0, 0, 0, 0, 0, 0, 0, 0, cap, col, 0), None)
+
+
+def _attend(lib, heads, cap=8, col=0):
+    return lib.mep_cache_attention(_lib.ATTENTION_ARGS.pack(
+        *heads, *[0] * 8, cap, 0, 0, col, 0, 0, 0, 0, 1.0, 0, 0, 0), None)
+
+
 def _heads(dtype=1, cache=1, B=2, T=1, Hq=4, Hk=2, D=64):
     return [dtype, cache, B, T, Hq, Hk, D]
 
@@ -44,23 +57,17 @@ def test_bad_heads(lib, bad, word):
     n = C.c_int64()
     assert lib.mep_cache_attention_workspace(*_heads(**bad), 8, 0, 0, C.byref(n)) == 1
     assert word in lib.mep_last_error(None)
-    store = [None, 0, 0, 0] * 3 + [None, None, 1e-6, None, None, 0, 8, None, 0, 0] + [None] * 5
-    assert lib.mep_norm_rope_store(*_heads(**bad), *store, 8, 0, None, None) == 1
+    assert _store(lib, _heads(**bad)) == 1
     assert word in lib.mep_last_error(None)
-    attend = [None, 0, 0, 0, None, None, None, None, 8, None, 0, 0, None, None, None, 0, 1.0, None,
-              None, 0, None]
-    assert lib.mep_cache_attention(*_heads(**bad), *attend) == 1
+    assert _attend(lib, _heads(**bad)) == 1
     assert word in lib.mep_last_error(None)
 
 
 def test_columns_and_null_tensors(lib):
-    store = [None, 0, 0, 0] * 3 + [None, None, 1e-6, None, None, 0, 8, None, 0, 0] + [None] * 5
     for cap, col, word in ((8, 8, b"fit"), (8, -1, b"fit"), (-1, 0, b"capacity"), (8, 0, b"null")):
-        assert lib.mep_norm_rope_store(*_heads(), *store, cap, col, None, None) == 1
+        assert _store(lib, _heads(), cap, col) == 1
         assert word in lib.mep_last_error(None)
-        attend = [None, 0, 0, 0, None, None, None, None, cap, None, 0, col, None, None, None, 0,
-                  1.0, None, None, 0, None]
-        assert lib.mep_cache_attention(*_heads(), *attend) == 1
+        assert _attend(lib, _heads(), cap, col) == 1
         assert (b"null" if cap == 8 and col == 0 else b"") in lib.mep_last_error(None)
     for start, n in ((-1, 2), (0, 9), (8, 1), (3, -1)):
         assert lib.mep_kv_read(1, 2, 2, 64, None, None, None, None, 8, start, n, None, None,
@@ -70,15 +77,27 @@ def test_columns_and_null_tensors(lib):
     assert lib.mep_kv_read(1, 2, 2, 64, None, None, None, None, 8, 0, 1, None, None, None) == 1
 
 
+def test_packed_arguments_match_the_header(lib):
+    """The structs are 8-byte fields in the header's order."""
+    text = (Path(__file__).resolve().parents[1] / "include" / "miniep_b200.h").read_text()
+    for name, packed in (("store", _lib.STORE_ARGS), ("attention", _lib.ATTENTION_ARGS)):
+        body = re.search(r"typedef struct mep_%s_args \{(.*?)\}" % name, text, re.S).group(1)
+        body = re.sub(r"/\*.*?\*/", "", body, flags=re.S)
+        fields = [f for d in body.split(";") if d.strip() for f in d.split(",")]
+        kinds = "".join("d" if "double" in f else "q" for f in fields)
+        want = "".join(c * int(n or 1) for n, c in re.findall(r"(\d*)([qd])", packed.format))
+        assert kinds == want
+        assert packed.size == 8 * len(fields)
+    assert lib.mep_norm_rope_store(None, None) == 1
+    assert lib.mep_cache_attention(None, None) == 1
+
+
 def test_calls_without_rows_do_nothing(lib):
     """No token, no row: fine, and no CUDA call (none would work here)."""
-    store = [None, 0, 0, 0] * 3 + [None, None, 1e-6, None, None, 0, 8, None, 0, 0] + [None] * 5
-    assert lib.mep_norm_rope_store(*_heads(B=0), *store, 8, 0, None, None) == 0
-    assert lib.mep_norm_rope_store(*_heads(T=0), *store, 8, 8, None, None) == 0
-    attend = [None, 0, 0, 0, None, None, None, None, 8, None, 0, 0, None, None, None, 0, 1.0, None,
-              None, 0, None]
-    assert lib.mep_cache_attention(*_heads(B=0), *attend) == 0
-    assert lib.mep_cache_attention(*_heads(T=0), *attend) == 0
+    assert _store(lib, _heads(B=0)) == 0
+    assert _store(lib, _heads(T=0), 8, 8) == 0
+    assert _attend(lib, _heads(B=0)) == 0
+    assert _attend(lib, _heads(T=0), 8, 8) == 0
     assert lib.mep_sample(0, None, 0, 5, 5, *[None] * 5, 1.0, 0, 1.0, 0.0, None, None, None) == 0
 
 

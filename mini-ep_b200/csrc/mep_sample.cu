@@ -90,16 +90,29 @@ constexpr int kBins = 1024;
 constexpr int kList = 1024;     // candidates the leading CTA can finish alone
 constexpr int kMaxCtas = 8;     // CTAs of a row
 
+constexpr int kCodes = 4096;    // 16-bit logits told apart by the table
+
 struct Shared {
   double tab[256];
-  uint32_t cnt[kBins], lo[kBins], hi[kBins];  // this CTA's histogram
-  u64 tmass[kBins];                           // the row's
-  uint32_t tcnt[kBins];
-  u64 item[kList], w[kList];
+  union {
+    struct {
+      uint32_t cnt[kBins], lo[kBins], hi[kBins];  // this CTA's histogram
+      u64 tmass[kBins];                           // the row's
+      uint32_t tcnt[kBins];
+      u64 item[kList], w[kList];
+    };
+    struct {
+      uint32_t total[kCodes];  // tokens of each code in the row
+      union {
+        uint32_t mine[kCodes];  // in this CTA, until they are summed
+        u64 weight[kCodes];     // a kept token's weight, by code
+      };
+    };
+  };
   u64 wmass[kMaxCtas * kNW];     // of every warp of the row
   uint32_t wties[kMaxCtas * kNW];
-  u64 best[kMaxCtas];
-  float lmin[kMaxCtas];
+  u64 best[kMaxCtas], zero[kMaxCtas];
+  float lmax[kMaxCtas], lmin[kMaxCtas];
   u64 red[kNW], red2[kNW];
   uint32_t n_items;
   // results that one thread finds for all
@@ -107,7 +120,8 @@ struct Shared {
   u64 r_above, r_mass;
 };
 
-// 16 bytes of a row: ids at `first` + 0..E-1, -inf outside [0, vocab)
+// 16 bytes of a row: ids from `id` on, NaN (which counts as -inf and is no
+// minimum) outside [0, vocab)
 template <typename T>
 struct Vec {
   static constexpr int E = 16 / sizeof(T);
@@ -131,9 +145,37 @@ __device__ __forceinline__ uint4 fetch(const T* row, int id, int vocab) {
   __align__(16) T x[E];
 #pragma unroll
   for (int i = 0; i < E; ++i)
-    x[i] = id + i >= 0 && id + i < vocab ? row[id + i] : Elt<T>::from_f(-INFINITY);
+    x[i] = id + i >= 0 && id + i < vocab ? row[id + i] : Elt<T>::from_f(__int_as_float(0x7fffffff));
   return *reinterpret_cast<const uint4*>(x);
 }
+
+// largest and smallest of a piece into hi and lo; NaN is neither
+__device__ __forceinline__ void extremes(const uint4& v, float (&hi)[1], float (&lo)[1]) {
+  float x[4];
+  unpack(v, x);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) hi[0] = fmaxf(hi[0], x[i]), lo[0] = fminf(lo[0], x[i]);
+}
+__device__ __forceinline__ void extremes(const uint4& v, __nv_bfloat162& hi, __nv_bfloat162& lo) {
+  const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __nv_bfloat162 x = *reinterpret_cast<const __nv_bfloat162*>(&u[i]);
+    hi = __hmax2(hi, x), lo = __hmin2(lo, x);
+  }
+}
+template <typename T>
+struct Extremes {
+  float hi[1] = {-INFINITY}, lo[1] = {INFINITY};
+  __device__ float high() const { return hi[0]; }
+  __device__ float low() const { return lo[0]; }
+};
+template <>
+struct Extremes<__nv_bfloat16> {
+  __nv_bfloat162 hi = __float2bfloat162_rn(-INFINITY), lo = __float2bfloat162_rn(INFINITY);
+  __device__ float high() const { return fmaxf(__low2float(hi), __high2float(hi)); }
+  __device__ float low() const { return fminf(__low2float(lo), __high2float(lo)); }
+};
 
 __device__ __forceinline__ u64 warp_sum(u64 v) {
 #pragma unroll
@@ -188,8 +230,14 @@ __device__ void sort_desc(u64* x, int n) {
 // per warp as without a filter. A bin too large for that, and a second border
 // behind a wide top_k, are found by histograms over ever narrower key ranges.
 // All sums are of integers: their order is free.
+//
+// 16-bit logits have few values: where those from lcut to lmax are at most
+// kCodes (with all below 2^-7 in magnitude taken as one), the row's tokens are
+// counted by value, one addition a token; the borders follow from the counts
+// and a weight for each value, and the sums over ids read a table of the kept
+// values' weights instead of computing 100,000 exponentials.
 template <typename T, bool CACHED>
-__global__ void __launch_bounds__(kNT) k_sample(const SampleArgs a) {
+__global__ void __launch_bounds__(kNT, 2) k_sample(const SampleArgs a) {
   constexpr int E = Vec<T>::E;
   extern __shared__ __align__(16) unsigned char smem_raw[];
   Shared& S = *reinterpret_cast<Shared*>(smem_raw);
@@ -227,63 +275,73 @@ __global__ void __launch_bounds__(kNT) k_sample(const SampleArgs a) {
     }
   };
 
-  // ---- the best token and the smallest finite logit
+  // ---- the largest and the smallest logit
+  constexpr bool kTable = sizeof(T) == 2;
   if (tid < 256) S.tab[tid] = exp2(tid / 256.0);
-  for (int i = tid; i < kBins; i += kNT) S.cnt[i] = S.lo[i] = S.hi[i] = 0;
+  if (kTable)
+    for (int i = tid; i < kCodes; i += kNT) S.mine[i] = 0;
   if (tid == 0) S.n_items = 0;
-  u64 best = 0;
-  float lmin = INFINITY;
+  Extremes<T> ex;
   for (int p = w0 + lane; p < w1; p += 32) {
     const uint4 v = fetch<T>(x, p * E - shift, V);
     if (CACHED) cache[p - p0] = v;
-    float l[E];
-    unpack(v, l);
-#pragma unroll
-    for (int i = 0; i < E; ++i) {
-      const int id = p * E - shift + i;
-      if (id >= 0 && id < V) {
-        const u64 c = (u64)key_of(l[i]) << 32 | (uint32_t)~(uint32_t)id;
-        best = c > best ? c : best;
-      }
-      if (l[i] > -INFINITY) lmin = fminf(lmin, l[i]);
-    }
+    extremes(v, ex.hi, ex.lo);
   }
+  float lmax = ex.high(), lmin = ex.low();
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
-    const u64 c = __shfl_xor_sync(0xffffffffu, best, o);
-    best = c > best ? c : best;
+    lmax = fmaxf(lmax, __shfl_xor_sync(0xffffffffu, lmax, o));
     lmin = fminf(lmin, __shfl_xor_sync(0xffffffffu, lmin, o));
   }
-  if (lane == 0) S.red[warp] = best, S.red2[warp] = __float_as_uint(lmin);
+  if (lane == 0) S.red[warp] = __float_as_uint(lmax), S.red2[warp] = __float_as_uint(lmin);
   __syncthreads();
   if (tid < nc) {
     for (int i = 0; i < kNW; ++i) {
-      best = S.red[i] > best ? S.red[i] : best;
+      lmax = fmaxf(lmax, __uint_as_float((uint32_t)S.red[i]));
       lmin = fminf(lmin, __uint_as_float((uint32_t)S.red2[i]));
     }
     Shared* to = cluster.map_shared_rank(&S, tid);
-    to->best[rank] = best;
+    to->lmax[rank] = lmax;
     to->lmin[rank] = lmin;
   }
   cluster.sync();
-  best = 0;
   for (int i = 0; i < nc; ++i) {
-    best = S.best[i] > best ? S.best[i] : best;
+    lmax = fmaxf(lmax, S.lmax[i]);
     lmin = fminf(lmin, S.lmin[i]);
   }
-  const uint32_t kmax = (uint32_t)(best >> 32);
-  if (kmax == kKeyNegInf || !(temp > 0.f)) {  // nothing to draw, or the best token
+  lmax += 0.f;
+  const uint32_t kmax = key_of(lmax);
+  if (kmax == kKeyNegInf) {  // nothing to draw
     if (rank == 0 && tid == 0) {
-      const bool none = kmax == kKeyNegInf;
-      a.tokens[row] = none ? -1 : (int64_t)(uint32_t)~(uint32_t)best;
-      if (a.logprobs) a.logprobs[row] = none ? -INFINITY : 0.f;
+      a.tokens[row] = -1;
+      if (a.logprobs) a.logprobs[row] = -INFINITY;
+    }
+    return;
+  }
+  if (!(temp > 0.f)) {  // the best token of the lowest id
+    int id0 = 0x7fffffff;
+    each([&](float l, int id) {
+      if (l == lmax) id0 = min(id0, id);
+    });
+    id0 = __reduce_min_sync(0xffffffffu, id0);
+    if (lane == 0) S.red[warp] = (uint32_t)id0;
+    __syncthreads();
+    if (tid == 0) {
+      for (int i = 0; i < kNW; ++i) id0 = min(id0, (int)S.red[i]);
+      cluster.map_shared_rank(&S, 0)->best[rank] = (uint32_t)id0;
+    }
+    cluster.sync();
+    if (rank == 0 && tid == 0) {
+      for (int i = 0; i < nc; ++i) id0 = min(id0, (int)S.best[i]);
+      a.tokens[row] = id0;
+      if (a.logprobs) a.logprobs[row] = 0.f;
     }
     return;
   }
   int bits = 0;
   while ((1 << bits) < V) ++bits;
   Weights W;
-  W.lmax = logit_of(kmax);
+  W.lmax = lmax;
   // 34 temperatures below the best a weight is 2^-49; lmax = inf leaves only
   // its equals, -inf never weighs
   W.lcut = fmaxf(W.lmax - 34.f * temp, -3.402823466e38f);
@@ -330,6 +388,213 @@ __global__ void __launch_bounds__(kNT) k_sample(const SampleArgs a) {
     }
     cluster.sync();
   };
+
+  // weights below min_p's border weigh nothing (the best token's is 2^scale)
+  auto floored = [&](u64 w) {
+    return (double)w < floor_p && w < 1ull << W.scale ? 0ull : w;
+  };
+  // ---- the draw: weigh(l) is a token's kept weight; of the tokens with
+  // on_edge(l) the first `ties` ids weigh `wedge` each
+  auto finish = [&](auto weigh, auto on_edge, u64 ties, u64 wedge) {
+    u64 mass = 0;
+    uint32_t n_edge = 0;
+    for (int p = w0 + lane; p < w1; p += 32) {
+      float l[E];
+      unpack(piece(p), l);
+#pragma unroll
+      for (int i = 0; i < E; ++i) mass += weigh(l[i]), n_edge += on_edge(l[i]);
+    }
+    mass = warp_sum(mass);
+    n_edge = __reduce_add_sync(0xffffffffu, n_edge);
+    if (lane < nc) {
+      Shared* to = cluster.map_shared_rank(&S, lane);
+      to->wmass[rank * kNW + warp] = mass;
+      to->wties[rank * kNW + warp] = n_edge;
+    }
+    cluster.sync();
+    // this warp's share begins at `start`; the row's kept mass is `total`
+    constexpr int PW = kMaxCtas * kNW / 32;
+    u64 share[PW], sum = 0, start = 0, total;
+    uint32_t t[PW], seen = 0;
+#pragma unroll
+    for (int i = 0; i < PW; ++i) {
+      const int j = lane * PW + i;
+      share[i] = j < nc * kNW ? S.wmass[j] : 0;
+      t[i] = j < nc * kNW ? S.wties[j] : 0;
+      seen += t[i];
+    }
+    uint32_t at = (uint32_t)warp_scan(seen) - seen, before = 0;
+    const int me = rank * kNW + warp;
+#pragma unroll
+    for (int i = 0; i < PW; ++i) {
+      if (lane * PW + i == me) before = at;
+      share[i] += min((u64)t[i], ties > at ? ties - at : 0) * wedge;
+      at += t[i];
+      sum += share[i];
+    }
+    const u64 inc = warp_scan(sum);
+    total = __shfl_sync(0xffffffffu, inc, 31);
+    u64 run0 = inc - sum;
+#pragma unroll
+    for (int i = 0; i < PW; ++i) {
+      if (lane * PW + i == me) start = run0;
+      run0 += share[i];
+    }
+    start = __shfl_sync(0xffffffffu, start, me / PW);
+    before = __shfl_sync(0xffffffffu, before, me / PW);
+    const u64 target = target_of(total);
+    const u64 own = mass + min((u64)n_edge, ties > before ? ties - before : 0) * wedge;
+    if (target < start || target >= start + own) return;
+    for (int p = w0; p < w1; p += 32) {
+      float l[E];
+      const bool have = p + lane < w1;
+      if (have) unpack(piece(p + lane), l);
+      u64 w[E], sum = 0;
+      uint32_t eq = 0;
+#pragma unroll
+      for (int i = 0; i < E; ++i) eq += have && on_edge(l[i]);
+      u64 nth = before + warp_scan(eq) - eq;  // ids on the edge before this lane's
+      before += __reduce_add_sync(0xffffffffu, eq);
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        w[i] = have ? weigh(l[i]) : 0;
+        if (have && on_edge(l[i])) w[i] = nth++ < ties ? wedge : 0;
+        sum += w[i];
+      }
+      u64 run = warp_scan(sum);
+      const u64 step = __shfl_sync(0xffffffffu, run, 31);
+      run += start - sum;
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        if (run <= target && run + w[i] > target)
+          answer((p + lane) * E - shift + i, w[i], total);
+        run += w[i];
+      }
+      start += step;
+      if (start > target) return;
+    }
+  };
+
+  if constexpr (kTable) {
+    // ---- codes: s(l) counts the 16-bit values from 2^-7 in magnitude on, 0
+    // for all below; a token's code is s(lmax) - s(l)
+    constexpr int kSmall = (127 - 7) << 7;
+    auto step_of = [&](float l) {
+      const int b = __float_as_int(l);
+      const int t = max(((b >> 16) & 0x7fff) - (kSmall - 1), 0);
+      return b < 0 ? -t : t;
+    };
+    const int smax = step_of(W.lmax), codes = smax - step_of(W.lcut) + 1;
+    if (codes <= kCodes) {
+      const uint32_t small = smax >= 0 ? smax : kCodes + 1;  // the code of the small ones
+      auto code_of = [&](float l) { return (uint32_t)(smax - step_of(l)); };
+      auto logit = [&](uint32_t code) {
+        const int s = smax - (int)code, t = s < 0 ? -s : s;
+        return __int_as_float((s < 0 ? 0x80000000u : 0u) | (uint32_t)(t + kSmall - 1) << 16);
+      };
+      u64 zall = 0, limit_k = 0;  // the small ones' mass, the mass top_p is of
+      if (by_k || by_p) {
+        each([&](float l, int) {
+          const uint32_t c = code_of(l);
+          if (c < (uint32_t)codes) {
+            atomicAdd(&S.mine[c], 1u);
+            if (c == small) zall += W(l);
+          }
+        });
+        u64 all;
+        block_scan(zall, S.red, all);
+        if (tid < nc) cluster.map_shared_rank(&S, tid)->zero[rank] = all;
+        cluster.sync();
+        for (int i = tid; i < kCodes / nc; i += kNT) {
+          const int c = rank * (kCodes / nc) + i;
+          uint32_t n = 0;
+          if (c < codes) {
+            for (int r = 0; r < nc; ++r) n += cluster.map_shared_rank(&S, r)->mine[c];
+            for (int r = 0; r < nc; ++r) cluster.map_shared_rank(&S, r)->total[c] = n;
+          }
+        }
+        cluster.sync();
+        zall = 0;
+        for (int i = 0; i < nc; ++i) zall += S.zero[i];
+      }
+      // ---- kCodes / kNT codes a thread: weights, then the borders
+      constexpr int PER = kCodes / kNT;
+      const int c0 = tid * PER;
+      uint32_t ecode = kCodes;  // codes before it are kept, and `ties` tokens of it
+      u64 ties = 0, w[PER];
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        w[i] = c0 + i < codes && c0 + i != (int)small ? W(logit(c0 + i)) : 0;
+      if (by_k || by_p) {
+        uint32_t t[PER];
+        u64 n = 0, m = 0, all;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          t[i] = c0 + i < codes ? S.total[c0 + i] : 0;
+          n += t[i];
+          m += c0 + i == (int)small ? zall : t[i] * w[i];
+        }
+        const u64 m0 = block_scan(m, S.red2, limit_k);
+        if (by_k) {
+          u64 nb = block_scan(n, S.red, all), mb = m0;
+          if ((u64)top_k < all) {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+              if (nb < (u64)top_k && nb + t[i] >= (u64)top_k) {
+                S.r_bin = c0 + i;
+                S.r_above = (u64)top_k - nb;
+                S.r_mass = mb + S.r_above * w[i];
+              }
+              nb += t[i];
+              mb += c0 + i == (int)small ? zall : t[i] * w[i];
+            }
+            __syncthreads();
+            ecode = S.r_bin, ties = S.r_above, limit_k = S.r_mass;
+            __syncthreads();
+          }
+        }
+        if (by_p && ecode != small) {
+          const double limit = (double)top_p * (double)limit_k;
+          if (tid == 0) S.r_bin = 0, S.r_above = 1;  // top_p <= 0: the best token
+          __syncthreads();
+          u64 mb = m0;
+#pragma unroll
+          for (int i = 0; i < PER; ++i) {
+            const u64 here = c0 + i == (int)small ? zall : t[i] * w[i];
+            if ((double)mb < limit && (double)(mb + here) >= limit && here > 0) {
+              S.r_bin = c0 + i;
+              S.r_above = w[i] > 0 ? (u64)fmax(1.0, ceil((limit - (double)mb) / (double)w[i])) : 0;
+            }
+            mb += here;
+          }
+          __syncthreads();
+          if (S.r_bin < ecode || S.r_above < ties) ecode = S.r_bin, ties = S.r_above;
+        }
+      }
+      // a border among the small ones is left to the search below
+      if (ecode != small) {
+        __syncthreads();  // `mine` becomes `weight`
+#pragma unroll
+        for (int i = 0; i < PER; ++i)  // 0 for the small ones, behind lcut and from the border on
+          S.weight[c0 + i] = c0 + i < (int)ecode ? floored(w[i]) : 0;
+        __syncthreads();
+        const u64 wedge = ecode < (uint32_t)codes ? floored(W(logit(ecode))) : 0;
+        const bool some_small = small < ecode;
+        finish(
+            [&](float l) -> u64 {
+              const uint32_t c = code_of(l);
+              if (c >= (uint32_t)codes) return 0;
+              if (c == small) return some_small ? floored(W(l)) : 0;
+              return S.weight[c];
+            },
+            [&](float l) { return code_of(l) == ecode; }, ties, wedge);
+        return;
+      }
+    }
+    cluster.sync();  // the counts have been read everywhere
+  }
+  for (int i = tid; i < kBins; i += kNT) S.cnt[i] = S.lo[i] = S.hi[i] = 0;
+  __syncthreads();
 
   uint32_t edge = 0;  // kept: keys above `edge`, and the first `ties` ids of key `edge`
   u64 ties = ~0ull;
@@ -587,82 +852,13 @@ __global__ void __launch_bounds__(kNT) k_sample(const SampleArgs a) {
     }
   }
 
-  // ---- each warp's kept mass and its tokens on the edge, to every CTA
-  const u64 wedge = W(logit_of(edge));
-  auto low = [&](u64 w) { return (double)w < floor_p && w < 1ull << W.scale; };
-  u64 mass = 0;
-  uint32_t on_edge = 0;
-  each([&](float l, int id) {
-    const uint32_t k = key_of(l);
-    if (k > edge) {
-      const u64 w = W(l);
-      if (!low(w)) mass += w;
-    }
-    on_edge += k == edge && id >= 0 && id < V;
-  });
-  mass = warp_sum(mass);
-  on_edge = __reduce_add_sync(0xffffffffu, on_edge);
-  if (lane < nc) {
-    Shared* to = cluster.map_shared_rank(&S, lane);
-    to->wmass[rank * kNW + warp] = mass;
-    to->wties[rank * kNW + warp] = on_edge;
-  }
-  cluster.sync();
-  // this warp's share begins at `start`; the row's kept mass is `total`
-  const bool edge_kept = edge && wedge > 0 && !low(wedge);
-  u64 start = 0, total = 0, ties_before = 0, seen = 0;
-  for (int i = 0; i < nc * kNW; ++i) {
-    if (i == rank * kNW + warp) start = total, ties_before = seen;
-    const u64 left = ties > seen ? ties - seen : 0;
-    total += S.wmass[i] + (edge_kept ? min((u64)S.wties[i], left) * wedge : 0);
-    seen += S.wties[i];
-  }
-  const u64 target = target_of(total);
-  u64 own = mass;
-  if (edge_kept) own += min((u64)on_edge, ties > ties_before ? ties - ties_before : 0) * wedge;
-  if (target < start || target >= start + own) return;
-  for (int p = w0; p < w1; p += 32) {
-    float l[E];
-    const bool have = p + lane < w1;
-    if (have) unpack(piece(p + lane), l);
-    u64 w[E], sum = 0;
-    uint32_t eq = 0;
-    const int id0 = (p + lane) * E - shift;
-#pragma unroll
-    for (int i = 0; i < E; ++i)
-      eq += have && id0 + i >= 0 && id0 + i < V && key_of(l[i]) == edge;
-    u64 rank_eq = ties_before + warp_scan(eq) - eq;
-    ties_before += __reduce_add_sync(0xffffffffu, eq);
-#pragma unroll
-    for (int i = 0; i < E; ++i) {
-      w[i] = 0;
-      if (have && id0 + i >= 0 && id0 + i < V) {
-        const uint32_t k = key_of(l[i]);
-        if (k > edge) {
-          w[i] = W(l[i]);
-          if (low(w[i])) w[i] = 0;
-        } else if (k == edge) {
-          if (edge_kept && rank_eq < ties) w[i] = wedge;
-          ++rank_eq;
-        }
-      }
-      sum += w[i];
-    }
-    u64 run = warp_scan(sum);
-    const u64 step = __shfl_sync(0xffffffffu, run, 31);
-    run += start - sum;
-#pragma unroll
-    for (int i = 0; i < E; ++i) {
-      if (run <= target && run + w[i] > target) answer(id0 + i, w[i], total);
-      run += w[i];
-    }
-    start += step;
-    if (start > target) return;
-  }
+  finish([&](float l) { return key_of(l) > edge ? floored(W(l)) : 0ull; },
+         [&](float l) { return key_of(l) == edge; }, ties,
+         edge ? floored(W(logit_of(edge))) : 0ull);
 }
 
 constexpr int kSharedBytes = (int)((sizeof(Shared) + 15) / 16 * 16);
-constexpr int64_t kSliceBytes = 64 << 10;       // of a row in a CTA: two CTAs an SM
+constexpr int64_t kSliceBytes = 56 << 10;       // of a row in a CTA: two CTAs an SM
 constexpr int64_t kMostSliceBytes = 160 << 10;  // one
 
 template <typename T>

@@ -422,6 +422,20 @@ def test_sample_wide_rows_and_nuclei(filt):
     draw_rows(tied, torch.rand(4, generator=gen(2), device="cuda"), *filt)
 
 
+def test_sample_small_and_large_logits():
+    """16-bit rows around zero (values below 2^-7 and the border among them),
+    all negative, far from zero, and wider than the table of values."""
+    for V in (300, 20011):
+        for scale, shift in ((1e-3, 0.0), (4e-3, 0.0), (0.05, 0.0), (1.0, -9.0), (1.0, 300.0),
+                             (900.0, 0.0), (30.0, 5000.0), (1e-6, 2e-3)):
+            g = gen(V)
+            logits = (randn(g, 3, V) * scale + shift).to(BF)
+            u = torch.rand(3, generator=g, device="cuda")
+            for filt in ((1.0, 0, 1.0, 0.0), (0.5, 100, 0.7, 0.0), (0.7, 0, 0.6, 1e-3),
+                         (1e-3, 0, 0.9, 0.0), (2.0, 150, 1.0, 0.2)):
+                draw_rows(logits, u, *filt)
+
+
 def test_sample_every_row_count():
     """Row counts that change how many CTAs share a row."""
     for B in (1, 9, 18, 37, 74, 150, 300):

@@ -220,9 +220,11 @@ __device__ void sort_desc(u64* x, int n) {
   __syncthreads();
 }
 
-// A cluster of CTAs takes a row; each keeps a run of its ids in shared memory
-// (CACHED) or re-reads it, each warp a run of that, so that sums over ids stay
-// in order. Without a filter the weights are summed per warp, and the warp
+// A cluster of CTAs takes a row, each a run of its ids, each warp a run of
+// that, so that sums over ids stay in order. The passes after the first read a
+// short run from shared memory and a long one from L2 (a whole row in shared
+// memory would take an SM for itself).
+// Without a filter the weights are summed per warp, and the warp
 // whose share holds the target finds the token. With top_k or top_p a
 // histogram over the logits (counts, or masses) tells which bins can hold kept
 // tokens. When those are at most kList the leading CTA sorts and finishes them
@@ -232,16 +234,15 @@ __device__ void sort_desc(u64* x, int n) {
 // All sums are of integers: their order is free.
 //
 // 16-bit logits have few values: where those from lcut to lmax are at most
-// kCodes (with all below 2^-7 in magnitude taken as one), the row's tokens are
+// kCodes (with all below 2^-9 in magnitude taken as one), the row's tokens are
 // counted by value, one addition a token; the borders follow from the counts
 // and a weight for each value, and the sums over ids read a table of the kept
 // values' weights instead of computing 100,000 exponentials.
-template <typename T, bool CACHED>
-__global__ void __launch_bounds__(kNT, 2) k_sample(const SampleArgs a) {
+template <typename T>
+__global__ void __launch_bounds__(kNT, 2) k_sample(const SampleArgs a, int cached) {
   constexpr int E = Vec<T>::E;
   extern __shared__ __align__(16) unsigned char smem_raw[];
   Shared& S = *reinterpret_cast<Shared*>(smem_raw);
-  uint4* cache = reinterpret_cast<uint4*>(smem_raw + (sizeof(Shared) + 15) / 16 * 16);
   cg::cluster_group cluster = cg::this_cluster();
   const int nc = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int64_t row = blockIdx.x / nc;
@@ -262,17 +263,25 @@ __global__ void __launch_bounds__(kNT, 2) k_sample(const SampleArgs a) {
   const int per_w = ((p1 - p0 + kNW - 1) / kNW + 31) / 32 * 32;
   const int w0 = min(p1, p0 + per_w * warp), w1 = min(p1, w0 + per_w);
 
-  auto piece = [&](int p) -> uint4 {
-    return CACHED ? cache[p - p0] : fetch<T>(x, p * E - shift, V);
+  uint4* kept = reinterpret_cast<uint4*>(smem_raw + (sizeof(Shared) + 15) / 16 * 16);
+  auto piece = [&](int p) { return cached ? kept[p - p0] : fetch<T>(x, p * E - shift, V); };
+  // f(piece, first id) for this lane's pieces, two loads under way
+  auto each_piece = [&](auto f) {
+    for (int p = w0 + lane; p < w1; p += 64) {
+      const uint4 a0 = piece(p);
+      const uint4 a1 = p + 32 < w1 ? piece(p + 32) : make_uint4(~0u, ~0u, ~0u, ~0u);  // NaN
+      f(a0, p * E - shift);
+      f(a1, (p + 32) * E - shift);
+    }
   };
   // f(l, id) for this warp's ids
   auto each = [&](auto f) {
-    for (int p = w0 + lane; p < w1; p += 32) {
+    each_piece([&](const uint4& v, int id0) {
       float l[E];
-      unpack(piece(p), l);
+      unpack(v, l);
 #pragma unroll
-      for (int i = 0; i < E; ++i) f(l[i], p * E - shift + i);
-    }
+      for (int i = 0; i < E; ++i) f(l[i], id0 + i);
+    });
   };
 
   // ---- the largest and the smallest logit
@@ -282,10 +291,17 @@ __global__ void __launch_bounds__(kNT, 2) k_sample(const SampleArgs a) {
     for (int i = tid; i < kCodes; i += kNT) S.mine[i] = 0;
   if (tid == 0) S.n_items = 0;
   Extremes<T> ex;
-  for (int p = w0 + lane; p < w1; p += 32) {
-    const uint4 v = fetch<T>(x, p * E - shift, V);
-    if (CACHED) cache[p - p0] = v;
-    extremes(v, ex.hi, ex.lo);
+  for (int p = w0 + lane; p < w1; p += 128) {  // four loads under way
+    uint4 v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      v[i] = p + 32 * i < w1 ? fetch<T>(x, (p + 32 * i) * E - shift, V)
+                             : make_uint4(~0u, ~0u, ~0u, ~0u);  // NaN
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (cached && p + 32 * i < w1) kept[p + 32 * i - p0] = v[i];
+      extremes(v[i], ex.hi, ex.lo);
+    }
   }
   float lmax = ex.high(), lmin = ex.low();
 #pragma unroll
@@ -350,7 +366,10 @@ __global__ void __launch_bounds__(kNT, 2) k_sample(const SampleArgs a) {
   W.scale = min(46, 62 - bits);
   W.tab = S.tab;
   const double one = (double)(1ull << W.scale);
-  const double floor_p = (double)min_p * one;
+  // integer borders: w >= min_p * one, and mass < top_p * total, are w >= and <
+  // their next integers
+  auto ceiling = [&](double v) { return v > 0.0 ? (u64)ceil(v) : 0ull; };
+  const u64 floor_p = ceiling((double)min_p * one);
   const bool by_k = top_k > 0 && top_k < V, by_p = top_p < 1.f;
   const double u = a.u[row];
   auto target_of = [&](u64 total) {
@@ -391,19 +410,17 @@ __global__ void __launch_bounds__(kNT, 2) k_sample(const SampleArgs a) {
 
   // weights below min_p's border weigh nothing (the best token's is 2^scale)
   auto floored = [&](u64 w) {
-    return (double)w < floor_p && w < 1ull << W.scale ? 0ull : w;
+    return w < floor_p && w < 1ull << W.scale ? 0ull : w;
   };
   // ---- the draw: weigh(l) is a token's kept weight; of the tokens with
   // on_edge(l) the first `ties` ids weigh `wedge` each
   auto finish = [&](auto weigh, auto on_edge, u64 ties, u64 wedge) {
     u64 mass = 0;
     uint32_t n_edge = 0;
-    for (int p = w0 + lane; p < w1; p += 32) {
-      float l[E];
-      unpack(piece(p), l);
-#pragma unroll
-      for (int i = 0; i < E; ++i) mass += weigh(l[i]), n_edge += on_edge(l[i]);
-    }
+    if (wedge)
+      each([&](float l, int) { mass += weigh(l), n_edge += on_edge(l); });
+    else
+      each([&](float l, int) { mass += weigh(l); });
     mass = warp_sum(mass);
     n_edge = __reduce_add_sync(0xffffffffu, n_edge);
     if (lane < nc) {
@@ -476,65 +493,89 @@ __global__ void __launch_bounds__(kNT, 2) k_sample(const SampleArgs a) {
   };
 
   if constexpr (kTable) {
-    // ---- codes: s(l) counts the 16-bit values from 2^-7 in magnitude on, 0
-    // for all below; a token's code is s(lmax) - s(l)
-    constexpr int kSmall = (127 - 7) << 7;
-    auto step_of = [&](float l) {
-      const int b = __float_as_int(l);
-      const int t = max(((b >> 16) & 0x7fff) - (kSmall - 1), 0);
-      return b < 0 ? -t : t;
-    };
-    const int smax = step_of(W.lmax), codes = smax - step_of(W.lcut) + 1;
-    if (codes <= kCodes) {
-      const uint32_t small = smax >= 0 ? smax : kCodes + 1;  // the code of the small ones
-      auto code_of = [&](float l) { return (uint32_t)(smax - step_of(l)); };
-      auto logit = [&](uint32_t code) {
-        const int s = smax - (int)code, t = s < 0 ? -s : s;
-        return __int_as_float((s < 0 ? 0x80000000u : 0u) | (uint32_t)(t + kSmall - 1) << 16);
+    // ---- a slot for each 16-bit value from 2^-9 to 2^7 in magnitude: kHalf of
+    // either sign in the order of their bits. By rank, best first: positive
+    // ones from lmax down, all smaller ones as one, negative ones.
+    constexpr int kSmall = (127 - 9) << 7, kHalf = kCodes / 2;
+    const int top_mag = __float_as_int(W.lmax) >> 16 & 0x7fff;
+    const bool neg = W.lmax < 0.f && top_mag >= kSmall;  // all negative, none small
+    const int n_pos = W.lmax < 0.f ? 0 : max(top_mag - kSmall + 1, 0);
+    const int cut_mag = __float_as_int(W.lcut) >> 16 & 0x7fff;
+    const bool fits = top_mag < kSmall + kHalf - 1 &&
+                      (W.lcut >= 0.f || cut_mag < kSmall + kHalf);
+    if (fits) {
+      auto slot_of = [&](uint32_t bits) {  // of 16 bits; >= kCodes: small, or none
+        const uint32_t c = (bits & 0x7fff) - kSmall;
+        return c < (uint32_t)kHalf ? c + (bits >> 15) * kHalf : ~0u;
       };
-      u64 zall = 0, limit_k = 0;  // the small ones' mass, the mass top_p is of
+      auto slot_at = [&](int rank) {  // n_pos (if not negative): the small ones' rank
+        return rank < n_pos ? n_pos - 1 - rank : kHalf + rank - n_pos - 1;
+      };
+      auto logit = [&](int slot) {
+        const int mag = kSmall + (slot < kHalf ? slot : slot - kHalf);
+        return __int_as_float((slot < kHalf ? 0u : 0x80000000u) | (uint32_t)mag << 16);
+      };
+      auto small = [&](float l) { return fabsf(l) < 0x1p-9f; };
+      u64 zall = 0, mass_p = 0;  // the small ones' mass, the mass top_p is of
+      uint32_t zcnt = 0;
       if (by_k || by_p) {
-        each([&](float l, int) {
-          const uint32_t c = code_of(l);
-          if (c < (uint32_t)codes) {
-            atomicAdd(&S.mine[c], 1u);
-            if (c == small) zall += W(l);
+        each_piece([&](const uint4& v, int) {
+          const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const uint32_t b = i & 1 ? u[i >> 1] >> 16 : u[i >> 1] & 0xffff, c = slot_of(b);
+            if (c < (uint32_t)kCodes) {
+              atomicAdd(&S.mine[c], 1u);
+            } else {
+              const float l = __uint_as_float(b << 16);
+              if (small(l)) zall += W(l), ++zcnt;
+            }
           }
         });
-        u64 all;
+        u64 all, nz;
         block_scan(zall, S.red, all);
-        if (tid < nc) cluster.map_shared_rank(&S, tid)->zero[rank] = all;
+        block_scan(zcnt, S.red2, nz);
+        if (tid < nc) {
+          Shared* to = cluster.map_shared_rank(&S, tid);
+          to->zero[rank] = all;
+          to->best[rank] = nz;
+        }
         cluster.sync();
-        for (int i = tid; i < kCodes / nc; i += kNT) {
-          const int c = rank * (kCodes / nc) + i;
-          uint32_t n = 0;
-          if (c < codes) {
+        if (nc > 1) {
+          const int share = kCodes / nc;
+          for (int i = tid; i < share; i += kNT) {
+            const int c = rank * share + i;
+            uint32_t n = 0;
             for (int r = 0; r < nc; ++r) n += cluster.map_shared_rank(&S, r)->mine[c];
             for (int r = 0; r < nc; ++r) cluster.map_shared_rank(&S, r)->total[c] = n;
           }
+          cluster.sync();
         }
-        cluster.sync();
-        zall = 0;
-        for (int i = 0; i < nc; ++i) zall += S.zero[i];
+        zall = 0, zcnt = 0;
+        for (int i = 0; i < nc; ++i) zall += S.zero[i], zcnt += (uint32_t)S.best[i];
       }
-      // ---- kCodes / kNT codes a thread: weights, then the borders
+      const uint32_t* total = nc > 1 ? S.total : S.mine;
+      // ---- PER ranks a thread: weights, then the borders
       constexpr int PER = kCodes / kNT;
-      const int c0 = tid * PER;
-      uint32_t ecode = kCodes;  // codes before it are kept, and `ties` tokens of it
+      const int c0 = tid * PER, z = neg ? -1 : n_pos;  // z: the small ones' rank
+      // all negative and large: ranks start behind slot kHalf
+      auto at = [&](int rank) { return neg ? kHalf + top_mag - kSmall + rank : slot_at(rank); };
+      const int ranks = neg ? kHalf - (top_mag - kSmall) : n_pos + 1 + kHalf;
+      int erank = 1 << 20;  // ranks before it are kept, and `ties` tokens of it
       u64 ties = 0, w[PER];
 #pragma unroll
       for (int i = 0; i < PER; ++i)
-        w[i] = c0 + i < codes && c0 + i != (int)small ? W(logit(c0 + i)) : 0;
+        w[i] = c0 + i < ranks && c0 + i != z ? W(logit(at(c0 + i))) : 0;
       if (by_k || by_p) {
         uint32_t t[PER];
         u64 n = 0, m = 0, all;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-          t[i] = c0 + i < codes ? S.total[c0 + i] : 0;
+          t[i] = c0 + i >= ranks ? 0 : c0 + i == z ? zcnt : total[at(c0 + i)];
           n += t[i];
-          m += c0 + i == (int)small ? zall : t[i] * w[i];
+          m += c0 + i == z ? zall : t[i] * w[i];
         }
-        const u64 m0 = block_scan(m, S.red2, limit_k);
+        const u64 m0 = block_scan(m, S.red2, mass_p);
         if (by_k) {
           u64 nb = block_scan(n, S.red, all), mb = m0;
           if ((u64)top_k < all) {
@@ -546,48 +587,52 @@ __global__ void __launch_bounds__(kNT, 2) k_sample(const SampleArgs a) {
                 S.r_mass = mb + S.r_above * w[i];
               }
               nb += t[i];
-              mb += c0 + i == (int)small ? zall : t[i] * w[i];
+              mb += c0 + i == z ? zall : t[i] * w[i];
             }
             __syncthreads();
-            ecode = S.r_bin, ties = S.r_above, limit_k = S.r_mass;
+            erank = S.r_bin, ties = S.r_above, mass_p = S.r_mass;
             __syncthreads();
           }
         }
-        if (by_p && ecode != small) {
-          const double limit = (double)top_p * (double)limit_k;
+        if (by_p && erank != z) {
+          const u64 limit = ceiling((double)top_p * (double)mass_p);
           if (tid == 0) S.r_bin = 0, S.r_above = 1;  // top_p <= 0: the best token
           __syncthreads();
           u64 mb = m0;
 #pragma unroll
           for (int i = 0; i < PER; ++i) {
-            const u64 here = c0 + i == (int)small ? zall : t[i] * w[i];
-            if ((double)mb < limit && (double)(mb + here) >= limit && here > 0) {
+            const u64 here = c0 + i == z ? zall : t[i] * w[i];
+            if (mb < limit && mb + here >= limit) {
               S.r_bin = c0 + i;
-              S.r_above = w[i] > 0 ? (u64)fmax(1.0, ceil((limit - (double)mb) / (double)w[i])) : 0;
+              S.r_above = w[i] > 0 ? (limit - mb + w[i] - 1) / w[i] : 0;
             }
             mb += here;
           }
           __syncthreads();
-          if (S.r_bin < ecode || S.r_above < ties) ecode = S.r_bin, ties = S.r_above;
+          if ((int)S.r_bin < erank || S.r_above < ties) erank = S.r_bin, ties = S.r_above;
         }
       }
       // a border among the small ones is left to the search below
-      if (ecode != small) {
+      if (erank != z) {
         __syncthreads();  // `mine` becomes `weight`
-#pragma unroll
-        for (int i = 0; i < PER; ++i)  // 0 for the small ones, behind lcut and from the border on
-          S.weight[c0 + i] = c0 + i < (int)ecode ? floored(w[i]) : 0;
+        for (int i = tid; i < kCodes; i += kNT) S.weight[i] = 0;
         __syncthreads();
-        const u64 wedge = ecode < (uint32_t)codes ? floored(W(logit(ecode))) : 0;
-        const bool some_small = small < ecode;
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+          if (c0 + i < ranks && c0 + i != z && c0 + i < erank)
+            S.weight[at(c0 + i)] = floored(w[i]);
+        const int eslot = erank < ranks ? at(erank) : -2;  // -1 is no slot either
+        u64 wedge = eslot >= 0 ? floored(W(logit(eslot))) : 0;
+        if (eslot >= 0 && tid == 0) S.weight[eslot] = 0;
+        __syncthreads();
+        const bool some_small = z >= 0 && z < erank;
         finish(
             [&](float l) -> u64 {
-              const uint32_t c = code_of(l);
-              if (c >= (uint32_t)codes) return 0;
-              if (c == small) return some_small ? floored(W(l)) : 0;
-              return S.weight[c];
+              const uint32_t c = slot_of(__float_as_uint(l) >> 16);
+              if (c < (uint32_t)kCodes) return S.weight[c];
+              return some_small && small(l) ? floored(W(l)) : 0;
             },
-            [&](float l) { return code_of(l) == ecode; }, ties, wedge);
+            [&](float l) { return (int)slot_of(__float_as_uint(l) >> 16) == eslot; }, ties, wedge);
         return;
       }
     }
@@ -681,7 +726,7 @@ __global__ void __launch_bounds__(kNT, 2) k_sample(const SampleArgs a) {
       for (int e = 0; e < 2; ++e) {
         const u64 bf = before + (e ? w[0] : 0);
         keep[e] = w[e] > 0 && (2 * tid + e == 0 ||
-                               ((!by_p || (double)bf < lim) && (double)w[e] >= floor_p));
+                               ((!by_p || (double)bf < lim) && w[e] >= floor_p));
         kept += keep[e];
       }
       u64 nkept;
@@ -857,25 +902,23 @@ __global__ void __launch_bounds__(kNT, 2) k_sample(const SampleArgs a) {
          edge ? floored(W(logit_of(edge))) : 0ull);
 }
 
-constexpr int kSharedBytes = (int)((sizeof(Shared) + 15) / 16 * 16);
-constexpr int64_t kSliceBytes = 56 << 10;       // of a row in a CTA: two CTAs an SM
-constexpr int64_t kMostSliceBytes = 160 << 10;  // one
+constexpr int64_t kRunBytes = 56 << 10;
 
 template <typename T>
 int launch_sample(const SampleArgs& a, int64_t rows, cudaStream_t st) {
-  const int64_t bytes = a.vocab * (int64_t)sizeof(T) + 32;
-  // CTAs of a row: enough for the row to fit their shared memory, and to give
-  // every SM work when the rows are few, at least 512 ids each
+  // CTAs of a row: one from 148 rows on (a table of weights in each costs more
+  // than it saves), else up to 8 so that every SM has work, 512 ids each or more
   int nc = 1;
-  while (nc < kMaxCtas && (bytes > nc * kSliceBytes || (rows * nc * 2 <= 148 && a.vocab >= nc * 1024)))
-    nc *= 2;
-  const int64_t per = (bytes / 16 + 2 + nc - 1) / nc * 16;
-  const bool cached = per <= kMostSliceBytes;
-  const int smem = kSharedBytes + (cached ? (int)per : 0);
-  auto* k = cached ? k_sample<T, true> : k_sample<T, false>;
-  static SmemLimit limits[2];
-  const int most = cached ? kSharedBytes + (int)kMostSliceBytes : kSharedBytes;
-  if (const int e = limits[cached].raise(reinterpret_cast<const void*>(k), most)) return e;
+  while (nc < kMaxCtas && rows * nc < 148 && a.vocab >= nc * 1024) nc *= 2;
+  // a CTA's run in shared memory if two CTAs still fit an SM
+  const int64_t run = (a.vocab * (int64_t)sizeof(T) / 16 + 2 + nc) / nc * 16;
+  const int cached = run <= kRunBytes;
+  const int smem = (int)((sizeof(Shared) + 15) / 16 * 16 + (cached ? run : 0));
+  auto* k = k_sample<T>;
+  static SmemLimit limit;
+  if (const int e = limit.raise(reinterpret_cast<const void*>(k),
+                                (int)((sizeof(Shared) + 15) / 16 * 16 + kRunBytes)))
+    return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(rows * nc));
   cfg.blockDim = dim3(kNT);
@@ -886,7 +929,7 @@ int launch_sample(const SampleArgs& a, int64_t rows, cudaStream_t st) {
   at.val.clusterDim.x = nc, at.val.clusterDim.y = 1, at.val.clusterDim.z = 1;
   cfg.attrs = &at;
   cfg.numAttrs = 1;
-  return (int)cudaLaunchKernelEx(&cfg, k, a);
+  return (int)cudaLaunchKernelEx(&cfg, k, a, cached);
 }
 
 }  // namespace

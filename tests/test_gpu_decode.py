@@ -423,11 +423,11 @@ def test_sample_wide_rows_and_nuclei(filt):
 
 
 def test_sample_small_and_large_logits():
-    """16-bit rows around zero (values below 2^-7 and the border among them),
+    """16-bit rows around zero (values below 2^-9 and the border among them),
     all negative, far from zero, and wider than the table of values."""
     for V in (300, 20011):
         for scale, shift in ((1e-3, 0.0), (4e-3, 0.0), (0.05, 0.0), (1.0, -9.0), (1.0, 300.0),
-                             (900.0, 0.0), (30.0, 5000.0), (1e-6, 2e-3)):
+                             (900.0, 0.0), (30.0, 5000.0), (1e-6, 2e-3), (10.0, 100.0)):
             g = gen(V)
             logits = (randn(g, 3, V) * scale + shift).to(BF)
             u = torch.rand(3, generator=g, device="cuda")

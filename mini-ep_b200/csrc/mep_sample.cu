@@ -63,7 +63,9 @@ struct Weights {
   double top, c;      // lmax; 256 log2(e) / temperature
   int scale;          // weight 1 is 2^scale
   const double* tab;  // 2^(j / 256)
-  __device__ u64 operator()(float l) const {
+  // a call where a copy at every use would only fill the instruction cache
+  __device__ u64 operator()(float l) const;
+  __device__ __forceinline__ u64 inlined(float l) const {
     if (l == lmax) return 1ull << scale;
     if (!(l >= lcut)) return 0;
     constexpr double kMagic = 6755399441055744.0;        // 1.5 * 2^52: rounds to an integer
@@ -83,6 +85,14 @@ struct Weights {
     return (u64)__double_as_longlong(y + 4503599627370496.0) & 0xfffffffffffffull;
   }
 };
+
+__device__ __noinline__ u64 weight_call(float l, float lmax, float lcut, double top, double c,
+                                        int scale, const double* tab) {
+  return Weights{lmax, lcut, top, c, scale, tab}.inlined(l);
+}
+__device__ __forceinline__ u64 Weights::operator()(float l) const {
+  return weight_call(l, lmax, lcut, top, c, scale, tab);
+}
 
 constexpr int kNT = 512;        // threads of a CTA
 constexpr int kNW = kNT / 32;
@@ -413,14 +423,9 @@ __global__ void __launch_bounds__(kNT, 2) k_sample(const SampleArgs a, int cache
     return w < floor_p && w < 1ull << W.scale ? 0ull : w;
   };
   // ---- the draw: weigh(l) is a token's kept weight; of the tokens with
-  // on_edge(l) the first `ties` ids weigh `wedge` each
-  auto finish = [&](auto weigh, auto on_edge, u64 ties, u64 wedge) {
-    u64 mass = 0;
-    uint32_t n_edge = 0;
-    if (wedge)
-      each([&](float l, int) { mass += weigh(l), n_edge += on_edge(l); });
-    else
-      each([&](float l, int) { mass += weigh(l); });
+  // on_edge(l) the first `ties` ids weigh `wedge` each; mass and n_edge are
+  // this thread's sums of them
+  auto finish = [&](u64 mass, uint32_t n_edge, auto weigh, auto on_edge, u64 ties, u64 wedge) {
     mass = warp_sum(mass);
     n_edge = __reduce_add_sync(0xffffffffu, n_edge);
     if (lane < nc) {
@@ -508,6 +513,24 @@ __global__ void __launch_bounds__(kNT, 2) k_sample(const SampleArgs a, int cache
         const uint32_t c = (bits & 0x7fff) - kSmall;
         return c < (uint32_t)kHalf ? c + (bits >> 15) * kHalf : ~0u;
       };
+      // f(slot) for a piece's values; the others are the result's bits
+      auto slots = [&](const uint4& v, auto f) {
+        const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+        uint32_t rest = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint32_t c = slot_of(i & 1 ? u[i >> 1] >> 16 : u[i >> 1] & 0xffff);
+          if (c < (uint32_t)kCodes)
+            f(c);
+          else
+            rest |= 1u << i;
+        }
+        return rest;
+      };
+      auto value = [&](const uint4& v, int i) {
+        const uint32_t u = i < 2 ? v.x : i < 4 ? v.y : i < 6 ? v.z : v.w;
+        return __uint_as_float(i & 1 ? u & 0xffff0000u : u << 16);
+      };
       auto slot_at = [&](int rank) {  // n_pos (if not negative): the small ones' rank
         return rank < n_pos ? n_pos - 1 - rank : kHalf + rank - n_pos - 1;
       };
@@ -520,16 +543,10 @@ __global__ void __launch_bounds__(kNT, 2) k_sample(const SampleArgs a, int cache
       uint32_t zcnt = 0;
       if (by_k || by_p) {
         each_piece([&](const uint4& v, int) {
-          const uint32_t u[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const uint32_t b = i & 1 ? u[i >> 1] >> 16 : u[i >> 1] & 0xffff, c = slot_of(b);
-            if (c < (uint32_t)kCodes) {
-              atomicAdd(&S.mine[c], 1u);
-            } else {
-              const float l = __uint_as_float(b << 16);
-              if (small(l)) zall += W(l), ++zcnt;
-            }
+          uint32_t rest = slots(v, [&](uint32_t c) { atomicAdd(&S.mine[c], 1u); });
+          for (; rest; rest &= rest - 1) {
+            const float l = value(v, __ffs(rest) - 1);
+            if (small(l)) zall += W(l), ++zcnt;
           }
         });
         u64 all, nz;
@@ -579,15 +596,17 @@ __global__ void __launch_bounds__(kNT, 2) k_sample(const SampleArgs a, int cache
         if (by_k) {
           u64 nb = block_scan(n, S.red, all), mb = m0;
           if ((u64)top_k < all) {
+            if (nb < (u64)top_k && nb + n >= (u64)top_k) {  // among this thread's
 #pragma unroll
-            for (int i = 0; i < PER; ++i) {
-              if (nb < (u64)top_k && nb + t[i] >= (u64)top_k) {
-                S.r_bin = c0 + i;
-                S.r_above = (u64)top_k - nb;
-                S.r_mass = mb + S.r_above * w[i];
+              for (int i = 0; i < PER; ++i) {
+                if (nb < (u64)top_k && nb + t[i] >= (u64)top_k) {
+                  S.r_bin = c0 + i;
+                  S.r_above = (u64)top_k - nb;
+                  S.r_mass = mb + S.r_above * w[i];
+                }
+                nb += t[i];
+                mb += c0 + i == z ? zall : t[i] * w[i];
               }
-              nb += t[i];
-              mb += c0 + i == z ? zall : t[i] * w[i];
             }
             __syncthreads();
             erank = S.r_bin, ties = S.r_above, mass_p = S.r_mass;
@@ -598,15 +617,15 @@ __global__ void __launch_bounds__(kNT, 2) k_sample(const SampleArgs a, int cache
           const u64 limit = ceiling((double)top_p * (double)mass_p);
           if (tid == 0) S.r_bin = 0, S.r_above = 1;  // top_p <= 0: the best token
           __syncthreads();
-          u64 mb = m0;
+          if (m0 < limit && m0 + m >= limit) {
+            u64 mb = m0, left = 0, each_w = 0;
 #pragma unroll
-          for (int i = 0; i < PER; ++i) {
-            const u64 here = c0 + i == z ? zall : t[i] * w[i];
-            if (mb < limit && mb + here >= limit) {
-              S.r_bin = c0 + i;
-              S.r_above = w[i] > 0 ? (limit - mb + w[i] - 1) / w[i] : 0;
+            for (int i = 0; i < PER; ++i) {
+              const u64 here = c0 + i == z ? zall : t[i] * w[i];
+              if (mb < limit && mb + here >= limit) S.r_bin = c0 + i, left = limit - mb, each_w = w[i];
+              mb += here;
             }
-            mb += here;
+            S.r_above = each_w > 0 ? (left + each_w - 1) / each_w : 0;
           }
           __syncthreads();
           if ((int)S.r_bin < erank || S.r_above < ties) erank = S.r_bin, ties = S.r_above;
@@ -626,13 +645,35 @@ __global__ void __launch_bounds__(kNT, 2) k_sample(const SampleArgs a, int cache
         if (eslot >= 0 && tid == 0) S.weight[eslot] = 0;
         __syncthreads();
         const bool some_small = z >= 0 && z < erank;
-        finish(
-            [&](float l) -> u64 {
+        auto weigh = [&](float l) -> u64 {
+          const uint32_t c = slot_of(__float_as_uint(l) >> 16);
+          if (c < (uint32_t)kCodes) return S.weight[c];
+          return some_small && small(l) ? floored(W(l)) : 0;
+        };
+        u64 mass = 0;
+        uint32_t n_edge = 0;
+        // most tokens lie behind the border: one comparison, no table read
+        const float border = eslot >= 0 ? logit(eslot) : -INFINITY;
+        each_piece([&](const uint4& v, int) {
+          uint32_t rest = 0;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float l = value(v, i);
+            if (l > border) {
               const uint32_t c = slot_of(__float_as_uint(l) >> 16);
-              if (c < (uint32_t)kCodes) return S.weight[c];
-              return some_small && small(l) ? floored(W(l)) : 0;
-            },
-            [&](float l) { return (int)slot_of(__float_as_uint(l) >> 16) == eslot; }, ties, wedge);
+              if (c < (uint32_t)kCodes)
+                mass += S.weight[c];
+              else
+                rest |= 1u << i;
+            }
+            n_edge += wedge && l == border;
+          }
+          if (some_small)
+            for (; rest; rest &= rest - 1) mass += weigh(value(v, __ffs(rest) - 1));
+        });
+        finish(mass, n_edge, weigh,
+               [&](float l) { return (int)slot_of(__float_as_uint(l) >> 16) == eslot; }, ties,
+               wedge);
         return;
       }
     }
@@ -656,7 +697,7 @@ __global__ void __launch_bounds__(kNT, 2) k_sample(const SampleArgs a, int cache
       if (l >= W.lcut) {
         const int b = bin_of(l);
         atomicAdd(&S.cnt[b], 1u);
-        if (!by_k) add_mass(b, W(l));
+        if (!by_k) add_mass(b, W.inlined(l));
       }
     });
     join();
@@ -897,7 +938,14 @@ __global__ void __launch_bounds__(kNT, 2) k_sample(const SampleArgs a, int cache
     }
   }
 
-  finish([&](float l) { return key_of(l) > edge ? floored(W(l)) : 0ull; },
+  u64 mass = 0;
+  uint32_t n_edge = 0;
+  each([&](float l, int) {
+    const uint32_t k = key_of(l);
+    if (k > edge) mass += floored(W.inlined(l));
+    n_edge += k == edge;
+  });
+  finish(mass, n_edge, [&](float l) { return key_of(l) > edge ? floored(W(l)) : 0ull; },
          [&](float l) { return key_of(l) == edge; }, ties,
          edge ? floored(W(logit_of(edge))) : 0ull);
 }

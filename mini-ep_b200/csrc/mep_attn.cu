@@ -52,6 +52,12 @@ __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], const void* p) {
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                : "r"(smem_u32(p)));
 }
+// an 8 x 8 block of 16-bit values, transposed
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
 __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
                                          uint32_t b1) {
   asm volatile(
@@ -143,14 +149,21 @@ struct PartArgs {
   float2* part_ml;       // [extra + splits][out_rows]: maximum (base 2), sum
 };
 
+// How a CTA's four warps share its work.
+enum Mode { kByRows = 0, kByKeys = 1, kFewRows = 2 };
+
 // The kernel for one (element types, padded head width, warp layout).
-// KS (key split): the four warps share 16 rows and take a quarter of each tile
-// of keys each, for matrices of few rows, where the keys' bytes bound it: a
+// kByRows: each warp has 16 of 64 rows and every key of the tile. kByKeys: the
+// four warps share 16 rows and take a quarter of each tile of keys each, for matrices of few rows, where the keys' bytes bound it: a
 // warp streams its own keys and meets the others only at the end; a cluster of
 // up to 8 CTAs, one a split, then joins its sums over distributed shared
-// memory. Otherwise each warp has 16 of 64 rows and every key of the tile.
-template <typename QT, typename CT, int DP, bool KS>
+// memory. kFewRows (16-bit queries): the same for up to 8 rows, with the keys
+// along the products' 16 and the rows along their 8, S^T = K Q^T and
+// O^T = V^T P^T: half the products and half the exponentials of rows that are
+// not there.
+template <typename QT, typename CT, int DP, int MODE>
 struct Tile {
+  static constexpr bool KS = MODE != kByRows;
   static constexpr int kElt = sizeof(CT);
   static constexpr int kRow = DP * kElt;  // bytes of a staged row
   // keys a warp works on at a time: 8 KB of keys and values a warp when the
@@ -158,7 +171,7 @@ struct Tile {
   static constexpr int kN = KS ? (kRow >= 256 ? 16 : 32) : (kRow >= 512 ? 32 : 64);
   static constexpr int kKeys = KS ? 4 * kN : kN;  // keys of a CTA's tile
   static constexpr int kStages = KS ? 3 : 2;
-  static constexpr int kRows = KS ? 16 : 64;
+  static constexpr int kRows = MODE == kFewRows ? 8 : KS ? 16 : 64;
   static constexpr bool kScaled = sizeof(CT) == 1;
   static constexpr int kScaleBytes = kScaled ? kKeys * 8 : 0;
   static constexpr int kStageBytes = 2 * kKeys * kRow + kScaleBytes;
@@ -197,10 +210,12 @@ __device__ __forceinline__ void add_part(float4& x, float2 ml, float base, float
   }
 }
 
-template <typename QT, typename CT, int DP, bool KS, bool PREFIX>
+template <typename QT, typename CT, int DP, int MODE, bool PREFIX>
 __global__ void __launch_bounds__(kThreads) k_attn_part(const PartArgs p) {
-  using X = Tile<QT, CT, DP, KS>;
-  constexpr int N = X::kN, NT = N / 8, OT = DP / 8;
+  using X = Tile<QT, CT, DP, MODE>;
+  constexpr bool KS = X::KS, kFew = MODE == kFewRows;
+  // accumulator tiles of the scores (8 keys, or 16) and of the values (8, or 16)
+  constexpr int N = X::kN, NT = N / (kFew ? 16 : 8), OT = DP / (kFew ? 16 : 8);
   constexpr bool kF32 = X::kF32, kScaled = X::kScaled;
   extern __shared__ __align__(128) unsigned char smem[];
   const AttnArgs& a = p.a;
@@ -329,41 +344,44 @@ __global__ void __launch_bounds__(kThreads) k_attn_part(const PartArgs p) {
     cp_commit();
   }
 
-  // ---- queries of this thread: rows row[0] and row[1] = row[0] + 8
+  // ---- this thread's rows: row[0] and row[1] = row[0] + 8, or neighbours
   const int wrow = KS ? 0 : warp * 16;
   int row[2];
   int64_t tq[2];  // last column that the row sees
   float rscale[2];
-  uint32_t qf[kF32 ? 1 : DP / 16][4];
+  uint32_t qf[kF32 ? 1 : DP / 16][kFew ? 2 : 4];
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
-    row[u] = r0 + wrow + g + 8 * u;
+    row[u] = kFew ? r0 + 2 * t4 + u : r0 + wrow + g + 8 * u;
     tq[u] = col + (row[u] < rN ? row[u] / p.group : 0);
     rscale[u] = a.scale * turn * kLog2e;
   }
   if constexpr (!kF32) {
     const uint32_t flip = turn < 0.f ? 0x80008000u : 0u;
+    // rows whose queries this thread holds: its own, or the one of its group
+    constexpr int QR = kFew ? 1 : 2;
     const __nv_bfloat16* qp[2] = {nullptr, nullptr};
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
-      if (row[u] < rN) qp[u] = query_ptr(row[u]);
+    for (int u = 0; u < QR; ++u) {
+      const int r = kFew ? r0 + g : row[u];
+      if (r < rN) qp[u] = query_ptr(r);
+    }
     if constexpr (!kScaled) {
 #pragma unroll
       for (int k = 0; k < DP / 16; ++k)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int d = k * 16 + t4 * 2 + (i >> 1) * 8;
-          qf[k][i] = qp[i & 1] && d < D
-                         ? *reinterpret_cast<const uint32_t*>(qp[i & 1] + d) ^ flip : 0u;
+        for (int i = 0; i < 2 * QR; ++i) {
+          const int u = kFew ? 0 : i & 1, d = k * 16 + t4 * 2 + (kFew ? i : i >> 1) * 8;
+          qf[k][i] = qp[u] && d < D ? *reinterpret_cast<const uint32_t*>(qp[u] + d) ^ flip : 0u;
         }
     } else {
       // Codes are exact in fp16, so the products are fp16 ones. A query row is
       // scaled by a power of two to a largest magnitude in [1, 2): its bf16
       // values stay exact down to 2^-14 of it, and below that are off by 2^-25
       // of it at most.
-      uint4 raw[2][DP / 32];
+      uint4 raw[QR][DP / 32];
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < QR; ++u)
 #pragma unroll
         for (int i = 0; i < DP / 32; ++i) {
           const int d = (i / 2) * 64 + t4 * 16 + (i % 2) * 8;
@@ -371,7 +389,7 @@ __global__ void __launch_bounds__(kThreads) k_attn_part(const PartArgs p) {
                                      : make_uint4(0, 0, 0, 0);
         }
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
+      for (int u = 0; u < QR; ++u) {
         float qv[DP / 4], m = 0.f;
 #pragma unroll
         for (int i = 0; i < DP / 32; ++i) {
@@ -388,12 +406,18 @@ __global__ void __launch_bounds__(kThreads) k_attn_part(const PartArgs p) {
         const int ex = (int)(__float_as_uint(m) >> 23) - 127;
         const int e = m > 0.f && ex < 128 ? min(max(ex, -126), 126) : 0;
         const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-        rscale[u] *= __uint_as_float((uint32_t)(127 + e) << 23);
+        const float up = __uint_as_float((uint32_t)(127 + e) << 23);
+        if (kFew) {
+          rscale[0] *= __shfl_sync(0xffffffffu, up, 8 * t4);
+          rscale[1] *= __shfl_sync(0xffffffffu, up, 8 * t4 + 4);
+        } else {
+          rscale[u] *= up;
+        }
         // k-step k of a 64-wide block takes values 4k..4k+3 of each thread's 16
 #pragma unroll
         for (int k = 0; k < DP / 16; ++k) {
           qf[k][u] = pack_f16x2(qv[k * 4] * down, qv[k * 4 + 1] * down);
-          qf[k][u + 2] = pack_f16x2(qv[k * 4 + 2] * down, qv[k * 4 + 3] * down);
+          qf[k][u + QR] = pack_f16x2(qv[k * 4 + 2] * down, qv[k * 4 + 3] * down);
         }
       }
     }
@@ -428,7 +452,34 @@ __global__ void __launch_bounds__(kThreads) k_attn_part(const PartArgs p) {
     for (int i = 0; i < NT; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
-    if constexpr (!kF32 && !kScaled) {
+    if constexpr (kFew) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        if constexpr (!kScaled) {
+          const int r = kr0 + i * 16 + (lane & 15);
+#pragma unroll
+          for (int k = 0; k < DP / 16; ++k) {
+            uint32_t ka[4];
+            ldsm4(ka, ks + r * X::kRow + X::k_chunk(r, k * 2 + (lane >> 4)) * 16);
+            mma_bf16(s[i], ka, qf[k][0], qf[k][1]);
+          }
+        } else {
+          const int r = kr0 + i * 16 + g;
+#pragma unroll
+          for (int w = 0; w < DP / 64; ++w) {
+            const uint4 v0 = *reinterpret_cast<const uint4*>(ks + r * X::kRow + X::k_chunk(r, w * 4 + t4) * 16);
+            const uint4 v1 = *reinterpret_cast<const uint4*>(ks + (r + 8) * X::kRow + X::k_chunk(r + 8, w * 4 + t4) * 16);
+            const uint32_t a0[4] = {v0.x, v0.y, v0.z, v0.w}, a1[4] = {v1.x, v1.y, v1.z, v1.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const uint32_t ka[4] = {e4m3x2_f16x2(a0[k] & 0xffff), e4m3x2_f16x2(a1[k] & 0xffff),
+                                      e4m3x2_f16x2(a0[k] >> 16), e4m3x2_f16x2(a1[k] >> 16)};
+              mma_f16(s[i], ka, qf[w * 4 + k][0], qf[w * 4 + k][1]);
+            }
+          }
+        }
+      }
+    } else if constexpr (!kF32 && !kScaled) {
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
         const int r = kr0 + i * 8 + (lane & 7);
@@ -502,33 +553,49 @@ __global__ void __launch_bounds__(kThreads) k_attn_part(const PartArgs p) {
       }
     }
 
-    // ---- scale, mask, running maximum
+    // ---- scale, mask, running maximum. Of accumulator element j of tile i:
+    // its row (u: the thread's first or second), its key
+    auto row_of = [](int j) { return kFew ? j & 1 : j >> 1; };
+    auto key_of = [&](int i, int j) {
+      return kFew ? i * 16 + g + 8 * (j >> 1) : i * 8 + t4 * 2 + (j & 1);
+    };
+    // over the lanes that hold other keys of the same rows
+    auto all_max = [](float x) {
+      if constexpr (kFew) {
+#pragma unroll
+        for (int w = 4; w < 32; w <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, w));
+        return x;
+      } else {
+        return quad_max(x);
+      }
+    };
     const bool edge = j0 + N > span.n || (!PREFIX && tokens > 1);
     float mx[2] = {m[0], m[1]};
-    float vmax = vref;
+    float vmax = vref, vv[kScaled ? NT : 1][2];
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
       if (kScaled) {
-        const float2 kk = *reinterpret_cast<const float2*>(sc + kr0 + i * 8 + t4 * 2);
-        const float2 vv = *reinterpret_cast<const float2*>(sc + X::kKeys + kr0 + i * 8 + t4 * 2);
-        s[i][0] *= kk.x, s[i][1] *= kk.y, s[i][2] *= kk.x, s[i][3] *= kk.y;
-        vmax = fmaxf(vmax, fmaxf(vv.x, vv.y));
+        const int k0 = kr0 + key_of(i, 0), k1 = kr0 + key_of(i, kFew ? 2 : 1);
+        const float f0 = sc[k0], f1 = sc[k1];
+        vv[i][0] = sc[X::kKeys + k0], vv[i][1] = sc[X::kKeys + k1];
+        s[i][0] *= f0, s[i][1] *= kFew ? f0 : f1, s[i][2] *= kFew ? f1 : f0, s[i][3] *= f1;
+        vmax = fmaxf(vmax, fmaxf(vv[i][0], vv[i][1]));
       }
       if (edge) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int jj = j0 + i * 8 + t4 * 2 + (j & 1);
-          const bool see = jj < span.n && (PREFIX || span.column(jj) <= tq[j >> 1]);
+          const int jj = j0 + key_of(i, j);
+          const bool see = jj < span.n && (PREFIX || span.column(jj) <= tq[row_of(j)]);
           if (!see) s[i][j] = -INFINITY;
         }
       }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) mx[j >> 1] = fmaxf(mx[j >> 1], s[i][j]);
+      for (int j = 0; j < 4; ++j) mx[row_of(j)] = fmaxf(mx[row_of(j)], s[i][j]);
     }
     float keep[2], base[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      mx[u] = quad_max(mx[u]);
+      mx[u] = all_max(mx[u]);
       base[u] = mx[u] == -INFINITY ? 0.f : mx[u] * rscale[u];
       keep[u] = m[u] == -INFINITY ? 0.f : ex2((m[u] - mx[u]) * rscale[u]);
       m[u] = mx[u];
@@ -536,7 +603,7 @@ __global__ void __launch_bounds__(kThreads) k_attn_part(const PartArgs p) {
     }
     float vinv = 1.f;
     if (kScaled) {
-      vmax = quad_max(vmax);
+      vmax = all_max(vmax);
       vinv = vmax > 1e-37f ? 1.f / vmax : 0.f;
       const float r = vref * vinv;
       keep[0] *= r, keep[1] *= r;
@@ -546,27 +613,60 @@ __global__ void __launch_bounds__(kThreads) k_attn_part(const PartArgs p) {
     for (int i = 0; i < NT; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        s[i][j] = ex2(fmaf(s[i][j], rscale[j >> 1], -base[j >> 1]));
-        l[j >> 1] += s[i][j];
+        s[i][j] = ex2(fmaf(s[i][j], rscale[row_of(j)], -base[row_of(j)]));
+        l[row_of(j)] += s[i][j];
       }
     // most tiles change neither maximum nor reference: nothing to rescale
     if (!kF32 && __any_sync(0xffffffffu, keep[0] != 1.f || keep[1] != 1.f)) {
 #pragma unroll
       for (int i = 0; i < OT; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) o[i][j] *= keep[j >> 1];
+        for (int j = 0; j < 4; ++j) o[i][j] *= keep[row_of(j)];
     }
     if (kScaled) {
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
-        const float2 vv = *reinterpret_cast<const float2*>(sc + X::kKeys + kr0 + i * 8 + t4 * 2);
-        const float v0 = vv.x * vinv, v1 = vv.y * vinv;
-        s[i][0] *= v0, s[i][1] *= v1, s[i][2] *= v0, s[i][3] *= v1;
+        const float v0 = vv[i][0] * vinv, v1 = vv[i][1] * vinv;
+        s[i][0] *= v0, s[i][1] *= kFew ? v0 : v1, s[i][2] *= kFew ? v1 : v0, s[i][3] *= v1;
       }
     }
 
     // ---- o += p v
-    if constexpr (!kF32 && !kScaled) {
+    if constexpr (kFew) {
+#pragma unroll
+      for (int k = 0; k < NT; ++k) {
+        // the 8 x 8 blocks (keys, rows) turned into (rows, keys)
+        uint32_t p0 = kScaled ? pack_f16x2(s[k][0], s[k][1]) : pack_bf16(s[k][0], s[k][1]);
+        uint32_t p1 = kScaled ? pack_f16x2(s[k][2], s[k][3]) : pack_bf16(s[k][2], s[k][3]);
+        p0 = transposed(p0), p1 = transposed(p1);
+        if constexpr (!kScaled) {
+          const int r = kr0 + k * 16 + (lane & 7) + (lane >> 4) * 8;
+#pragma unroll
+          for (int n = 0; n < OT; ++n) {
+            uint32_t va[4];
+            ldsm4t(va, vs + r * X::kRow + X::v_chunk(r, n * 2 + (lane >> 3 & 1)) * 16);
+            mma_bf16(o[n], va, p0, p1);
+          }
+        } else {
+          // of the byte pair of a key, the first is value 16 n + 2 g, the
+          // second 16 n + 2 g + 1: the tile's rows g and g + 8
+          const int r = kr0 + k * 16 + (lane & 15);
+#pragma unroll
+          for (int n = 0; n < OT; n += 2) {
+            uint32_t b[4];
+            ldsm4t(b, vs + r * X::kRow + X::v_chunk(r, n + (lane >> 4)) * 16);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const uint32_t c0 = __byte_perm(b[2 * e], 0, 0x3120);
+              const uint32_t c1 = __byte_perm(b[2 * e + 1], 0, 0x3120);
+              const uint32_t va[4] = {e4m3x2_f16x2(c0 & 0xffff), e4m3x2_f16x2(c0 >> 16),
+                                      e4m3x2_f16x2(c1 & 0xffff), e4m3x2_f16x2(c1 >> 16)};
+              mma_f16(o[n + e], va, p0, p1);
+            }
+          }
+        }
+      }
+    } else if constexpr (!kF32 && !kScaled) {
 #pragma unroll
       for (int k = 0; k < N / 16; ++k) {
         const uint32_t pa[4] = {pack_bf16(s[2 * k][0], s[2 * k][1]),
@@ -659,7 +759,14 @@ __global__ void __launch_bounds__(kThreads) k_attn_part(const PartArgs p) {
   }
   cp_wait<0>();
 #pragma unroll
-  for (int u = 0; u < 2; ++u) l[u] = quad_sum(l[u]);
+  for (int u = 0; u < 2; ++u) {
+    if (kFew) {
+#pragma unroll
+      for (int w = 4; w < 32; w <<= 1) l[u] += __shfl_xor_sync(0xffffffffu, l[u], w);
+    } else {
+      l[u] = quad_sum(l[u]);
+    }
+  }
   if (kScaled)
 #pragma unroll
     for (int i = 0; i < OT; ++i)
@@ -672,6 +779,7 @@ __global__ void __launch_bounds__(kThreads) k_attn_part(const PartArgs p) {
 
   // value index of accumulator element (tile n, j)
   auto value_of = [&](int n, int j) {
+    if (kFew) return kScaled ? n * 16 + 2 * g + (j >> 1) : n * 16 + g + 8 * (j >> 1);
     return kScaled ? (n >> 1) * 16 + (t4 * 2 + (j & 1)) * 2 + (n & 1) : n * 8 + t4 * 2 + (j & 1);
   };
   const int nrow = rN - r0;
@@ -686,10 +794,11 @@ __global__ void __launch_bounds__(kThreads) k_attn_part(const PartArgs p) {
     for (int i = 0; i < OT; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        jo[(warp * 16 + g + 8 * (j >> 1)) * DP + value_of(i, j)] = o[i][j];
-    if (t4 == 0) {
-      jm[warp * 16 + g] = make_float2(m[0], l[0]);
-      jm[warp * 16 + g + 8] = make_float2(m[1], l[1]);
+        jo[(warp * 16 + (kFew ? 2 * t4 + (j & 1) : g + 8 * (j >> 1))) * DP + value_of(i, j)] =
+            o[i][j];
+    if (kFew ? g == 0 : t4 == 0) {
+      jm[warp * 16 + (kFew ? 2 * t4 : g)] = make_float2(m[0], l[0]);
+      jm[warp * 16 + (kFew ? 2 * t4 + 1 : g + 8)] = make_float2(m[1], l[1]);
     }
     __syncthreads();
     const int quads = D >> 2;
@@ -749,7 +858,7 @@ __global__ void __launch_bounds__(kThreads) k_attn_part(const PartArgs p) {
       store4(static_cast<QT*>(a.out) + orow * D + d, x.x * inv, x.y * inv, x.z * inv, x.w * inv);
     }
     if (p.splits > 1) cluster.sync();  // nobody leaves while its sums are read
-  } else if (!p.joined) {
+  } else if (!p.joined) {  // kByRows
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       if (row[u] >= rN) continue;
@@ -856,7 +965,8 @@ __global__ void __launch_bounds__(128) k_attn_join(const float* part_o, const fl
 // How a call is cut: splits of the own columns and of the prefix, and whether
 // the own part's clusters join everything (else k_attn_join does).
 struct Plan {
-  bool own_ks, prefix_ks, joined, prefix_tc;
+  Mode own, prefix;
+  bool joined, prefix_tc;
   int own_splits, prefix_splits;
   PrefixTcPlan tc;
   int64_t out_rows, bytes;
@@ -873,6 +983,11 @@ int splits_for(int64_t keys, int64_t ctas) {
   return (int)(want < most ? want : most);
 }
 
+Mode mode_for(int dtype, int64_t rows) {
+  return rows <= 8 && dtype == MEP_BF16 ? kFewRows : rows <= 16 ? kByKeys : kByRows;
+}
+int rows_of(Mode m) { return m == kFewRows ? 8 : m == kByKeys ? 16 : 64; }
+
 constexpr int64_t kTcRows = 128;  // rows of a key/value head from which the prefix is tcgen05's
 
 Plan plan_for(int dtype, int64_t batch, int64_t tokens, int q_heads, int kv_heads, int head_dim,
@@ -881,9 +996,9 @@ Plan plan_for(int dtype, int64_t batch, int64_t tokens, int q_heads, int kv_head
   const int group = q_heads / kv_heads;
   const int64_t keys = col < 0 ? capacity : col + tokens;
   const int64_t own_rows = tokens * group, pre_rows = batch * own_rows;
-  p.own_ks = own_rows <= 16;
-  p.prefix_ks = pre_rows <= 16;
-  const int ot = p.own_ks ? 16 : 64, pt = p.prefix_ks ? 16 : 64;
+  p.own = mode_for(dtype, own_rows);
+  p.prefix = mode_for(dtype, pre_rows);
+  const int ot = rows_of(p.own), pt = rows_of(p.prefix);
   p.own_splits = splits_for(keys, batch * kv_heads * ((own_rows + ot - 1) / ot));
   p.prefix_splits =
       prefix_cols > 0 ? splits_for(prefix_cols, kv_heads * ((pre_rows + pt - 1) / pt)) : 0;
@@ -893,19 +1008,19 @@ Plan plan_for(int dtype, int64_t batch, int64_t tokens, int q_heads, int kv_head
     p.prefix_splits = p.tc.slots;
   }
   // a split or two more than a cluster holds costs less than another launch
-  if (p.own_ks && p.own_splits <= 2 * kMaxCluster && p.own_splits > kMaxCluster)
+  if (p.own != kByRows && p.own_splits <= 2 * kMaxCluster && p.own_splits > kMaxCluster)
     p.own_splits = kMaxCluster;
-  p.joined = p.own_ks ? p.own_splits <= kMaxCluster : p.own_splits == 1;
+  p.joined = p.own != kByRows ? p.own_splits <= kMaxCluster : p.own_splits == 1;
   p.out_rows = batch * tokens * q_heads;
   const int parts = p.prefix_splits + (p.joined ? 0 : p.own_splits);
   p.bytes = parts * p.out_rows * (head_dim * 4 + 8);
   return p;
 }
 
-template <typename QT, typename CT, int DP, bool KS, bool PREFIX>
+template <typename QT, typename CT, int DP, int MODE, bool PREFIX>
 int run_part(const PartArgs& p, int64_t mats, cudaStream_t st) {
-  using X = Tile<QT, CT, DP, KS>;
-  auto* k = k_attn_part<QT, CT, DP, KS, PREFIX>;
+  using X = Tile<QT, CT, DP, MODE>;
+  auto* k = k_attn_part<QT, CT, DP, MODE, PREFIX>;
   static SmemLimit limit;
   if (const int e = limit.raise(reinterpret_cast<const void*>(k), X::kSmem)) return e;
   cudaLaunchConfig_t cfg{};
@@ -915,16 +1030,24 @@ int run_part(const PartArgs& p, int64_t mats, cudaStream_t st) {
   cfg.stream = st;
   cudaLaunchAttribute at{};
   at.id = cudaLaunchAttributeClusterDimension;
-  at.val.clusterDim.x = KS && p.joined ? p.splits : 1, at.val.clusterDim.y = 1,
+  at.val.clusterDim.x = X::KS && p.joined ? p.splits : 1, at.val.clusterDim.y = 1,
   at.val.clusterDim.z = 1;
   cfg.attrs = &at;
   cfg.numAttrs = 1;
   return (int)cudaLaunchKernelEx(&cfg, k, p);
 }
-template <typename QT, typename CT, bool KS, bool PREFIX>
+template <typename QT, typename CT, int MODE, bool PREFIX>
 int run_dp(const PartArgs& p, int64_t mats, cudaStream_t st) {
-  return p.a.head_dim <= 64 ? run_part<QT, CT, 64, KS, PREFIX>(p, mats, st)
-                            : run_part<QT, CT, 128, KS, PREFIX>(p, mats, st);
+  return p.a.head_dim <= 64 ? run_part<QT, CT, 64, MODE, PREFIX>(p, mats, st)
+                            : run_part<QT, CT, 128, MODE, PREFIX>(p, mats, st);
+}
+template <typename QT, typename CT, bool PREFIX>
+int run_mode(Mode m, PartArgs& p, int64_t mats, cudaStream_t st) {
+  p.row_tiles = (p.rows + rows_of(m) - 1) / rows_of(m);
+  if constexpr (sizeof(QT) == 2)
+    if (m == kFewRows) return run_dp<QT, CT, kFewRows, PREFIX>(p, mats, st);
+  return m == kByKeys ? run_dp<QT, CT, kByKeys, PREFIX>(p, mats, st)
+                      : run_dp<QT, CT, kByRows, PREFIX>(p, mats, st);
 }
 
 template <typename QT, typename CT>
@@ -938,17 +1061,11 @@ int run_attention(const AttnArgs& a, const Plan& pl, void* workspace, cudaStream
   } else if (pl.prefix_splits) {
     PartArgs x{a, group, (int)(a.batch * a.tokens * group), 0, pl.prefix_splits, 0, 0, pl.out_rows,
                po, pm};
-    x.row_tiles = (x.rows + (pl.prefix_ks ? 15 : 63)) / (pl.prefix_ks ? 16 : 64);
-    const int rc = pl.prefix_ks ? run_dp<QT, QT, true, true>(x, 1, st)
-                                : run_dp<QT, QT, false, true>(x, 1, st);
-    if (rc) return rc;
+    if (const int rc = run_mode<QT, QT, true>(pl.prefix, x, 1, st)) return rc;
   }
   PartArgs p{a, group, (int)(a.tokens * group), 0, pl.own_splits, pl.joined, pl.prefix_splits,
              pl.out_rows, po, pm};
-  p.row_tiles = (p.rows + (pl.own_ks ? 15 : 63)) / (pl.own_ks ? 16 : 64);
-  const int rc = pl.own_ks ? run_dp<QT, CT, true, false>(p, a.batch, st)
-                           : run_dp<QT, CT, false, false>(p, a.batch, st);
-  if (rc) return rc;
+  if (const int rc = run_mode<QT, CT, false>(pl.own, p, a.batch, st)) return rc;
   if (!pl.joined) {
     const int64_t n = pl.out_rows * (a.head_dim / 4);
     k_attn_join<QT><<<(unsigned)((n + 127) / 128), 128, 0, st>>>(po, pm, parts, pl.out_rows,

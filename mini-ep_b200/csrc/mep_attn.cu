@@ -211,7 +211,8 @@ __device__ __forceinline__ void add_part(float4& x, float2 ml, float base, float
 }
 
 template <typename QT, typename CT, int DP, int MODE, bool PREFIX>
-__global__ void __launch_bounds__(kThreads) k_attn_part(const PartArgs p) {
+__global__ void __launch_bounds__(kThreads, MODE == kByRows && sizeof(QT) == 2 ? 3 : 1)
+    k_attn_part(const PartArgs p) {
   using X = Tile<QT, CT, DP, MODE>;
   constexpr bool KS = X::KS, kFew = MODE == kFewRows;
   // accumulator tiles of the scores (8 keys, or 16) and of the values (8, or 16)

@@ -97,7 +97,8 @@ __device__ __forceinline__ u64 Weights::operator()(float l) const {
 constexpr int kNT = 512;        // threads of a CTA
 constexpr int kNW = kNT / 32;
 constexpr int kBins = 1024;
-constexpr int kList = 1024;     // candidates the leading CTA can finish alone
+constexpr int kList = 2048;     // candidates the leading CTA can finish alone
+constexpr int kPer = kList / kNT;  // of them a thread
 constexpr int kMaxCtas = 8;     // CTAs of a row
 
 constexpr int kCodes = 4096;    // 16-bit logits told apart by the table
@@ -752,23 +753,24 @@ __global__ void __launch_bounds__(kNT, 2) k_sample(const SampleArgs a, int cache
       while (n2 < (int)n) n2 <<= 1;
       for (int i = (int)n + tid; i < n2; i += kNT) S.item[i] = 0;
       sort_desc(S.item, n2);
-      // two neighbours a thread: their weights, and the mass before them
-      u64 w[2], before, mass;
+      // kPer neighbours a thread: their weights, and the mass before them
+      u64 w[kPer], sum = 0, before, mass;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int i = 2 * tid + e;
+      for (int e = 0; e < kPer; ++e) {
+        const int i = kPer * tid + e;
         w[e] = i < (int)n && !(by_k && i >= top_k) ? W(logit_of((uint32_t)(S.item[i] >> 32))) : 0;
+        sum += w[e];
       }
-      before = block_scan(w[0] + w[1], S.red, mass);
+      before = block_scan(sum, S.red, mass);
       const double lim = by_k ? (double)top_p * (double)mass : limit;
-      bool keep[2];
+      bool keep[kPer];
       u64 kept = 0;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const u64 bf = before + (e ? w[0] : 0);
-        keep[e] = w[e] > 0 && (2 * tid + e == 0 ||
-                               ((!by_p || (double)bf < lim) && w[e] >= floor_p));
+      for (int e = 0; e < kPer; ++e) {
+        keep[e] = w[e] > 0 && (kPer * tid + e == 0 ||
+                               ((!by_p || (double)before < lim) && w[e] >= floor_p));
         kept += keep[e];
+        before += w[e];
       }
       u64 nkept;
       block_scan(kept, S.red2, nkept);  // the kept are the first nkept of the list
@@ -776,24 +778,26 @@ __global__ void __launch_bounds__(kNT, 2) k_sample(const SampleArgs a, int cache
       n2 = 32;
       while (n2 < (int)nkept) n2 <<= 1;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int i = 2 * tid + e;
+      for (int e = 0; e < kPer; ++e) {
+        const int i = kPer * tid + e;
         S.w[i] = w[e];
         if (i < n2) S.item[i] = keep[e] ? S.item[i] << 32 | (uint32_t)i : 0;
       }
       sort_desc(S.item, n2);
+      sum = 0;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int i = 2 * tid + e;
+      for (int e = 0; e < kPer; ++e) {
+        const int i = kPer * tid + e;
         w[e] = i < (int)nkept ? S.w[(uint32_t)S.item[i]] : 0;
+        sum += w[e];
       }
       u64 total;
-      u64 run = block_scan(w[0] + w[1], S.red, total);
+      u64 run = block_scan(sum, S.red, total);
       const u64 target = target_of(total);
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
+      for (int e = 0; e < kPer; ++e) {
         if (run <= target && run + w[e] > target)
-          answer((uint32_t)~(uint32_t)(S.item[2 * tid + e] >> 32), w[e], total);
+          answer((uint32_t)~(uint32_t)(S.item[kPer * tid + e] >> 32), w[e], total);
         run += w[e];
       }
       return;
@@ -806,17 +810,18 @@ __global__ void __launch_bounds__(kNT, 2) k_sample(const SampleArgs a, int cache
         while (n2 < m) n2 <<= 1;
         for (int i = m + tid; i < n2; i += kNT) S.item[i] = 0;
         sort_desc(S.item, n2);
-        u64 v[2], all;
+        u64 v[kPer], sum = 0, all;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int i = 2 * tid + e;
+        for (int e = 0; e < kPer; ++e) {
+          const int i = kPer * tid + e;
           v[e] = i >= m ? 0 : mass ? W(logit_of((uint32_t)(S.item[i] >> 32))) : 1;
+          sum += v[e];
         }
-        u64 run = above0 + block_scan(v[0] + v[1], S.red, all);
+        u64 run = above0 + block_scan(sum, S.red, all);
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
+        for (int e = 0; e < kPer; ++e) {
           // the last token that begins before the border (the first there is, if none does)
-          const int i = 2 * tid + e;
+          const int i = kPer * tid + e;
           const u64 next = run + v[e];
           if (i < m && ((double)run < want || i == 0) && (!((double)next < want) || i == m - 1)) {
             const uint32_t k = (uint32_t)(S.item[i] >> 32);
@@ -950,7 +955,7 @@ __global__ void __launch_bounds__(kNT, 2) k_sample(const SampleArgs a, int cache
          edge ? floored(W(logit_of(edge))) : 0ull);
 }
 
-constexpr int64_t kRunBytes = 56 << 10;
+constexpr int64_t kRunBytes = 52 << 10;
 
 template <typename T>
 int launch_sample(const SampleArgs& a, int64_t rows, cudaStream_t st) {

@@ -110,7 +110,8 @@ struct Shared {
       uint32_t cnt[kBins], lo[kBins], hi[kBins];  // this CTA's histogram
       u64 tmass[kBins];                           // the row's
       uint32_t tcnt[kBins];
-      u64 item[kList], w[kList];
+      alignas(16) u64 item[kList];
+      u64 w[kList];
     };
     struct {
       uint32_t total[kCodes];  // tokens of each code in the row
@@ -207,18 +208,34 @@ __device__ __forceinline__ u64 block_scan(u64 v, u64* buf, u64& total) {
   __syncthreads();
   if (lane_id() == 31) buf[warp_id()] = inc;
   __syncthreads();
-  u64 before = 0;
-  total = 0;
-#pragma unroll
-  for (int i = 0; i < kNW; ++i) {
-    if (i < warp_id()) before += buf[i];
-    total += buf[i];
-  }
-  return before + inc - v;
+  const u64 own = lane_id() < kNW ? buf[lane_id()] : 0;
+  const u64 sums = warp_scan(own);
+  total = __shfl_sync(0xffffffffu, sums, 31);
+  return __shfl_sync(0xffffffffu, sums - own, warp_id()) + inc - v;
 }
 
-// descending bitonic sort of x[0..n), n a power of two
-__device__ void sort_desc(u64* x, int n) {
+// descending sort of x[0..n), n a power of two from 32 on: by counting the
+// larger ones where each thread has one value at most, else bitonic (64
+// barriers, 6 us at 2048)
+__device__ __noinline__ void sort_desc(u64* x, int n) {
+  __syncthreads();
+  if (n <= kNT) {
+    const int i = threadIdx.x;
+    u64 v = 0;
+    int rank = 0;
+    if (i < n) {
+      v = x[i];
+#pragma unroll 4
+      for (int j = 0; j < n; j += 2) {
+        const ulonglong2 y = *reinterpret_cast<const ulonglong2*>(x + j);
+        rank += (y.x > v || (y.x == v && j < i)) + (y.y > v || (y.y == v && j + 1 < i));
+      }
+    }
+    __syncthreads();
+    if (i < n) x[rank] = v;
+    __syncthreads();
+    return;
+  }
   for (int k = 2; k <= n; k <<= 1)
     for (int j = k >> 1; j > 0; j >>= 1) {
       __syncthreads();
@@ -238,8 +255,7 @@ __device__ void sort_desc(u64* x, int n) {
 // Without a filter the weights are summed per warp, and the warp
 // whose share holds the target finds the token. With top_k or top_p a
 // histogram over the logits (counts, or masses) tells which bins can hold kept
-// tokens. When those are at most kList the leading CTA sorts and finishes them
-// alone. Else it sorts the bin of the border, and the kept weights are summed
+// tokens. When those are few the leading CTA sorts and finishes them alone. Else it sorts the bin of the border, and the kept weights are summed
 // per warp as without a filter. A bin too large for that, and a second border
 // behind a wide top_k, are found by histograms over ever narrower key ranges.
 // All sums are of integers: their order is free.
@@ -731,9 +747,10 @@ __global__ void __launch_bounds__(kNT, 2) k_sample(const SampleArgs a, int cache
     __syncthreads();
     const uint32_t n = S.r_cnt, n_bin = S.r_hi;
     const u64 above0 = S.r_above;
-    // all candidates to the leading CTA if it can finish them alone, else the
+    // all candidates to the leading CTA if it finishes them sooner than all
+    // CTAs the row (behind one border; two borders cost much more), else the
     // border's bin alone, if it can sort that
-    const bool whole = n <= kList;
+    const bool whole = n <= (by_k && by_p ? kList : kNT / 2);
     if (whole || n_bin <= kList) {
       Shared* lead = cluster.map_shared_rank(&S, 0);
       const uint32_t from = whole ? 0 : last;

@@ -286,6 +286,32 @@ def test_attention_large_scores_and_signs():
             within(got, out, R.attention_tol(out, spread, size, n, dtype, 64, False))
 
 
+@pytest.mark.parametrize("heads", [(16, 8, 64), (32, 8, 128), (4, 2, 16), (8, 8, 80)], ids=str)
+@pytest.mark.parametrize("scale", [0.1, -0.1])
+def test_attention_prefix_with_growing_scores(heads, scale):
+    """A large batch behind a prefix whose later keys weigh more and more (each
+    step of keys raises the maximum far beyond the last), or less and less."""
+    Hq, Hk, D = heads
+    for B, P, up in ((160, 700, True), (160, 700, False), (300, 65, True)):
+        g = gen(B + P)
+        q = randn(g, B, 1, Hq, D, dtype=BF).abs()
+        grow = torch.linspace(0.0, 40.0, P, device="cuda")
+        kp = randn(g, 1, Hk, P, D) * 0.3 + (grow if up else grow.flip(0))[:, None] * 8 / D
+        prefix = SharedPrefix(kp.to(BF), randn(g, 1, Hk, P, D, dtype=BF))
+        cache = KVCache(randn(g, 1, B, Hk, 4, D, dtype=BF), randn(g, 1, B, Hk, 4, D, dtype=BF))
+        got = cache_attention(q, cache, 0, 2, scale, prefix=prefix)
+        keep = R.visible(1, 4, 2, None, 0, B, "cuda")
+        out, spread, size, n = R.attention(q, cache.k[0], cache.v[0], keep, scale, prefix.k[0],
+                                           prefix.v[0])
+        within(got, out, R.attention_tol(out, spread, size, n, BF, D, False))
+
+
+def test_attention_prefix_far_larger_than_a_run():
+    """Key tiles dealt over all SMs, tiles cut between them, tails of a tile."""
+    for heads, B, P in (((2, 1, 64), 64, 20001), ((16, 8, 64), 1100, 333), ((8, 1, 128), 33, 4097)):
+        attend_case(11, heads, (B, 1, 5, 2, 0), BF, True, P)
+
+
 @pytest.mark.parametrize("quant", [False, True], ids=["bf16", "e4m3"])
 @pytest.mark.parametrize("P", [0, 300])
 def test_attention_replayed_with_a_device_column(P, quant):

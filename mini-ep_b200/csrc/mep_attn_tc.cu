@@ -19,6 +19,7 @@
 // equal runs, so a tile's keys may be cut between CTAs. A run's result is a
 // partial one (fp32 sums, maximum in base 2) in the tile's next slot.
 #include <cstdint>
+#include <cudaTypedefs.h>
 #include <cuda_bf16.h>
 
 #include "mep_attn.cuh"
@@ -26,11 +27,33 @@
 #include "mep_tc.cuh"
 
 namespace mep {
-int encode_bf16_3d(CUtensorMap* m, const void* base, const uint64_t (&dims)[3],
-                   const uint32_t (&box)[3]);  // mep_ffn.cu
 namespace {
 namespace px {
 using namespace ::mep::tc;
+
+// the driver's cuTensorMapEncodeTiled, looked up once (no device state)
+PFN_cuTensorMapEncodeTiled_v12000 encoder() {
+  static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    const cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q);
+    return e == cudaSuccess && q == cudaDriverEntryPointSuccess
+               ? reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f) : nullptr;
+  }();
+  return fn;
+}
+// bf16 (z, y, x) with 128-byte swizzle, zeros outside; 0 ok
+int encode_3d(CUtensorMap* m, const void* base, const cuuint64_t (&dims)[3],
+              const cuuint32_t (&box)[3]) {
+  if (!encoder()) return -1;
+  const cuuint64_t strides[2] = {dims[0] * 2, dims[0] * dims[1] * 2};
+  const cuuint32_t es[3] = {1, 1, 1};
+  const CUresult r = encoder()(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base),
+                               dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : -100 - (int)r;
+}
 
 constexpr int kRows = 128;   // rows of a half
 constexpr int kKeys = 128;   // keys of a tile
@@ -525,10 +548,11 @@ template <int DP>
 int launch(const Args& p, int ctas, cudaStream_t st) {
   const AttnArgs& a = p.a;
   CUtensorMap tk, tv;
-  const uint64_t dims[3] = {(uint64_t)a.head_dim, (uint64_t)a.prefix_cols, (uint64_t)a.kv_heads};
-  const uint32_t box[3] = {64, kKeys, 1};
-  if (int rc = encode_bf16_3d(&tk, a.kp, dims, box)) return rc;
-  if (int rc = encode_bf16_3d(&tv, a.vp, dims, box)) return rc;
+  const cuuint64_t dims[3] = {(cuuint64_t)a.head_dim, (cuuint64_t)a.prefix_cols,
+                              (cuuint64_t)a.kv_heads};
+  const cuuint32_t box[3] = {64, kKeys, 1};
+  if (const int rc = encode_3d(&tk, a.kp, dims, box)) return rc;
+  if (const int rc = encode_3d(&tv, a.vp, dims, box)) return rc;
   static SmemLimit limit;
   if (const int e = limit.raise(reinterpret_cast<const void*>(k_attn_prefix_tc<DP>), Cfg<DP>::SMEM))
     return e;

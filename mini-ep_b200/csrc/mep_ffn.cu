@@ -697,18 +697,6 @@ bool tc_shape_ok(int hidden, int inter) {
   return hidden % ffn::BN == 0 && inter % 128 == 0;
 }
 
-int encode_bf16_3d(CUtensorMap* m, const void* base, const uint64_t (&dims)[3],
-                   const uint32_t (&box)[3]) {
-  if (int rc = tc_init()) return rc;
-  const cuuint64_t d[3] = {dims[0], dims[1], dims[2]};
-  const cuuint64_t strides[2] = {dims[0] * 2, dims[0] * dims[1] * 2};
-  const cuuint32_t es[3] = {1, 1, 1};
-  const CUresult r = ffn::g_encode(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base),
-                                  d, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? 0 : -100 - (int)r;
-}
 int tc_init() {
   if (ffn::g_encode) return 0;
   void* fn = nullptr;

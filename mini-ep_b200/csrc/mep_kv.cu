@@ -267,31 +267,33 @@ void launch_store(const StoreArgs& a, int table_f32, cudaStream_t st) {
 // columns [start, start + n) of a quantised layer, code * scale rounded once:
 // 16 codes a thread (one 16-byte load), K and V of a head (blockIdx.y, z)
 template <typename T>
-__global__ void __launch_bounds__(256) k_kv_read(CacheView c, int D, int64_t start, int64_t n,
-                                                 T* k_out, T* v_out) {
+__global__ void __launch_bounds__(256) k_kv_read(CacheView c, int64_t heads, int D,
+                                                 int64_t start, int64_t n, T* k_out, T* v_out) {
   const unsigned per_row = (unsigned)D >> 4;
-  const unsigned bh = blockIdx.z, kv = blockIdx.y;
-  const uint8_t* codes = static_cast<const uint8_t*>(kv ? c.v : c.k);
-  const float* scales = (kv ? c.vs : c.ks) + bh * c.capacity + start;
-  codes += (bh * c.capacity + start) * D;
-  T* out = (kv ? v_out : k_out) + bh * n * D;
+  const unsigned kv = blockIdx.y;
   const unsigned pieces = (unsigned)n * per_row;
-  for (unsigned i = blockIdx.x * blockDim.x + threadIdx.x; i < pieces;
-       i += gridDim.x * blockDim.x) {
-    const float scale = scales[i / per_row];
-    const uint4 u = reinterpret_cast<const uint4*>(codes)[i];
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-    float x[2][8];
+  for (int64_t bh = blockIdx.z; bh < heads; bh += gridDim.z) {
+    const uint8_t* codes =
+        static_cast<const uint8_t*>(kv ? c.v : c.k) + (bh * c.capacity + start) * D;
+    const float* scales = (kv ? c.vs : c.ks) + bh * c.capacity + start;
+    T* out = (kv ? v_out : k_out) + bh * n * D;
+    for (unsigned i = blockIdx.x * blockDim.x + threadIdx.x; i < pieces;
+         i += gridDim.x * blockDim.x) {
+      const float scale = scales[i / per_row];
+      const uint4 u = reinterpret_cast<const uint4*>(codes)[i];
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+      float x[2][8];
 #pragma unroll
-    for (int q = 0; q < 8; ++q) {
-      const uint32_t two = q & 1 ? w[q >> 1] >> 16 : w[q >> 1] & 0xffff;
-      const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, __NV_E4M3);
-      const float2 f = __half22float2(__half2(h));
-      x[q >> 2][(2 * q) & 7] = f.x * scale;
-      x[q >> 2][(2 * q + 1) & 7] = f.y * scale;
+      for (int q = 0; q < 8; ++q) {
+        const uint32_t two = q & 1 ? w[q >> 1] >> 16 : w[q >> 1] & 0xffff;
+        const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, __NV_E4M3);
+        const float2 f = __half22float2(__half2(h));
+        x[q >> 2][(2 * q) & 7] = f.x * scale;
+        x[q >> 2][(2 * q + 1) & 7] = f.y * scale;
+      }
+      store8(out + (size_t)i * 16, x[0]);
+      store8(out + (size_t)i * 16 + 8, x[1]);
     }
-    store8(out + (size_t)i * 16, x[0]);
-    store8(out + (size_t)i * 16 + 8, x[1]);
   }
 }
 
@@ -358,20 +360,20 @@ extern "C" int mep_kv_read(int dtype, int64_t batch, int kv_heads, int head_dim,
   if (!aligned16(k_cache) || !aligned16(v_cache) || !aligned16(k_out) || !aligned16(v_out))
     return serve_invalid(op, "tensors must start on a 16-byte boundary");
   const int64_t heads = batch * kv_heads;
-  if (heads > 65535) return serve_invalid(op, "batch * kv_heads up to 65535");
   if (columns * head_dim > 0xffffffffll) return serve_invalid(op, "columns * head_dim up to 2^32 - 1");
   const int64_t pieces = columns * (head_dim / 16);
   const int64_t most = 148 * 64 / heads + 1;  // CTAs of a head: some 64 an SM in all
   const int64_t want = (pieces + 255) / 256;
-  const dim3 grid((unsigned)(want < most ? want : most), 2, (unsigned)heads);
+  const dim3 grid((unsigned)(want < most ? want : most), 2,
+                  (unsigned)(heads < 65535 ? heads : 65535));
   const CacheView c{k_cache, v_cache, k_scale, v_scale, capacity};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == MEP_BF16)
-    k_kv_read<__nv_bfloat16><<<grid, 256, 0, st>>>(c, head_dim, start, columns,
+    k_kv_read<__nv_bfloat16><<<grid, 256, 0, st>>>(c, heads, head_dim, start, columns,
                                                    static_cast<__nv_bfloat16*>(k_out),
                                                    static_cast<__nv_bfloat16*>(v_out));
   else
-    k_kv_read<float><<<grid, 256, 0, st>>>(c, head_dim, start, columns,
+    k_kv_read<float><<<grid, 256, 0, st>>>(c, heads, head_dim, start, columns,
                                            static_cast<float*>(k_out), static_cast<float*>(v_out));
   return serve_launched(op);
 }

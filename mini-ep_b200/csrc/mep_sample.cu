@@ -279,7 +279,8 @@ __global__ void __launch_bounds__(kNT, 2) k_sample(const SampleArgs a, int cache
   const float temp = a.temperature ? a.temperature[row] : a.temperature_s;
   const int64_t top_k = a.top_k ? a.top_k[row] : a.top_k_s;
   const float top_p = a.top_p ? a.top_p[row] : a.top_p_s;
-  const float min_p = a.min_p ? a.min_p[row] : a.min_p_s;
+  const float min_p_given = a.min_p ? a.min_p[row] : a.min_p_s;
+  const float min_p = min_p_given > 1.f ? 1.f : min_p_given;
 
   // 16-byte pieces of the row on the grid of its addresses; piece p holds the
   // ids from p * E - shift on. This CTA has [p0, p1), this warp [w0, w1).

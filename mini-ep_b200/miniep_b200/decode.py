@@ -271,7 +271,9 @@ def cache_attention(q, cache: KVCache, layer: int, col, scale: float, *, lengths
     (`lengths` (B,) int64: the row's prompt inside the padded prompt columns;
     None: every c <= col + t), and all of `prefix`. `col` is an int or a
     one-element int64 device tensor. Returns (B, T, Hq, D) contiguous; zeros
-    for a query that sees nothing."""
+    for a query that sees nothing. What a column holds that none of the call's
+    queries of its row sees does not matter (NaN included); with T > 1, a NaN
+    in a column that a later query sees reaches the row's earlier ones too."""
     B, T, Hq, D = _heads(q, cache)
     dev, dt, Hk = cache.device, cache.dtype, cache.kv_heads
     lens = 0
@@ -312,7 +314,7 @@ def sample_tokens(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, *,
     are the first top_k (0: all), of those the ones whose preceding mass is
     below top_p of their mass, of those w >= min_p; the token is the first id,
     ascending, whose running kept weight exceeds u times its sum. Temperature 0
-    takes the best token (lowest id). Each of temperature, top_p, min_p (fp32)
+    (or NaN) takes the best token (lowest id). Each of temperature, top_p, min_p (fp32)
     and top_k (int32) is a number or a (B,) device tensor. A row whose logits
     are all -inf or NaN gives token -1."""
     _tensor(logits, "logits", None)
@@ -367,7 +369,10 @@ class Sampler:
 
     def uniform(self, *shape, device):
         """The next uniform numbers of the sequence."""
-        if self._gen is None or self._gen.device != torch.device(device):
+        device = torch.device(device)
+        if device.type == "cuda" and device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
+        if self._gen is None or self._gen.device != device:
             self._gen = torch.Generator(device=device)
             self._gen.manual_seed(self.seed)
         return torch.rand(*shape, generator=self._gen, device=device)

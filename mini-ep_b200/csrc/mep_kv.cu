@@ -13,6 +13,7 @@
 #include <cstdint>
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
+#include <type_traits>
 
 #include "mep_device.cuh"
 #include "mep_serve.cuh"
@@ -96,29 +97,31 @@ struct StoreArgs {
 // group when that is a power of two, else 0 (n lanes, this one the j-th).
 template <int L>
 __device__ __forceinline__ float group_sum(float x, int j, int n, int first) {
-  if (L) {
+  if constexpr (L != 0) {
 #pragma unroll
     for (int o = 1; o < L; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
     return x;
+  } else {
+    for (int o = 1; o < n; o <<= 1) {
+      const float y = __shfl_down_sync(0xffffffffu, x, o);
+      if (j + o < n) x += y;
+    }
+    return __shfl_sync(0xffffffffu, x, first);
   }
-  for (int o = 1; o < n; o <<= 1) {
-    const float y = __shfl_down_sync(0xffffffffu, x, o);
-    if (j + o < n) x += y;
-  }
-  return __shfl_sync(0xffffffffu, x, first);
 }
 template <int L>
 __device__ __forceinline__ float group_max(float x, int j, int n, int first) {
-  if (L) {
+  if constexpr (L != 0) {
 #pragma unroll
     for (int o = 1; o < L; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
     return x;
+  } else {
+    for (int o = 1; o < n; o <<= 1) {
+      const float y = __shfl_down_sync(0xffffffffu, x, o);
+      if (j + o < n) x = fmaxf(x, y);
+    }
+    return __shfl_sync(0xffffffffu, x, first);
   }
-  for (int o = 1; o < n; o <<= 1) {
-    const float y = __shfl_down_sync(0xffffffffu, x, o);
-    if (j + o < n) x = fmaxf(x, y);
-  }
-  return __shfl_sync(0xffffffffu, x, first);
 }
 
 // A lane holds values 4j..4j+3 of a head row and the same of its other half,
@@ -140,27 +143,6 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 3)
   if (tok >= a.batch * a.tokens) return;
   const int p0 = (int)(item - tok * parts) * share, p1 = min(qp + 2 * kp, p0 + share);
   const int64_t b = tok / a.tokens, t = tok - b * a.tokens;
-
-  // pass p: its kind (0 q, 1 k, 2 v), this lane's head of it
-  auto kind_of = [&](int p) { return p < qp ? 0 : p < qp + kp ? 1 : 2; };
-  auto head_of = [&](int p, int kind) {
-    return (p - (kind == 0 ? 0 : kind == 1 ? qp : qp + kp)) * per_warp + sub;
-  };
-  auto live = [&](int kind, int h) {
-    return sub < per_warp && h < (kind == 0 ? a.q_heads : a.kv_heads);
-  };
-  Raw4<T> raw[2];
-  auto load = [&](int p) {
-    const int kind = kind_of(p), h = head_of(p, kind);
-    if (live(kind, h)) {
-      const HeadsView& in = kind == 0 ? a.q : kind == 1 ? a.k : a.v;
-      const T* x = static_cast<const T*>(in.p) + b * in.sb + t * in.st + h * in.sh + 4 * j;
-      raw[0].load(x);
-      raw[1].load(x + half);
-    }
-  };
-  load(p0);
-
   const int64_t col = (a.col_dev ? *a.col_dev : a.col) + t;
   const bool stored = col >= 0 && col < a.capacity;
   float c[8], s[8];
@@ -176,62 +158,97 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 3)
       for (int i = 0; i < 8; ++i) c[i] = s[i] = __int_as_float(0x7fffffff);
     }
   }
-  for (int p = p0; p < p1; ++p) {
-    const int kind = kind_of(p), h = head_of(p, kind);
-    const bool on = live(kind, h);
-    float x[8];
-    raw[0].get(x);
-    raw[1].get(x + 4);
-    if (!on)
+
+  // the warp's passes [p, end) over the heads of one of q, k and v (KIND 0, 1, 2)
+  auto heads = [&](auto kind_tag, const HeadsView& in, int count, const void* norm, int p, int end) {
+    constexpr int KIND = decltype(kind_tag)::value;
+    if (p >= end) return;
+    const T* x0 = static_cast<const T*>(in.p) + b * in.sb + t * in.st + 4 * j +
+                  (int64_t)(p * per_warp + sub) * in.sh;
+    const int64_t step = (int64_t)per_warp * in.sh;
+    int h = p * per_warp + sub;  // this lane's head
+    const bool lane_on = sub < per_warp;
+    float w[8];
+    if (KIND < 2 && norm) {
+      const T* nw = static_cast<const T*>(norm) + (lane_on ? 4 * j : 0);
+      load4<T>(nw, w), load4<T>(nw + half, w + 4);
+    }
+    // rows of this call: where they go, and how far the next pass's are
+    T* q_to = nullptr;
+    C* kv_to = nullptr;
+    float* scale_to = nullptr;
+    if (KIND == 0) {
+      q_to = static_cast<T*>(a.q_out) + (tok * a.q_heads + h) * D + 4 * j;
+    } else {
+      const int64_t at = (b * a.kv_heads + h) * a.capacity + col;
+      kv_to = static_cast<C*>(KIND == 1 ? a.kc : a.vc) + at * D + 4 * j;
+      if (sizeof(C) == 1) scale_to = (KIND == 1 ? a.ks : a.vs) + at;
+    }
+    const int64_t kv_step = per_warp * a.capacity;
+    Raw4<T> raw[2] = {};
+    bool on = lane_on && h < count;
+    if (on) raw[0].load(x0), raw[1].load(x0 + half);
+    for (; p < end; ++p) {
+      float x[8];
+      raw[0].get(x);
+      raw[1].get(x + 4);
+      x0 += step;
+      h += per_warp;
+      const bool next = lane_on && h < count;
+      if (p + 1 < end && next) raw[0].load(x0), raw[1].load(x0 + half);
+      if (KIND < 2) {
+        if (norm) {
+          float ss = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = 0.f;
-    if (p + 1 < p1) load(p + 1);
-    if (kind < 2) {
-      const T* nw = static_cast<const T*>(kind == 0 ? a.q_norm : a.k_norm);
-      if (nw) {
-        float ss = 0.f, w[8];
+          for (int i = 0; i < 8; ++i) ss += x[i] * x[i];
+          ss = group_sum<LT>(ss, j, L, first);
+          const float r = rsqrtf(ss / (float)D + a.eps);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) ss += x[i] * x[i];
-        ss = group_sum<LT>(ss, j, L, first);
-        const float r = rsqrtf(ss / (float)D + a.eps);
-        const int at = sub < per_warp ? 4 * j : 0;
-        load4<T>(nw + at, w), load4<T>(nw + at + half, w + 4);
+          for (int i = 0; i < 8; ++i) x[i] = x[i] * r * w[i];
+        }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = x[i] * r * w[i];
+        for (int i = 0; i < 4; ++i) {
+          const float lo = x[i], hi = x[i + 4];
+          x[i] = lo * c[i] - hi * s[i];
+          x[i + 4] = hi * c[i + 4] + lo * s[i + 4];
+        }
       }
+      if (KIND == 0) {
+        if (on) {
+          store4(q_to, x);
+          store4(q_to + half, x + 4);
+        }
+        q_to += per_warp * D;
+      } else {
+        if (sizeof(C) == 1) {
+          float m = 0.f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float lo = x[i], hi = x[i + 4];
-        x[i] = lo * c[i] - hi * s[i];
-        x[i + 4] = hi * c[i + 4] + lo * s[i + 4];
+          for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(x[i]));
+          m = group_max<LT>(m, j, L, first);
+          const bool some = m >= kTinyRow;
+          // 448 / m in the row's first lane and m / 448 in its second: one
+          // division an instruction for both
+          const float d = (j & 1 ? m : kE4M3Max) / (j & 1 ? kE4M3Max : m);
+          const float inv = some ? __shfl_sync(0xffffffffu, d, first & 31) : 0.f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] *= inv;
+          if (on && stored && j == 1) *scale_to = some ? d : 0.f;
+          scale_to += kv_step;
+        }
+        if (on && stored) {
+          store4(kv_to, x);
+          store4(kv_to + half, x + 4);
+        }
+        kv_to += kv_step * D;
       }
+      on = next;
     }
-    if (kind == 0) {
-      if (on) {
-        T* out = static_cast<T*>(a.q_out) + (tok * a.q_heads + h) * D + 4 * j;
-        store4(out, x);
-        store4(out + half, x + 4);
-      }
-      continue;
-    }
-    const int64_t at = (b * a.kv_heads + h) * a.capacity + col;
-    if (sizeof(C) == 1) {
-      float m = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(x[i]));
-      m = group_max<LT>(m, j, L, first);
-      const bool some = m >= kTinyRow;
-      const float inv = some ? kE4M3Max / m : 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] *= inv;
-      if (on && stored && j == 0) (kind == 1 ? a.ks : a.vs)[at] = some ? m / kE4M3Max : 0.f;
-    }
-    if (on && stored) {
-      C* out = static_cast<C*>(kind == 1 ? a.kc : a.vc) + at * D + 4 * j;
-      store4(out, x);
-      store4(out + half, x + 4);
-    }
-  }
+  };
+  heads(std::integral_constant<int, 0>(), a.q, a.q_heads, a.q_norm, p0, min(p1, qp));
+  heads(std::integral_constant<int, 1>(), a.k, a.kv_heads, a.k_norm, max(p0 - qp, 0),
+        min(p1 - qp, kp));
+  heads(std::integral_constant<int, 2>(), a.v, a.kv_heads, nullptr, max(p0 - qp - kp, 0),
+        p1 - qp - kp);
 }
 
 template <typename T, typename C, typename W, int LT>

@@ -215,7 +215,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int w = 0; w < 2; ++w) {
       mbar_init(&S->qready[w], 4), mbar_init(&S->qfree[w], 4), mbar_init(&S->odone[w], 1);
       mbar_init(&S->ofull[w], 1);
-      for (int i = 0; i < 2; ++i) mbar_init(&S->sfull[w][i], 1), mbar_init(&S->pfull[w][i], 4);
+      for (int i = 0; i < 2; ++i) mbar_init(&S->sfull[w][i], 1), mbar_init(&S->pfull[w][i], kRows);
     }
     S->abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -232,8 +232,21 @@ __global__ void __launch_bounds__(kThreads, 1)
   fence_after();
   // S of half w, buffer i: columns 128 w + 64 i; O: 256 + DP w
   const uint32_t tmem = S->tmem_base;
+  // bounded; the clock is first read after 256 tries, well past any wait of a
+  // healthy run (reading it at the first miss held up every wait)
   auto wait = [&](uint64_t* b, uint32_t parity) {
-    return mbar_wait_for(b, parity, kWaitNs, &S->abort);
+    unsigned long long t0 = 0;
+    for (uint32_t it = 1; !mbar_try(b, parity); ++it) {
+      if (it & 255u) continue;
+      if (*reinterpret_cast<volatile int*>(&S->abort)) return false;
+      const unsigned long long now = globaltimer_ns();
+      if (t0 == 0) t0 = now;
+      if (now - t0 > kWaitNs) {
+        *reinterpret_cast<volatile int*>(&S->abort) = 1;
+        return false;
+      }
+    }
+    return true;
   };
   // this CTA's run of units; f(tile, first key tile, last + 1) for each tile in it
   const int64_t u0 = p.units * blockIdx.x / gridDim.x, u1 = p.units * (blockIdx.x + 1) / gridDim.x;
@@ -384,8 +397,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // ---- this thread's query row, K-major with the 128-byte swizzle, once the
       // half's four warps have written the last tile's results out of the buffer
       int ok = 1;
-      if (lane == 0) ok = wait(&S->qfree[w], fph);
-      ok = __shfl_sync(0xffffffffu, ok, 0);
+      ok = __all_sync(0xffffffffu, wait(&S->qfree[w], fph));
       fph ^= 1u;
       if (ok) {
         const __nv_bfloat16* q =
@@ -409,8 +421,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int steps = steps_of(k0, k1);
       for (int t = 0; ok && t < steps; ++t) {
         const int i = t & 1;
-        if (lane == 0) ok = wait(&S->sfull[w][i], sph[i]);
-        ok = __shfl_sync(0xffffffffu, ok, 0);
+        ok = __all_sync(0xffffffffu, wait(&S->sfull[w][i], sph[i]));
         if (!ok) break;
         sph[i] ^= 1u;
         fence_after();
@@ -438,8 +449,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           m = mx;
         } else if (__any_sync(0xffffffffu, grow)) {
           // the last step's product has to be done before O is touched
-          if (lane == 0) ok = wait(&S->odone[w], dph);
-          ok = __shfl_sync(0xffffffffu, ok, 0);
+          ok = __all_sync(0xffffffffu, wait(&S->odone[w], dph));
           if (!ok) break;
           fence_after();
           const float f = grow ? ex2((m - mx) * rs) : 1.f;
@@ -473,8 +483,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         tmem_wait_st();
         fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&S->pfull[w][i]);
+        mbar_arrive(&S->pfull[w][i]);
         dph ^= 1u;
         float x, y;
         unpair(add2(sum[0], sum[1]), x, y);
@@ -482,8 +491,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       // ---- the run's result to its slot; slots behind the tile's last are empty
       if (ok) {
-        if (lane == 0) ok = wait(&S->ofull[w], oph);
-        ok = __shfl_sync(0xffffffffu, ok, 0);
+        ok = __all_sync(0xffffffffu, wait(&S->ofull[w], oph));
         oph ^= 1u;
       }
       fence_after();

@@ -9,8 +9,9 @@
 // maximum and the exponentials, P goes back to TMEM over S as bf16 and is the A
 // operand of O += P V, which stays in TMEM. Each half has two S buffers, so
 // that the next step's scores are there when a step's exponentials are done:
-// with one of 128 keys the products' latency (1900 of 4100 clocks a tile) lay
-// open. Q lies in shared memory, K and V come by TMA through rings (a 3D
+// with one buffer of 128 keys the products' latency (1900 of 4100 clocks a
+// tile) lay open, 128 us where this takes 109, although a product of 64 columns
+// holds the tensor cores as long as one of 128. Q lies in shared memory, K and V come by TMA through rings (a 3D
 // tensor map, so that the last tile's missing keys read as zeros). O is
 // rescaled only when a row's maximum has grown by more than 2^8 since it was
 // last fixed: weights up to 2^8 are as exact in bf16 and fp32 as weights up to 1.
@@ -18,6 +19,13 @@
 // Persistent: the (head, 256-row tile, key tile) units are dealt to the CTAs in
 // equal runs, so a tile's keys may be cut between CTAs. A run's result is a
 // partial one (fp32 sums, maximum in base 2) in the tile's next slot.
+//
+// 6144 rows on each of 8 heads of 128 behind 4099 keys: 109 us, 950 TFLOP/s,
+// 0.59 of the measured bf16 rate (on warp-level products the call took 477 us).
+// A tile of 128 keys takes the two halves 2 x 2 x (4 + 8) products of some 64
+// clocks each, about three quarters of its time; the exponentials (2048 clocks
+// of the unit that does 16 a clock) run beside them. 128 rows on each of 8 heads
+// of 64 behind 4096 keys: 10.7 us, latency.
 #include <cstdint>
 #include <cudaTypedefs.h>
 #include <cuda_bf16.h>

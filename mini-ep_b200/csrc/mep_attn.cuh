@@ -23,6 +23,9 @@ struct AttnArgs {
 };
 
 constexpr float kLog2e = 1.4426950408889634f;
+// Least factor of the scores: a masked score is -inf and has to stay that, which
+// it would not times 0. Scores below 2^100 all weigh alike under it, as under 0.
+constexpr float kLeastScale = 1.17549435e-38f;  // 2^-126
 
 __device__ __forceinline__ float ex2(float x) {
   float y;

@@ -390,7 +390,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int w = wp >> 2, quad = wp & 3, tr = quad * 32 + lane;  // half, lane quadrant, row
     const uint32_t lanes = (uint32_t)(quad * 32) << 16;
     const uint32_t ts = tmem + lanes + 128 * w, to = tmem + lanes + 256 + DP * w;
-    const float turn = a.scale < 0.f ? -1.f : 1.f, rs = a.scale * turn * kLog2e;
+    const float turn = a.scale < 0.f ? -1.f : 1.f;
+    const float rs = fmaxf(a.scale * turn * kLog2e, kLeastScale);
     const uint32_t flip = turn < 0.f ? 0x80008000u : 0u;
     // dph: parity of the last step's product. Its wait in step t may lag by one
     // phase only: the scores of step t came behind the product of step t - 2.

@@ -316,6 +316,27 @@ def test_attention_prefix_with_growing_scores(heads, scale):
         within(got, out, R.attention_tol(out, spread, size, n, BF, D, False))
 
 
+@pytest.mark.parametrize("quant", [False, True], ids=["plain", "e4m3"])
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+def test_attention_scale_zero_weighs_every_seen_column_alike(dtype, quant):
+    """Masked columns stay out at a scale of 0, one of -0, and one so small that
+    it vanishes against small queries."""
+    for heads, span, P in (((8, 4, 64), (2, 1, 300, 2, 200), 0),
+                           ((8, 4, 64), (2, 3, 70, 5, 1), 37),
+                           ((16, 8, 64), (160, 1, 5, 2, 1), 333)):
+        g = gen(17)
+        q, cache, kd, vd, lengths, col, prefix = make(g, heads, span, dtype, quant, P)
+        B, T, prompt = span[:3]
+        kp, vp = (None, None) if prefix is None else (prefix.k[0], prefix.v[0])
+        keep = R.visible(T, cache.capacity, col, lengths, prompt, B, "cuda")
+        for scale, by in ((0.0, 1.0), (-0.0, 1.0), (1e-30, 1e-30)):
+            x = q * by
+            got = cache_attention(x, cache, 0, col, scale, lengths=lengths, prompt_cols=prompt,
+                                  prefix=prefix)
+            out, spread, size, n = R.attention(x, kd[0], vd[0], keep, scale, kp, vp)
+            within(got, out, R.attention_tol(out, spread, size, n, dtype, heads[2], quant))
+
+
 def test_attention_prefix_far_larger_than_a_run():
     """Key tiles dealt over all SMs, tiles cut between them, tails of a tile."""
     for heads, B, P in (((2, 1, 64), 64, 20001), ((16, 8, 64), 1100, 333), ((8, 1, 128), 33, 4097)):

@@ -366,7 +366,8 @@ int mep_kv_read(int dtype, int64_t batch, int kv_heads, int head_dim, const void
  * c <= col + t and (c < lengths[b] or c >= prompt_cols): the row's prompt in
  * columns [0, lengths[b]) of the padded prompt_cols, and what was decoded
  * behind them (lengths NULL: every c <= col + t). A query that sees nothing
- * gets zeros. q: (batch, tokens, q_heads, head_dim) strided; out the same,
+ * gets zeros. scale: finite, |scale| <= 2^127. q: (batch, tokens, q_heads,
+ * head_dim) strided; out the same,
  * contiguous. workspace: mep_cache_attention_workspace bytes, the caller's, in
  * use until the call's work on `stream` is done.
  */

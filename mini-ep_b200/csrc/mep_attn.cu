@@ -1112,6 +1112,8 @@ extern "C" int mep_cache_attention(const mep_attention_args* x, void* stream) {
     return serve_invalid(op, "columns up to 2^31 - 1025");
   if (!x->col_dev && (x->col < 0 || x->col > x->capacity - x->tokens))
     return serve_invalid(op, "columns [col, col + tokens) do not fit the cache");
+  if (!(x->scale >= -0x1p127 && x->scale <= 0x1p127))  // times log2 e it still has to fit fp32
+    return serve_invalid(op, "scale must be finite, up to 2^127");
   if (x->batch == 0 || x->tokens == 0) return MEP_OK;
   const AttnArgs a{x->batch, x->tokens, (int)x->q_heads, (int)x->kv_heads, (int)x->head_dim,
                    {x->q, x->q_sb, x->q_st, x->q_sh},

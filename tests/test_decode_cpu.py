@@ -120,3 +120,10 @@ def test_workspace_is_host_arithmetic(lib):
     assert lib.mep_cache_attention_workspace(*_heads(), 4096, 4000, 512, C.byref(n)) == 0
     assert n.value >= 0
     assert lib.mep_cache_attention_workspace(*_heads(), 4096, 4000, 512, None) == 1
+
+
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), -float("inf"), 1e39])
+def test_scale_must_be_finite(lib, scale):
+    args = _lib.ATTENTION_ARGS.pack(*_heads(), *[0] * 8, 8, 0, 0, 0, 0, 0, 0, 0, scale, 0, 0, 0)
+    assert lib.mep_cache_attention(args, None) == 1
+    assert b"scale" in lib.mep_last_error(None)

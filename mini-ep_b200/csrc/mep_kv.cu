@@ -263,7 +263,8 @@ void launch_store_l(const StoreArgs& a, cudaStream_t st) {
   const int passes = (a.q_heads + per_warp - 1) / per_warp + 2 * ((a.kv_heads + per_warp - 1) / per_warp);
   const int64_t tokens = a.batch * a.tokens;
   // few tokens: one pass a warp, for the latency; many (32 warps on each of
-  // 148 SMs, four passes each): up to 12, which share the table rows
+  // 148 SMs, four passes each): all of a token's up to 12, else half of them,
+  // which share the table rows
   const int share = tokens * passes < (int64_t)148 * 32 * 4 ? 1 : passes <= 12 ? passes : (passes + 1) / 2;
   const int parts = (passes + share - 1) / share;
   const int warps = share == 1 ? 4 : 8;
@@ -375,7 +376,7 @@ extern "C" int mep_kv_read(int dtype, int64_t batch, int kv_heads, int head_dim,
   const char* op = "mep_kv_read";
   if (const char* why = bad_heads(dtype, MEP_E4M3, batch, 1, kv_heads, kv_heads, head_dim))
     return serve_invalid(op, why);
-  if (start < 0 || columns < 0 || start + columns > capacity)
+  if (start < 0 || columns < 0 || capacity < 0 || columns > capacity - start)
     return serve_invalid(op, "columns outside the cache");
   if (batch == 0 || columns == 0) return MEP_OK;
   if (!k_cache || !v_cache || !k_scale || !v_scale || !k_out || !v_out)

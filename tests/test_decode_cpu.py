@@ -127,3 +127,9 @@ def test_scale_must_be_finite(lib, scale):
     args = _lib.ATTENTION_ARGS.pack(*_heads(), *[0] * 8, 8, 0, 0, 0, 0, 0, 0, 0, scale, 0, 0, 0)
     assert lib.mep_cache_attention(args, None) == 1
     assert b"scale" in lib.mep_last_error(None)
+
+
+@pytest.mark.parametrize("start,n", [(2 ** 63 - 1, 2), (2 ** 63 - 1, 2 ** 63 - 1), (5, 2 ** 63 - 1)])
+def test_columns_to_read_whose_end_passes_64_bits(lib, start, n):
+    assert lib.mep_kv_read(1, 2, 2, 64, None, None, None, None, 8, start, n, None, None, None) == 1
+    assert b"columns" in lib.mep_last_error(None)

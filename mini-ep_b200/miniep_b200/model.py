@@ -343,6 +343,8 @@ class Engine:
         """Keys and values of a common prompt, computed once: shards built with
         ``prefix=`` see it in front of every row. Every rank calls it (one
         lockstep forward over a shard of one row)."""
+        if not tokens:
+            raise ValueError("a common prompt needs at least one token")
         shard = Shard([tokens], self.model.cfg, 0, self.model.device, self.model.dtype,
                       kernels=True)
         self.prefill(shard, dummy=dummy)

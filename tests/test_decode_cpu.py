@@ -9,6 +9,7 @@ import torch
 
 import miniep_b200 as M
 from miniep_b200 import MEPError, _lib, build
+from miniep_b200.model import GRANITE_1B_A400M, Engine, ModelConfig
 
 
 @pytest.fixture(scope="module")
@@ -133,3 +134,17 @@ def test_scale_must_be_finite(lib, scale):
 def test_columns_to_read_whose_end_passes_64_bits(lib, start, n):
     assert lib.mep_kv_read(1, 2, 2, 64, None, None, None, None, 8, start, n, None, None, None) == 1
     assert b"columns" in lib.mep_last_error(None)
+
+
+class _NoForward:
+    """A model that must not be reached."""
+    cfg = ModelConfig.from_dict(dict(GRANITE_1B_A400M, num_hidden_layers=1))
+    device, dtype = torch.device("cpu"), torch.float32
+
+    def forward(self, *a, **k):
+        raise AssertionError("a forward ran")
+
+
+def test_an_empty_common_prompt_is_refused():
+    with pytest.raises(ValueError, match="token"):
+        Engine(_NoForward()).build_prefix([])

@@ -402,6 +402,9 @@ class Engine:
         rank (dummy shard) passes idle=True and adds no expert load."""
         if steps < 1:
             return shard.last_tokens
+        if shard.used + steps > shard.cap:
+            raise ValueError(f"{steps} steps need {shard.used + steps} cache columns, the shard "
+                             f"has {shard.cap}")
         m, dev = self.model, shard.input.device
         cols = torch.arange(shard.cap, device=dev)
         col = torch.full((1,), shard.used, dtype=torch.long, device=dev)

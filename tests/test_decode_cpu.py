@@ -9,7 +9,7 @@ import torch
 
 import miniep_b200 as M
 from miniep_b200 import MEPError, _lib, build
-from miniep_b200.model import GRANITE_1B_A400M, Engine, ModelConfig
+from miniep_b200.model import GRANITE_1B_A400M, Engine, ModelConfig, Shard
 
 
 @pytest.fixture(scope="module")
@@ -148,3 +148,12 @@ class _NoForward:
 def test_an_empty_common_prompt_is_refused():
     with pytest.raises(ValueError, match="token"):
         Engine(_NoForward()).build_prefix([])
+
+
+def test_replayed_steps_behind_the_cache_are_refused():
+    m = _NoForward()
+    shard = Shard([[1, 2, 3]], m.cfg, 2, "cpu", torch.float32)
+    shard.used, shard.last_tokens = 3, torch.zeros(1, dtype=torch.long)
+    with pytest.raises(ValueError, match="columns"):
+        Engine(m).decode_graphed(shard, 3)
+    assert shard.used == 3 and shard.generated == [[]]

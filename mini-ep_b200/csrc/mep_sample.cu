@@ -459,10 +459,11 @@ __global__ void __launch_bounds__(kNT, 2) k_sample(const SampleArgs a, int cache
       to->wties[rank * kNW + warp] = n_edge;
     }
     cluster.sync();
-    // this warp's share begins at `start`; the row's kept mass is `total`
+    // of every warp's run its share of the row's kept mass, `total`, and the ids
+    // on the edge before it; the run that the target falls in is `owner`'s
     constexpr int PW = kMaxCtas * kNW / 32;
-    u64 share[PW], sum = 0, start = 0, total;
-    uint32_t t[PW], seen = 0;
+    u64 share[PW], sum = 0, start = 0;
+    uint32_t t[PW], seen = 0, before = 0;
 #pragma unroll
     for (int i = 0; i < PW; ++i) {
       const int j = lane * PW + i;
@@ -470,31 +471,70 @@ __global__ void __launch_bounds__(kNT, 2) k_sample(const SampleArgs a, int cache
       t[i] = j < nc * kNW ? S.wties[j] : 0;
       seen += t[i];
     }
-    uint32_t at = (uint32_t)warp_scan(seen) - seen, before = 0;
-    const int me = rank * kNW + warp;
+    const uint32_t at0 = (uint32_t)warp_scan(seen) - seen;
+    uint32_t at = at0;
 #pragma unroll
     for (int i = 0; i < PW; ++i) {
-      if (lane * PW + i == me) before = at;
       share[i] += min((u64)t[i], ties > at ? ties - at : 0) * wedge;
       at += t[i];
       sum += share[i];
     }
-    const u64 inc = warp_scan(sum);
-    total = __shfl_sync(0xffffffffu, inc, 31);
+    const u64 inc = warp_scan(sum), total = __shfl_sync(0xffffffffu, inc, 31);
+    const u64 target = target_of(total);
     u64 run0 = inc - sum;
+    int owner = -1;
+    at = at0;
 #pragma unroll
     for (int i = 0; i < PW; ++i) {
-      if (lane * PW + i == me) start = run0;
+      if (target >= run0 && target - run0 < share[i])
+        owner = lane * PW + i, start = run0, before = at;
       run0 += share[i];
+      at += t[i];
     }
-    start = __shfl_sync(0xffffffffu, start, me / PW);
-    before = __shfl_sync(0xffffffffu, before, me / PW);
-    const u64 target = target_of(total);
-    const u64 own = mass + min((u64)n_edge, ties > before ? ties - before : 0) * wedge;
-    if (target < start || target >= start + own) return;
-    for (int p = w0; p < w1; p += 32) {
+    const uint32_t found = __ballot_sync(0xffffffffu, owner >= 0);
+    if (!found) return;
+    int src = __ffs(found) - 1;
+    owner = __shfl_sync(0xffffffffu, owner, src);
+    start = __shfl_sync(0xffffffffu, start, src);
+    before = __shfl_sync(0xffffffffu, before, src);
+    if (owner / kNW != rank) return;  // all warps of the CTA alike
+    int r0 = min(p1, p0 + per_w * (owner % kNW)), r1 = min(p1, r0 + per_w);
+    if (r1 - r0 > 64) {
+      // a long run is dealt to all warps first: one warp alone took up to 50 us
+      // for its 800 pieces, some 2 us for 32 of them
+      const int part = ((r1 - r0 + kNW - 1) / kNW + 31) / 32 * 32;
+      const int q0 = min(r1, r0 + part * warp), q1 = min(r1, q0 + part);
+      u64 m = 0;
+      uint32_t eq = 0;
+      for (int p = q0 + lane; p < q1; p += 32) {
+        float l[E];
+        unpack(piece(p), l);
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+          m += weigh(l[i]);  // 0 on the edge
+          eq += on_edge(l[i]);
+        }
+      }
+      m = warp_sum(m);
+      eq = __reduce_add_sync(0xffffffffu, eq);
+      if (lane == 0) S.red[warp] = m, S.red2[warp] = eq;
+      __syncthreads();
+      m = lane < kNW ? S.red[lane] : 0;
+      eq = lane < kNW ? (uint32_t)S.red2[lane] : 0;
+      before += (uint32_t)warp_scan(eq) - eq;
+      m += min((u64)eq, ties > before ? ties - before : 0) * wedge;
+      start += warp_scan(m) - m;
+      src = __ffs(__ballot_sync(0xffffffffu, target >= start && target - start < m)) - 1;
+      if (warp != src) return;
+      start = __shfl_sync(0xffffffffu, start, src);
+      before = __shfl_sync(0xffffffffu, before, src);
+      r0 = q0, r1 = q1;
+    } else if (warp != owner % kNW) {
+      return;
+    }
+    for (int p = r0; p < r1; p += 32) {
       float l[E];
-      const bool have = p + lane < w1;
+      const bool have = p + lane < r1;
       if (have) unpack(piece(p + lane), l);
       u64 w[E], sum = 0;
       uint32_t eq = 0;

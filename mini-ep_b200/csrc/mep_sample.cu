@@ -573,10 +573,11 @@ __global__ void __launch_bounds__(kNT, 2) k_sample(const SampleArgs a, int cache
     const int cut_mag = __float_as_int(W.lcut) >> 16 & 0x7fff;
     const bool fits = top_mag < kSmall + kHalf - 1 &&
                       (W.lcut >= 0.f || cut_mag < kSmall + kHalf);
-    // a few tokens by top_k are sooner on one CTA's list (71 us against 113 at
-    // 256 x 100003, 17 against 23 for one row), short runs without a border
-    // sooner by their exponentials (12.5 against 16.5 us at 6000 ids a CTA)
-    const bool brief = by_k ? top_k <= 128 : !by_p && (p1 - p0) * E < 8192;
+    // a few tokens by top_k are sooner on one CTA's list (15 us against 20 for a
+    // row of 49,155, 22 against 29 for 64; alike at 256 x 100003), short runs
+    // without a border by their exponentials (11.9 against 12.5 us at 2000 ids a
+    // CTA, 15.9 against 15.1 at 6000)
+    const bool brief = by_k ? top_k <= 128 : !by_p && (p1 - p0) * E < 4096;
     if (fits && !brief) {
       auto slot_of = [&](uint32_t bits) {  // of 16 bits; >= kCodes: small, or none
         const uint32_t c = (bits & 0x7fff) - kSmall;

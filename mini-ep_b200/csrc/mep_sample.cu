@@ -564,7 +564,9 @@ __global__ void __launch_bounds__(kNT, 2) k_sample(const SampleArgs a, int cache
 
   if constexpr (kTable) {
     // ---- a slot for each 16-bit value from 2^-9 to 2^7 in magnitude: kHalf of
-    // either sign in the order of their bits. By rank, best first: positive
+    // either sign in the order of their bits. The last of each sign takes all
+    // that has none (what the table is used for leaves no positive one there,
+    // and negative ones there weigh nothing). By rank, best first: positive
     // ones from lmax down, all smaller ones as one, negative ones.
     constexpr int kSmall = (127 - 9) << 7, kHalf = kCodes / 2;
     const int top_mag = __float_as_int(W.lmax) >> 16 & 0x7fff;
@@ -572,34 +574,32 @@ __global__ void __launch_bounds__(kNT, 2) k_sample(const SampleArgs a, int cache
     const int n_pos = W.lmax < 0.f ? 0 : max(top_mag - kSmall + 1, 0);
     const int cut_mag = __float_as_int(W.lcut) >> 16 & 0x7fff;
     const bool fits = top_mag < kSmall + kHalf - 1 &&
-                      (W.lcut >= 0.f || cut_mag < kSmall + kHalf);
+                      (W.lcut >= 0.f || cut_mag < kSmall + kHalf - 1);
     // a few tokens by top_k are sooner on one CTA's list (15 us against 20 for a
     // row of 49,155, 22 against 29 for 64; alike at 256 x 100003), short runs
     // without a border by their exponentials (11.9 against 12.5 us at 2000 ids a
     // CTA, 15.9 against 15.1 at 6000)
     const bool brief = by_k ? top_k <= 128 : !by_p && (p1 - p0) * E < 4096;
     if (fits && !brief) {
-      auto slot_of = [&](uint32_t bits) {  // of 16 bits; >= kCodes: small, or none
-        const uint32_t c = (bits & 0x7fff) - kSmall;
-        return c < (uint32_t)kHalf ? c + (bits >> 15) * kHalf : ~0u;
-      };
-      // f(slot) for a piece's values; the others are the result's bits
-      auto slots = [&](const uint4& v, auto f) {
-        const uint32_t u[4] = {v.x, v.y, v.z, v.w};
-        uint32_t rest = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const uint32_t c = slot_of(i & 1 ? u[i >> 1] >> 16 : u[i >> 1] & 0xffff);
-          if (c < (uint32_t)kCodes)
-            f(c);
-          else
-            rest |= 1u << i;
-        }
-        return rest;
+      auto slot_of = [&](uint32_t u, int high) {  // of a pair's low or high half
+        const uint32_t c = min((high ? u >> 16 & 0x7fff : u & 0x7fff) - kSmall, kHalf - 1u);
+        return c | ((high ? u >> 20 : u >> 4) & kHalf);
       };
       auto value = [&](const uint4& v, int i) {
         const uint32_t u = i < 2 ? v.x : i < 4 ? v.y : i < 6 ? v.z : v.w;
         return __uint_as_float(i & 1 ? u & 0xffff0000u : u << 16);
+      };
+      // f(value) for a piece's values below 2^-9 in magnitude
+      auto each_small = [&](const uint4& v, auto f) {
+        const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+        const uint32_t m = __vminu2(__vminu2(v.x & 0x7fff7fff, v.y & 0x7fff7fff),
+                                    __vminu2(v.z & 0x7fff7fff, v.w & 0x7fff7fff));
+        if (min(m & 0xffff, m >> 16) >= (uint32_t)kSmall) return;
+        uint32_t rest = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          rest |= (uint32_t)((i & 1 ? u[i >> 1] >> 16 & 0x7fff : u[i >> 1] & 0x7fff) < kSmall) << i;
+        for (; rest; rest &= rest - 1) f(value(v, __ffs(rest) - 1));
       };
       auto slot_at = [&](int rank) {  // n_pos (if not negative): the small ones' rank
         return rank < n_pos ? n_pos - 1 - rank : kHalf + rank - n_pos - 1;
@@ -613,11 +613,10 @@ __global__ void __launch_bounds__(kNT, 2) k_sample(const SampleArgs a, int cache
       uint32_t zcnt = 0;
       if (by_k || by_p) {
         each_piece([&](const uint4& v, int) {
-          uint32_t rest = slots(v, [&](uint32_t c) { atomicAdd(&S.mine[c], 1u); });
-          for (; rest; rest &= rest - 1) {
-            const float l = value(v, __ffs(rest) - 1);
-            if (small(l)) zall += W(l), ++zcnt;
-          }
+          const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int i = 0; i < 8; ++i) atomicAdd(&S.mine[slot_of(u[i >> 1], i & 1)], 1u);
+          each_small(v, [&](float l) { zall += W(l), ++zcnt; });
         });
         u64 all, nz;
         block_scan(zall, S.red, all);
@@ -710,40 +709,36 @@ __global__ void __launch_bounds__(kNT, 2) k_sample(const SampleArgs a, int cache
         for (int i = 0; i < PER; ++i)
           if (c0 + i < ranks && c0 + i != z && c0 + i < erank)
             S.weight[at(c0 + i)] = floored(w[i]);
-        const int eslot = erank < ranks ? at(erank) : -2;  // -1 is no slot either
+        // a border in the last slot leaves nothing out that weighs
+        const int eslot = erank < ranks && at(erank) != kCodes - 1 ? at(erank) : -1;
         u64 wedge = eslot >= 0 ? floored(W(logit(eslot))) : 0;
         if (eslot >= 0 && tid == 0) S.weight[eslot] = 0;
         __syncthreads();
         const bool some_small = z >= 0 && z < erank;
         auto weigh = [&](float l) -> u64 {
-          const uint32_t c = slot_of(__float_as_uint(l) >> 16);
-          if (c < (uint32_t)kCodes) return S.weight[c];
-          return some_small && small(l) ? floored(W(l)) : 0;
+          if (small(l)) return some_small ? floored(W(l)) : 0;
+          return S.weight[slot_of(__float_as_uint(l), 1)];
         };
         u64 mass = 0;
         uint32_t n_edge = 0;
-        // most tokens lie behind the border: one comparison, no table read
+        // a table read for every token, without a branch: tokens behind the border
+        // weigh 0 in it (72 us at 256 x 100003 against 81 with a comparison first)
         const float border = eslot >= 0 ? logit(eslot) : -INFINITY;
         each_piece([&](const uint4& v, int) {
-          uint32_t rest = 0;
+          const uint32_t u[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const float l = value(v, i);
-            if (l > border) {
-              const uint32_t c = slot_of(__float_as_uint(l) >> 16);
-              if (c < (uint32_t)kCodes)
-                mass += S.weight[c];
-              else
-                rest |= 1u << i;
-            }
+            mass += S.weight[slot_of(u[i >> 1], i & 1)];
             n_edge += wedge && l == border;
           }
-          if (some_small)
-            for (; rest; rest &= rest - 1) mass += weigh(value(v, __ffs(rest) - 1));
+          if (some_small) each_small(v, [&](float l) { mass += floored(W(l)); });
         });
         finish(mass, n_edge, weigh,
-               [&](float l) { return (int)slot_of(__float_as_uint(l) >> 16) == eslot; }, ties,
-               wedge);
+               [&](float l) {
+                 return !small(l) && (int)slot_of(__float_as_uint(l), 1) == eslot;
+               },
+               ties, wedge);
         return;
       }
     }

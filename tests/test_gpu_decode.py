@@ -493,6 +493,26 @@ def test_sample_small_and_large_logits():
                 draw_rows(logits, u, *filt)
 
 
+@pytest.mark.parametrize("top,temps", [(5.0, (3.7, 3.85)), (-100.0, (0.7, 0.79))], ids=str)
+def test_sample_values_past_the_end_of_the_table(top, temps):
+    """16-bit rows whose smallest weights lie near -127, with tokens below them
+    (finite ones, -inf, NaN) and, where the best is positive, around zero."""
+    inf, nan = math.inf, math.nan
+    pool = [top, top - 1, top - 2, -119.0, -123.5, -126.0, -127.0, -127.5, -128.0, -200.0, -inf,
+            nan, -nan]
+    if top > 0:
+        pool += [1e-4, -1e-4, 1.9e-3, -1.9e-3, 2e-3, 0.0, -0.0, 1.0, -1.0]
+    for B, V in ((3, 9001), (150, 4200)):
+        g = gen(V)
+        at = torch.randint(0, len(pool), (B, V), generator=g, device="cuda")
+        logits = torch.tensor(pool, device="cuda").to(BF)[at]
+        u = torch.rand(B, generator=g, device="cuda")
+        for temp in temps:
+            for k, p in (((0, 1.0), (300, 1.0), (V // 2, 0.9), (V - 1, 1.0), (V + 5, 0.9999999),
+                          (0, 0.9999999), (0, 0.3)) if B == 3 else ((V // 2, 0.9), (0, 1.0))):
+                draw_rows(logits, u, temp, k, p, 0.0)
+
+
 def test_sample_every_row_count():
     """Row counts that change how many CTAs share a row."""
     for B in (1, 9, 18, 37, 74, 150, 300):

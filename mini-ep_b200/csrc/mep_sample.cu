@@ -12,11 +12,12 @@
 // less where the row's sum would pass 62 bits): integer sums do not depend on
 // their order, and a weight, computed in 64 bits, is off by half a unit.
 //
-// Measured, bf16 / fp32 logits: 256 rows of 100,003 with top_p 0.95 125 / 273
-// us, with top_k 50 71 / 86 us, greedy 21 / 34 us; one row of 49,155 with top_k
-// and top_p 16.5 us, greedy 6.3 us. Reading the logits would take 8 / 16 us at
-// 256 rows: what bounds it is the work on every token (a shared-memory addition
-// and its conflicts, 15 to 20 instructions), for a few rows the chain of
+// Measured, bf16 / fp32 logits: 256 rows of 100,003 with top_p 0.95 72 / 207
+// us, unfiltered 53 / 103 us, with top_k 50 71 / 86 us, greedy 21 / 35 us; one
+// row of 49,155 with top_k and top_p 16.5 us, greedy 6.3 us. Reading the logits
+// would take 8 / 16 us at 256 rows: what bounds it is the work on every token
+// (bf16, top_p: 51 warp instructions for 32 tokens, a shared-memory addition
+// and a read among them) and 256 CTAs on 148 SMs, for a few rows the chain of
 // passes between cluster barriers.
 #include <cstdint>
 #include <cooperative_groups.h>

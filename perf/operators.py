@@ -21,19 +21,12 @@ E4M3_MAX = 448.0
 TINY = 2.0 ** -100
 
 
-_package = None
-
-
 def _framework():
-    """The package, imported once as a program imports it."""
-    global _package
-    if _package is None:
-        root = str(Path(__file__).resolve().parents[1] / "mini-ep_b200")
-        if root not in sys.path:
-            sys.path.insert(0, root)
-        import miniep_b200
-        _package = miniep_b200
-    return _package
+    root = str(Path(__file__).resolve().parents[1] / "mini-ep_b200")
+    if root not in sys.path:
+        sys.path.insert(0, root)
+    import miniep_b200
+    return miniep_b200
 
 
 # ------------------------------------------------------------------ cases

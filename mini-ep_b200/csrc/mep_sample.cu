@@ -579,8 +579,10 @@ __global__ void __launch_bounds__(kNT, 2) k_sample(const SampleArgs a, int cache
     // a few tokens by top_k are sooner on one CTA's list (15 us against 20 for a
     // row of 49,155, 22 against 29 for 64; alike at 256 x 100003), short runs
     // without a border by their exponentials (11.9 against 12.5 us at 2000 ids a
-    // CTA, 15.9 against 15.1 at 6000)
-    const bool brief = by_k ? top_k <= 128 : !by_p && (p1 - p0) * E < 4096;
+    // CTA, 15.9 against 15.1 at 6000). The row's CTAs have to choose alike, as
+    // the two ways meet at different barriers: `per` is the same in all of them,
+    // the last one's own run may be shorter.
+    const bool brief = by_k ? top_k <= 128 : !by_p && per * E < 4096;
     if (fits && !brief) {
       auto slot_of = [&](uint32_t u, int high) {  // of a pair's low or high half
         const uint32_t c = min((high ? u >> 16 & 0x7fff : u & 0x7fff) - kSmall, kHalf - 1u);

@@ -521,6 +521,22 @@ def test_sample_every_row_count():
         draw_rows(logits, torch.rand(B, generator=g, device="cuda"), 0.9, 30, 0.9, 0.0)
 
 
+@pytest.mark.parametrize("rows,V", [(1, 32705), (1, 32770), (36, 32770), (1, 32768), (37, 16346),
+                                    (73, 16384), (73, 16420), (74, 8177), (147, 8180),
+                                    (147, 8184)], ids=str)
+@pytest.mark.parametrize("aligned", [True, False], ids=["aligned", "shifted"])
+def test_sample_last_run_of_a_row_shorter_than_the_others(rows, V, aligned):
+    """Unfiltered 16-bit rows whose runs lie about 4096 ids, the row's last run
+    below it and the others not: all CTAs of a row go the same way."""
+    g = gen(V + rows)
+    pad = (-V) % 8 if aligned else 9 + V % 2  # an odd row stride: every start there is
+    whole = randn(g, rows, V + pad, dtype=BF, std=2.0)
+    logits = whole[:, :V] if aligned else whole[:, 1:1 + V]
+    u = torch.rand(rows, generator=g, device="cuda")
+    for filt in ((1.0, 0, 1.0, 0.0), (0.8, 0, 1.0, 0.01)):
+        draw_rows(logits, u, *filt)
+
+
 def test_sample_ties_take_the_lowest_ids():
     """Equal logits: exact shares, kept from the lowest id up."""
     for V in (16, 1000, 40000):

@@ -280,6 +280,9 @@ __global__ void __launch_bounds__(kNT, 2) k_sample(const SampleArgs a, int cache
   Shared& S = *reinterpret_cast<Shared*>(smem_raw);
   cg::cluster_group cluster = cg::this_cluster();
   const int nc = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  // others' shared memory may be touched once they run: waited for behind the
+  // first pass
+  if (nc > 1) cluster.barrier_arrive();
   const int64_t row = blockIdx.x / nc;
   const int V = (int)a.vocab;
   const int tid = threadIdx.x, lane = lane_id(), warp = warp_id();
@@ -347,6 +350,7 @@ __global__ void __launch_bounds__(kNT, 2) k_sample(const SampleArgs a, int cache
   }
   if (lane == 0) S.red[warp] = __float_as_uint(lmax), S.red2[warp] = __float_as_uint(lmin);
   __syncthreads();
+  if (nc > 1) cluster.barrier_wait();  // every CTA of the row has begun
   if (tid < nc) {
     for (int i = 0; i < kNW; ++i) {
       lmax = fmaxf(lmax, __uint_as_float((uint32_t)S.red[i]));

@@ -537,6 +537,22 @@ def test_sample_last_run_of_a_row_shorter_than_the_others(rows, V, aligned):
         draw_rows(logits, u, *filt)
 
 
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+def test_sample_short_runs_on_several_ctas(dtype):
+    """Rows just long enough for several CTAs each, whose first pass is over at
+    once, in many calls: the largest logit comes from every CTA's run."""
+    for rows, V in ((1, 1024), (37, 1025), (74, 1024), (147, 2047), (9, 8192), (36, 8193)):
+        g = gen(V)
+        for i in range(20):
+            logits = randn(g, rows, V, dtype=dtype)
+            at = torch.randint(0, V, (rows,), generator=g, device="cuda")
+            logits[torch.arange(rows, device="cuda"), at] = 60.0  # the others' share: V e^-54
+            u = torch.rand(rows, generator=g, device="cuda") * 0.999
+            assert torch.equal(sample_tokens(logits, u, 0.0), at)
+            assert torch.equal(sample_tokens(logits, u, 1.0), at)
+            assert torch.equal(sample_tokens(logits, u, 1.0, 3, 0.9), at)
+
+
 def test_sample_ties_take_the_lowest_ids():
     """Equal logits: exact shares, kept from the lowest id up."""
     for V in (16, 1000, 40000):

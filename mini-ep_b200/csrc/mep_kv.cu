@@ -235,7 +235,9 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 3)
           // 448 / m in the row's first lane and m / 448 in its second: one
           // division an instruction for both
           const float d = (j & 1 ? m : kE4M3Max) / (j & 1 ? kE4M3Max : m);
-          const float inv = some ? __shfl_sync(0xffffffffu, d, first & 31) : 0.f;
+          // every lane takes part, whatever its row holds
+          const float d0 = __shfl_sync(0xffffffffu, d, first & 31);
+          const float inv = some ? d0 : 0.f;
 #pragma unroll
           for (int i = 0; i < 8; ++i) x[i] *= inv;
           if (on && stored && j == 1) *scale_to = some ? d : 0.f;

@@ -141,6 +141,36 @@ def test_store_column_on_the_device():
     assert not cache.v.isnan().any()
 
 
+@pytest.mark.parametrize("heads", [(4, 8, 64), (2, 6, 16), (2, 1, 128), (3, 7, 80), (2, 5, 48)],
+                         ids=str)
+@pytest.mark.parametrize("B,T", [(2, 3), (4, 1900)], ids=str)
+def test_store_quantised_rows_of_zeros_among_others(heads, B, T):
+    """Rows of zeros and of numbers too small to scale in one pass of a warp
+    with others, lanes without a row, one pass a warp and several."""
+    Hq, Hk, D = heads
+    g = gen(D + T)
+    q, k, v = (randn(g, B, T, h, D, dtype=BF, std=2.0) for h in (Hq, Hk, Hk))
+    for x in (k, v):
+        kind = torch.randint(0, 3, x.shape[:3], generator=g, device="cuda")
+        x[kind == 1] = 0
+        x[kind == 2] *= torch.where(torch.rand(int((kind == 2).sum()), 1, generator=g,
+                                               device="cuda") < 0.5, 2.0 ** -110, 1.0).to(BF)
+    cos, sin = R.rope_tables(64, D)
+    pos = torch.randint(0, 64, (B, T), generator=g, device="cuda")
+    cache = KVCache.empty(1, B, Hk, T + 2, D, BF, quantized=True)
+    norm_rope_store(q, k, v, cos, sin, pos, cache, 0, 1)
+    kr, vr = cache.read(0, 1, 1 + T)
+    ref, mag = (t.transpose(1, 2) for t in R.rotated(k, None, cos, sin, pos, 0.0))
+    vt = v.transpose(1, 2).double()
+    for got, codes, scale, want, size in ((kr, cache.k, cache.k_scale, ref, mag),
+                                          (vr, cache.v, cache.v_scale, vt, vt.abs())):
+        tiny = want.abs().amax(-1) < 2.0 ** -100
+        assert not got[tiny].any() and not scale[0, :, :, 1:1 + T][tiny].any()
+        assert not codes[0, :, :, 1:1 + T].float()[tiny].any()
+        want = want.masked_fill(tiny[..., None], 0.0)
+        within(got, want, R.quantised_tol(want, size.masked_fill(tiny[..., None], 0.0), BF))
+
+
 def test_store_quantised_extremes():
     """Rows of zeros, of tiny and of huge numbers; a NaN stays one."""
     D = 64

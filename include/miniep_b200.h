@@ -392,6 +392,13 @@ typedef struct mep_attention_args {
   int64_t workspace_bytes;
 } mep_attention_args;
 int mep_cache_attention(const mep_attention_args* args, void* stream);
+/*
+ * Test hook: until it is called with -1, the loader of every CTA of the large
+ * batches' prefix kernel stops behind its K load number `loads` (from 0) as if
+ * a wait had run out. Waits are bounded (2 s); the rows that one leaves
+ * unfinished come out as NaN, and the context stays usable.
+ */
+int mep_debug_prefix_loads(int loads);
 /* Workspace of such a call (host arithmetic only). col: as given to the call,
  * or -1 when it is read on the device. */
 int mep_cache_attention_workspace(int dtype, int cache_dtype, int64_t batch, int64_t tokens,

@@ -26,6 +26,7 @@
 // clocks each, about three quarters of its time; the exponentials (2048 clocks
 // of the unit that does 16 a clock) run beside them. 128 rows on each of 8 heads
 // of 64 behind 4096 keys: 10.7 us, latency.
+#include <atomic>
 #include <cstdint>
 #include <cudaTypedefs.h>
 #include <cuda_bf16.h>
@@ -85,7 +86,7 @@ struct Cfg {
 
 struct Smem {
   uint64_t kfull[4], kempty[4], vfull[4], vempty[4];
-  uint64_t qready[2], qfree[2], sfull[2][2], pfull[2][2], odone[2], ofull[2];
+  uint64_t qready[2], qfree[2], sfull[2][2], pfull[2][2], odone[2], ofull[2], drained[2];
   uint32_t tmem_base;
   int abort;
 };
@@ -93,6 +94,7 @@ struct Smem {
 struct Args {
   AttnArgs a;
   int group, rows, row_tiles, key_tiles, slots;
+  int last_load;  // a CTA's loads stop at this one of K, as if a wait ran out (-1: never)
   int64_t units, out_rows;
   float* part_o;
   float2* part_ml;
@@ -222,7 +224,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int w = 0; w < 2; ++w) {
       mbar_init(&S->qready[w], 4), mbar_init(&S->qfree[w], 4), mbar_init(&S->odone[w], 1);
-      mbar_init(&S->ofull[w], 1);
+      mbar_init(&S->ofull[w], 1), mbar_init(&S->drained[w], 1);
       for (int i = 0; i < 2; ++i) mbar_init(&S->sfull[w][i], 1), mbar_init(&S->pfull[w][i], kRows);
     }
     S->abort = 0;
@@ -277,7 +279,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (wp == 10) {
     // ------------------------------------------------------------ TMA loads
     if (lane == 0) {
-      int s = 0, issued = 0;
+      int s = 0, k_loads = 0, v_loads = 0;
       uint32_t ph = 0;
       each_tile([&](int tile, int k0, int k1) {
         const int kh = tile / p.row_tiles;
@@ -286,23 +288,24 @@ __global__ void __launch_bounds__(kThreads, 1)
           mbar_expect_tx(&S->kfull[s], C::TILE);
           for (int d = 0; d < DP / 64; ++d)
             tma_load_3d(sk + s * C::TILE + d * C::SUB, &tmK, d * 64, k * kKeys, kh, &S->kfull[s]);
+          if (k_loads++ == p.last_load) {
+            *reinterpret_cast<volatile int*>(&S->abort) = 1;
+            return false;
+          }
           if (!wait(&S->vempty[s], ph ^ 1u)) return false;
           mbar_expect_tx(&S->vfull[s], C::TILE);
           for (int d = 0; d < DP / 64; ++d)
             tma_load_3d(sv + s * C::TILE + d * C::SUB, &tmV, d * 64, k * kKeys, kh, &S->vfull[s]);
-          ++issued;
+          ++v_loads;
           if (++s == C::STAGES) s = 0, ph ^= 1u;
         }
         return true;
       });
-      if (S->abort) {  // leave no copy in flight: wait for each stage's last one
-        for (int i = 0; i < C::STAGES && i < issued; ++i) {
-          s = s == 0 ? C::STAGES - 1 : s - 1;
-          if (s == C::STAGES - 1) ph ^= 1u;
-          mbar_wait_for(&S->kfull[s], ph, kWaitNs, nullptr);
-          mbar_wait_for(&S->vfull[s], ph, kWaitNs, nullptr);
-        }
-      }
+      // leave no copy in flight, whoever gave up: load n fills stage n % STAGES
+      for (int n = max(0, k_loads - C::STAGES); n < k_loads; ++n)
+        mbar_wait_for(&S->kfull[n % C::STAGES], n / C::STAGES & 1, kWaitNs, nullptr);
+      for (int n = max(0, v_loads - C::STAGES); n < v_loads; ++n)
+        mbar_wait_for(&S->vfull[n % C::STAGES], n / C::STAGES & 1, kWaitNs, nullptr);
     }
   } else if (wp >= 8) {
     // ------------------------------------------------------------ MMA issue
@@ -385,6 +388,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       return true;
     });
+    // leave no product in flight either
+    if (elect_one()) mma_commit<false>(&S->drained[w]);
+    __syncwarp();
+    mbar_wait_for(&S->drained[w], 0, kWaitNs, nullptr);
   } else {
     // ------------------------------------------------------------ softmax
     const int w = wp >> 2, quad = wp & 3, tr = quad * 32 + lane;  // half, lane quadrant, row
@@ -397,6 +404,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     // phase only: the scores of step t came behind the product of step t - 2.
     uint32_t sph[2] = {0, 0}, dph = 1, oph = 0, fph = 1;
     const int D = a.head_dim;
+    // Once a wait has run out the rest of the run is only marked: sums of NaN,
+    // which the join carries into every value of those rows.
+    int ok = 1;
     each_tile([&](int tile, int k0, int k1) {
       if (w >= halves_of(tile)) return true;
       const int kh = tile / p.row_tiles, r = (tile % p.row_tiles) * 2 * kRows + w * kRows + tr;
@@ -405,8 +415,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int b = bt / (int)a.tokens, t = bt - b * (int)a.tokens;
       // ---- this thread's query row, K-major with the 128-byte swizzle, once the
       // half's four warps have written the last tile's results out of the buffer
-      int ok = 1;
-      ok = __all_sync(0xffffffffu, wait(&S->qfree[w], fph));
+      if (ok) ok = __all_sync(0xffffffffu, wait(&S->qfree[w], fph));
       fph ^= 1u;
       if (ok) {
         const __nv_bfloat16* q =
@@ -509,14 +518,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int64_t orow = ((int64_t)b * a.tokens + t) * a.q_heads + h;
       if (real) {
         const float mb = m == -INFINITY ? m : m * rs;
-        // a wait that ran out leaves a result that cannot be missed
         p.part_ml[slot * p.out_rows + orow] =
             ok ? make_float2(mb, l) : make_float2(0.f, __int_as_float(0x7fffffff));
         if (k1 == p.key_tiles)
           for (int e = slot + 1; e < p.slots; ++e)
             p.part_ml[e * p.out_rows + orow] = make_float2(-INFINITY, 0.f);
       }
-      if (!ok) return false;
+      if (!ok) return true;
       // O through the half's query buffer, which no product reads any more: W
       // values of the warp's 32 rows at a time, written out a row at a time
       constexpr int W = DP / 4, STRIDE = W * 4 + 16, PER = W / 4;  // 16: rows in other banks
@@ -580,6 +588,8 @@ int launch(const Args& p, int ctas, cudaStream_t st) {
 }  // namespace px
 }  // namespace
 
+std::atomic<int> g_last_load{-1};
+
 constexpr int kMinUnits = 4;  // units of a CTA, at least (while the others suffice)
 
 PrefixTcPlan plan_prefix_tc(int64_t rows, int kv_heads, int64_t prefix_cols) {
@@ -597,7 +607,8 @@ PrefixTcPlan plan_prefix_tc(int64_t rows, int kv_heads, int64_t prefix_cols) {
 
 int launch_prefix_tc(const AttnArgs& a, const PrefixTcPlan& plan, int64_t out_rows, float* part_o,
                      float2* part_ml, cudaStream_t st) {
-  px::Args p{a, a.q_heads / a.kv_heads, 0, 0, 0, plan.slots, 0, out_rows, part_o, part_ml};
+  px::Args p{a, a.q_heads / a.kv_heads, 0, 0, 0, plan.slots,
+             g_last_load.load(std::memory_order_relaxed), 0, out_rows, part_o, part_ml};
   p.rows = (int)(a.batch * a.tokens * p.group);
   p.row_tiles = (p.rows + 2 * px::kRows - 1) / (2 * px::kRows);
   p.key_tiles = (int)((a.prefix_cols + px::kKeys - 1) / px::kKeys);
@@ -606,3 +617,8 @@ int launch_prefix_tc(const AttnArgs& a, const PrefixTcPlan& plan, int64_t out_ro
 }
 
 }  // namespace mep
+
+extern "C" int mep_debug_prefix_loads(int loads) {
+  mep::g_last_load.store(loads < 0 ? -1 : loads, std::memory_order_relaxed);
+  return MEP_OK;
+}

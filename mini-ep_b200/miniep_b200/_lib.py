@@ -67,6 +67,7 @@ SIGNATURES = {
     "mep_norm_rope_store": [C.c_char_p, _P],  # packed structs: STORE_ARGS, ATTENTION_ARGS
     "mep_kv_read": [_I, _I64, _I, _I, _P, _P, _P, _P, _I64, _I64, _I64, _P, _P, _P],
     "mep_cache_attention": [C.c_char_p, _P],
+    "mep_debug_prefix_loads": [_I],
     "mep_cache_attention_workspace": [_I, _I, _I64, _I64, _I, _I, _I, _I64, _I64, _I64,
                                       C.POINTER(_I64)],
     "mep_sample": [_I, _P, _I64, _I64, _I64, _P, _P, _P, _P, _P, C.c_float, C.c_int32, C.c_float,

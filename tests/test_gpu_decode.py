@@ -8,8 +8,8 @@ import torch
 
 import decode_ref as R
 from gpu_util import require_gpu
-from miniep_b200 import (KVCache, MEPError, Sampler, SharedPrefix, cache_attention, norm_rope_store,
-                         sample_tokens)
+from miniep_b200 import (KVCache, MEPError, Sampler, SharedPrefix, _lib, cache_attention,
+                         norm_rope_store, sample_tokens)
 
 pytestmark = pytest.mark.gpu
 BF, F32 = torch.bfloat16, torch.float32
@@ -371,6 +371,37 @@ def test_attention_prefix_far_larger_than_a_run():
     """Key tiles dealt over all SMs, tiles cut between them, tails of a tile."""
     for heads, B, P in (((2, 1, 64), 64, 20001), ((16, 8, 64), 1100, 333), ((8, 1, 128), 33, 4097)):
         attend_case(11, heads, (B, 1, 5, 2, 0), BF, True, P)
+
+
+@pytest.mark.parametrize("heads,B,P,last", [((16, 8, 64), 300, 1300, 3),
+                                            ((32, 8, 128), 200, 2500, 4),
+                                            ((32, 8, 128), 1500, 700, 7),
+                                            ((8, 1, 128), 33, 4097, 3)], ids=str)
+def test_attention_prefix_that_gives_up_leaves_no_finite_row(heads, B, P, last):
+    """Loads that stop early, as after a wait that ran out: every row is NaN or,
+    where all its keys had been read, what it is without; nothing is left in
+    flight, and the next call is whole."""
+    Hq, Hk, D = heads
+    g = gen(B)
+    q = randn(g, B, 1, Hq, D, dtype=BF)
+    cache = KVCache(randn(g, 1, B, Hk, 6, D, dtype=BF), randn(g, 1, B, Hk, 6, D, dtype=BF))
+    prefix = SharedPrefix(randn(g, 1, Hk, P, D, dtype=BF), randn(g, 1, Hk, P, D, dtype=BF))
+    want = cache_attention(q, cache, 0, 3, 0.1, prefix=prefix)
+    assert torch.isfinite(want.float()).all()
+    try:
+        for loads in (0, 1, 2, 3, last):  # the workspace holds the last call's sums
+            _lib.lib().mep_debug_prefix_loads(loads)
+            got = cache_attention(q, cache, 0, 3, 0.1, prefix=prefix)
+            _lib.lib().mep_debug_prefix_loads(-1)
+            nan = got.isnan()
+            assert torch.equal(nan.any(-1), nan.all(-1))
+            lost = nan.all(-1)
+            assert lost.all() if loads == 0 else lost.any()
+            assert torch.equal(got[~lost], want[~lost])
+            again = cache_attention(q, cache, 0, 3, 0.1, prefix=prefix)
+            assert torch.equal(again, want)
+    finally:
+        _lib.lib().mep_debug_prefix_loads(-1)
 
 
 @pytest.mark.parametrize("quant", [False, True], ids=["bf16", "e4m3"])

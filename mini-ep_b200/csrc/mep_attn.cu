@@ -93,6 +93,9 @@ __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) 
   hi = tf32(x);
   lo = tf32(x - __uint_as_float(hi));
 }
+__device__ __forceinline__ float two_to(int e) {  // 2^e, e in [-126, 127]
+  return __uint_as_float((uint32_t)(127 + e) << 23);
+}
 __device__ __forceinline__ uint32_t e4m3x2_f16x2(uint32_t two) {
   uint32_t r;
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((unsigned short)two));
@@ -433,7 +436,12 @@ __global__ void __launch_bounds__(kThreads, MODE == kByRows && sizeof(QT) == 2 ?
 #pragma unroll
     for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};  // m before rscale
-  float vref = 0.f;  // what o counts in, for scaled values: their largest scale so far
+  // Codes are weighed by p times their row's scale, in fp16 for 16-bit queries:
+  // times 2^wexp, which takes the row's largest such weight so far, wtop (before
+  // it, in units of the running maximum), to about 2^12. Weights then keep fp16's
+  // 11 bits down to 2^-26 of the largest, whatever p and scale are by themselves.
+  float wtop[2] = {0.f, 0.f};
+  int wexp[2] = {0, 0};
 
   int buf = 0, ahead = X::kStages - 1;
   for (int tile = tile0; tile < tile1; ++tile) {
@@ -575,7 +583,7 @@ __global__ void __launch_bounds__(kThreads, MODE == kByRows && sizeof(QT) == 2 ?
     };
     const bool edge = j0 + N > span.n || (!PREFIX && tokens > 1);
     float mx[2] = {m[0], m[1]};
-    float vmax = vref, vv[kScaled ? NT : 1][2];
+    float vv[kScaled ? NT : 1][2];
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
       if (kScaled) {
@@ -583,7 +591,6 @@ __global__ void __launch_bounds__(kThreads, MODE == kByRows && sizeof(QT) == 2 ?
         const float f0 = sc[k0], f1 = sc[k1];
         vv[i][0] = sc[X::kKeys + k0], vv[i][1] = sc[X::kKeys + k1];
         s[i][0] *= f0, s[i][1] *= kFew ? f0 : f1, s[i][2] *= kFew ? f1 : f0, s[i][3] *= f1;
-        vmax = fmaxf(vmax, fmaxf(vv[i][0], vv[i][1]));
       }
       if (edge) {
 #pragma unroll
@@ -605,14 +612,6 @@ __global__ void __launch_bounds__(kThreads, MODE == kByRows && sizeof(QT) == 2 ?
       m[u] = mx[u];
       l[u] *= keep[u];
     }
-    float vinv = 1.f;
-    if (kScaled) {
-      vmax = all_max(vmax);
-      vinv = vmax > 1e-37f ? 1.f / vmax : 0.f;
-      const float r = vref * vinv;
-      keep[0] *= r, keep[1] *= r;
-      vref = vmax;
-    }
 #pragma unroll
     for (int i = 0; i < NT; ++i)
 #pragma unroll
@@ -620,19 +619,44 @@ __global__ void __launch_bounds__(kThreads, MODE == kByRows && sizeof(QT) == 2 ?
         s[i][j] = ex2(fmaf(s[i][j], rscale[row_of(j)], -base[row_of(j)]));
         l[row_of(j)] += s[i][j];
       }
-    // most tiles change neither maximum nor reference: nothing to rescale
+    if (kScaled) {
+      float top[2] = {0.f, 0.f}, times[2];
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        s[i][0] *= vv[i][0], s[i][1] *= vv[i][kFew ? 0 : 1];
+        s[i][2] *= vv[i][kFew ? 1 : 0], s[i][3] *= vv[i][1];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) top[row_of(j)] = fmaxf(top[row_of(j)], s[i][j]);
+      }
+      bool renew = false;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        wtop[u] *= keep[u];
+        times[u] = two_to(wexp[u]);
+        renew |= keep[u] != 1.f || top[u] * times[u] > 32768.f;
+      }
+      if (__any_sync(0xffffffffu, renew)) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          wtop[u] = fmaxf(wtop[u], all_max(top[u]));
+          const int e = wtop[u] > 0.f ? 12 + 127 - (int)(__float_as_uint(wtop[u]) >> 23) : 0;
+          const int was = wexp[u];
+          wexp[u] = min(max(e, -126), 126);
+          keep[u] *= two_to(min(max(wexp[u] - was, -126), 127));
+          times[u] = two_to(wexp[u]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[i][j] *= times[row_of(j)];
+    }
+    // most tiles change neither maximum nor wexp: nothing to rescale
     if (!kF32 && __any_sync(0xffffffffu, keep[0] != 1.f || keep[1] != 1.f)) {
 #pragma unroll
       for (int i = 0; i < OT; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) o[i][j] *= keep[row_of(j)];
-    }
-    if (kScaled) {
-#pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        const float v0 = vv[i][0] * vinv, v1 = vv[i][1] * vinv;
-        s[i][0] *= v0, s[i][1] *= kFew ? v0 : v1, s[i][2] *= kFew ? v1 : v0, s[i][3] *= v1;
-      }
     }
 
     // ---- o += p v
@@ -775,7 +799,7 @@ __global__ void __launch_bounds__(kThreads, MODE == kByRows && sizeof(QT) == 2 ?
 #pragma unroll
     for (int i = 0; i < OT; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) o[i][j] *= vref;
+      for (int j = 0; j < 4; ++j) o[i][j] *= two_to(-wexp[kFew ? j & 1 : j >> 1]);
 
   // maxima in base 2 from here on
 #pragma unroll

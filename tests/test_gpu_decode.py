@@ -326,6 +326,42 @@ def test_attention_large_scores_and_signs():
             within(got, out, R.attention_tol(out, spread, size, n, dtype, 64, False))
 
 
+@pytest.mark.parametrize("dtype,quant", KINDS, ids=KIND_IDS)
+@pytest.mark.parametrize("heads,T", [((8, 2, 64), 1), ((8, 1, 128), 1), ((12, 1, 32), 1),
+                                     ((8, 2, 64), 24), ((4, 2, 80), 3)], ids=str)
+@pytest.mark.parametrize("gap", [6, 14, 17, 21, 28, 45])
+def test_attention_weights_far_below_the_largest(gap, heads, T, dtype, quant):
+    """A key far above the others in score and far below them in value (at the
+    first, a middle or the last column): what the others weigh still counts, in
+    equal and in unequal measure. Where the values grow as the weights fall, the
+    same in turn."""
+    Hq, Hk, D = heads
+    g = gen(gap + T)
+    B, n, scale = 6, 700, 0.125
+    q = (1 + 0.05 * randn(g, B, T, Hq, D)).to(dtype)
+    k, v = 0.02 * randn(g, 1, B, Hk, n, D), randn(g, 1, B, Hk, n, D)
+    v.abs_()  # nothing cancels
+    at = [0, 3, 350, 500, n - T, 0]
+    for b in range(B):
+        k[0, b, :, at[b]] = gap / (D * scale)
+        v[0, b, :, at[b]] *= (0.0, 2.0 ** -60, 2.0 ** -75, 0.0, 2.0 ** -60, 1e-3)[b]
+    # the last row: a tenth of the others is larger by what it lies lower
+    k[0, -1, :, 7::10] = -gap / (D * scale)
+    v[0, -1, :, 7::10] *= math.exp(gap)
+    if quant:
+        (k, ks), (v, vs) = R.quantise(k), R.quantise(v)
+        cache = KVCache(k, v, ks, vs, dtype=dtype)
+        kd, vd = R.dequantised(k, ks), R.dequantised(v, vs)
+    else:
+        cache = KVCache(k.to(dtype), v.to(dtype))
+        kd, vd = cache.k.double(), cache.v.double()
+    col = n - T
+    got = cache_attention(q, cache, 0, col, scale)
+    keep = R.visible(T, n, col, None, 0, B, "cuda")
+    out, spread, size, m = R.attention(q, kd[0], vd[0], keep, scale)
+    within(got, out, R.attention_tol(out, spread, size, m, dtype, D, quant))
+
+
 @pytest.mark.parametrize("heads", [(16, 8, 64), (32, 8, 128), (4, 2, 16), (8, 8, 80)], ids=str)
 @pytest.mark.parametrize("scale", [0.1, -0.1])
 def test_attention_prefix_with_growing_scores(heads, scale):

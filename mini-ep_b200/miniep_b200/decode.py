@@ -64,9 +64,6 @@ def _flat(t):
     return t if t.data_ptr() & 15 == 0 else t.clone()
 
 
-_stream_of = torch._C._cuda_getCurrentRawStream
-
-
 class _on:
     """Calls into the library with the tensors' device current."""
 
@@ -77,7 +74,7 @@ class _on:
         self.before = torch.cuda.current_device()
         if self.before != self.index:
             torch.cuda.set_device(self.index)
-        return _stream_of(self.index)
+        return torch._C._cuda_getCurrentRawStream(self.index)
 
     def __exit__(self, *exc):
         if self.before != self.index:

@@ -2,6 +2,8 @@
 library's own argument checks (all made before any CUDA call)."""
 import ctypes as C
 import re
+import subprocess
+import sys
 from pathlib import Path
 
 import pytest
@@ -157,3 +159,17 @@ def test_replayed_steps_behind_the_cache_are_refused():
     with pytest.raises(ValueError, match="columns"):
         Engine(m).decode_graphed(shard, 3)
     assert shard.used == 3 and shard.generated == [[]]
+
+
+def test_the_package_imports_on_a_torch_without_cuda():
+    """Planners, oracle forms and the host side need no CUDA build of torch:
+    without its bindings' private names the package still imports."""
+    code = ("import torch\n"
+            "for n in [n for n in dir(torch._C) if n.startswith('_cuda_')]:\n"
+            "    delattr(torch._C, n)\n"
+            "import miniep_b200 as M\n"
+            "M.plan_balanced, M.Placement, M.KVCache\n")
+    root = Path(M.__file__).resolve().parents[1]
+    r = subprocess.run([sys.executable, "-c", f"import sys; sys.path.insert(0, {str(root)!r})\n" + code],
+                       capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr

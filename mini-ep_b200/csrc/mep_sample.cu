@@ -400,7 +400,7 @@ __global__ void __launch_bounds__(kNT, 2) k_sample(const SampleArgs a, int cache
   W.lmax = lmax;
   // 34 temperatures below the best a weight is 2^-49; lmax = inf leaves only
   // its equals, -inf never weighs
-  W.lcut = fmaxf(W.lmax - 34.f * temp, -3.402823466e38f);
+  W.lcut = W.lmax == INFINITY ? W.lmax : fmaxf(W.lmax - 34.f * temp, -3.402823466e38f);
   W.top = W.lmax;
   W.c = 369.329930467574632284 / (double)temp;  // 256 log2(e)
   W.scale = min(46, 62 - bits);

@@ -688,6 +688,28 @@ def test_sample_infinities_nan_and_bounds():
     assert sample_tokens(logits, u).tolist() == [0, 9, 9, 0]
 
 
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("V", [5, 3001, 70001])
+def test_sample_infinite_logits_at_any_temperature(V, dtype):
+    """+inf logits share the mass even where 34 temperatures pass fp32's range,
+    and finite ones share it alike where the temperature is infinite."""
+    inf = math.inf
+    logits = randn(gen(V), 8, V, dtype=dtype)
+    at = torch.tensor([1, V // 2, V - 2], device="cuda")
+    logits[:4, at] = inf
+    u = torch.tensor([0.0, 0.34, 0.67, 0.99] * 2, device="cuda")
+    for t in (1.0, 1e37, 3e38, inf):
+        temp = torch.full((8,), t, device="cuda")
+        for k, p, m in ((0, 1.0, 0.0), (0, 1.0, 0.3), (3, 1.0, 0.0), (0, 0.9999, 0.0),
+                        (4, 0.9999, 0.0)):
+            tok, lp = sample_tokens(logits, u, temp, k, p, m, return_logprobs=True)
+            assert tok[:4].tolist() == [at[0].item(), at[1].item(), at[2].item(), at[2].item()]
+            assert ((lp[:4] + math.log(3)).abs() <= 2 * R.FP32 * math.log(3)).all()
+        if t == inf:  # every finite logit weighs the same
+            want = (u[4:].double() * V).floor().long()
+            assert torch.equal(sample_tokens(logits, u, temp)[4:], want)
+
+
 def test_sample_row_values_outside_their_ranges():
     """Per-row values cannot be refused without waiting for them: each has a
     meaning (temperature below 0 or NaN: greedy; top_k below 0: all; top_p not

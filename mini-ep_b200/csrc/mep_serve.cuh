@@ -78,7 +78,9 @@ inline const char* bad_heads(int64_t dtype, int64_t cache_dtype, int64_t batch, 
   if (batch > 65535 || tokens > (1 << 24)) return "batch up to 65535, tokens up to 2^24";
   if (kv_heads < 1 || q_heads < 1 || q_heads % kv_heads != 0 || q_heads > 1024)
     return "q_heads must be a multiple of kv_heads, up to 1024";
-  if (batch * tokens * q_heads > 0x7fffffff) return "batch * tokens * q_heads up to 2^31 - 1";
+  // rows are counted in 32 bits, and up to whole tiles of 256
+  if (batch * tokens * q_heads > 0x7fffffff - 1024)
+    return "batch * tokens * q_heads up to 2^31 - 1025";
   if (head_dim < 16 || head_dim > kMaxHeadDim || head_dim % 16 != 0)
     return "head_dim must be a multiple of 16 up to 128";
   return nullptr;

@@ -66,6 +66,17 @@ def test_bad_heads(lib, bad, word):
     assert word in lib.mep_last_error(None)
 
 
+@pytest.mark.parametrize("B,T,Hq", [(14351, 149640, 1), (1, 1 << 21, 1023), (65535, 1 << 15, 1)],
+                         ids=str)
+def test_rows_that_round_up_past_32_bits(lib, B, T, Hq):
+    """Rows are counted in tiles of up to 256: the last whole one has to fit 32 bits."""
+    n = C.c_int64()
+    rc = lib.mep_cache_attention_workspace(*_heads(B=B, T=T, Hq=Hq, Hk=1), T, 0, 0, C.byref(n))
+    assert rc == (1 if B * T * Hq > 2 ** 31 - 1025 else 0)
+    if rc:
+        assert b"2^31" in lib.mep_last_error(None)
+
+
 def test_columns_and_null_tensors(lib):
     for cap, col, word in ((8, 8, b"fit"), (8, -1, b"fit"), (-1, 0, b"capacity"), (8, 0, b"null")):
         assert _store(lib, _heads(), cap, col) == 1

@@ -191,7 +191,9 @@ def _column(col, device):
         _tensor(col, "col", device, torch.int64)
         _need(col.numel() == 1, "col must hold one column")
         return -1, col.data_ptr()
-    return int(col), 0
+    col = int(col)
+    _need(0 <= col < 1 << 62, f"column {col} does not fit the cache")
+    return col, 0
 
 
 def _heads(q, cache: KVCache):
@@ -287,6 +289,7 @@ def cache_attention(q, cache: KVCache, layer: int, col, scale: float, *, lengths
               "the prefix and the cache have different heads")
         _need(0 <= layer < prefix.layers, f"layer {layer} outside the prefix's {prefix.layers}")
         P, (pk, pv) = prefix.columns, prefix._ptrs[layer]
+    _need(0 <= prompt_cols < 1 << 62, "prompt_cols must not be negative, up to 2^62 - 1")
     host, devcol = _column(col, dev)
     dc, code = _DTYPES[dt], cache._code
     nbytes = _attention_workspace(dc, code, B, T, Hq, Hk, D, cache.capacity, host, P)

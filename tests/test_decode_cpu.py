@@ -77,6 +77,12 @@ def test_rows_that_round_up_past_32_bits(lib, B, T, Hq):
         assert b"2^31" in lib.mep_last_error(None)
 
 
+@pytest.mark.parametrize("col", [-1, 1 << 62, 1 << 63, 1 << 70, -(1 << 63) - 1])
+def test_host_columns_past_64_bits(col):
+    with pytest.raises(MEPError, match="column"):
+        M.decode._column(col, None)
+
+
 def test_columns_and_null_tensors(lib):
     for cap, col, word in ((8, 8, b"fit"), (8, -1, b"fit"), (-1, 0, b"capacity"), (8, 0, b"null")):
         assert _store(lib, _heads(), cap, col) == 1

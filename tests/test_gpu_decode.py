@@ -823,3 +823,17 @@ def test_refusals_on_the_gpu():
                  (x, u, 1.0, 0, 1.0, 1.5), (x, u, u.double()), (x, u, u[:1]), (x, u, 1.0, u)):
         with pytest.raises(MEPError):
             sample_tokens(*args)
+
+
+@pytest.mark.parametrize("col", [-1, 1 << 62, (1 << 63) - 1, 1 << 63, 1 << 70, -(1 << 63) - 1])
+def test_columns_past_64_bits_are_refused(col):
+    cache = KVCache.empty(1, 2, 2, 8, 64, BF)
+    q, k = (torch.zeros(2, 1, h, 64, dtype=BF, device="cuda") for h in (4, 2))
+    cos, sin = R.rope_tables(8, 64)
+    pos = torch.zeros(2, 1, dtype=torch.long, device="cuda")
+    with pytest.raises(MEPError):
+        norm_rope_store(q, k, k, cos, sin, pos, cache, 0, col)
+    with pytest.raises(MEPError):
+        cache_attention(q, cache, 0, col, 1.0)
+    with pytest.raises(MEPError):
+        cache_attention(q, cache, 0, 0, 1.0, prompt_cols=col)

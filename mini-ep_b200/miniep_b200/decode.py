@@ -341,7 +341,8 @@ def sample_tokens(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, *,
             nums.append(num(1))
         else:
             ptrs.append(None)
-            nums.append(min(num(x), 0x7fffffff) if dt == torch.int32 else num(x))
+            # an integer far below 0 stays below it in 32 bits
+            nums.append(max(min(num(x), 0x7fffffff), -1) if dt == torch.int32 else num(x))
     tokens = torch.empty(B, dtype=torch.int64, device=dev)
     logprobs = torch.empty(B, dtype=torch.float32, device=dev) if return_logprobs else None
     with _on(dev) as stream:

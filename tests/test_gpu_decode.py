@@ -837,3 +837,9 @@ def test_columns_past_64_bits_are_refused(col):
         cache_attention(q, cache, 0, col, 1.0)
     with pytest.raises(MEPError):
         cache_attention(q, cache, 0, 0, 1.0, prompt_cols=col)
+
+
+@pytest.mark.parametrize("k", [-1, -(1 << 31) - 1, 5 - (1 << 32), 5 - (1 << 64)])
+def test_negative_top_k_is_refused(k):
+    with pytest.raises(MEPError, match="top_k"):
+        sample_tokens(torch.zeros(2, 9, device="cuda"), torch.zeros(2, device="cuda"), 1.0, k)

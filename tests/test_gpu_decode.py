@@ -282,6 +282,17 @@ def test_attention_with_prefix(span, P, heads, dtype, quant):
     attend_case(4, heads, span, dtype, quant, P)
 
 
+@pytest.mark.parametrize("dtype,quant", KINDS, ids=KIND_IDS)
+@pytest.mark.parametrize("heads,span", [((4, 2, 64), (2, 1024, 1024, 0, 5)),
+                                        ((8, 2, 128), (2, 333, 333, 0, 1)),
+                                        ((6, 1, 80), (1, 1021, 1500, 300, 900))], ids=str)
+@pytest.mark.parametrize("P", [0, 200])
+def test_attention_of_whole_prompts(P, heads, span, dtype, quant):
+    """What a prefill asks for: every token of ragged prompts at once over the
+    prompt's own columns, and a later part of one over what was there before."""
+    attend_case(12, heads, span, dtype, quant, P)
+
+
 def test_attention_without_lengths():
     for P in (0, 77):
         attend_case(5, (16, 8, 64), (3, 4, 130, 9, 1), BF, True, P, use_lengths=False)

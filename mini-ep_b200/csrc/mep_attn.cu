@@ -12,6 +12,16 @@
 // whole batch, so that each key is read once for all of them. The keys are cut
 // into splits that run on different SMs; their partial results (fp32 sums, the
 // maximum in base 2) meet in k_attn_join.
+//
+// Measured, device time. One token a row: 8 rows over 32,768 columns, 32 / 8
+// heads of 128, bf16: 158 us, the bytes at the measured copy rate; in e4m3 92 us
+// for 81 of bytes. 64 ragged rows of 577 to 1089 columns, 16 / 8 heads of 64,
+// e4m3: 16.6 us for 8.9 (the chain of a row's 9 tiles, and issue at 0.46). One row
+// of 257 columns: 8.2 us, launch and latency. Whole prompts over their own columns
+// go by the warp-level products, which bound them with the exponentials beside
+// (tensor pipe 0.42, issue 0.44 busy): 16 x 1021 tokens, 32 / 8 heads of 128, bf16
+// 591 us, 212 TFLOP/s of the visible products (78 us at the measured rate), e4m3
+// 730, fp32 4.7 ms (three tf32 products for one, spills at 255 registers).
 #include <cstdint>
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
@@ -1000,8 +1010,17 @@ struct Plan {
   int64_t out_rows, bytes;
 };
 
-constexpr int kSlots = 296;         // CTAs resident at a time: 148 SMs, two each
-constexpr int64_t kMinKeys = 128;   // keys of a split, at least
+// CTAs counted as resident at a time (148 SMs, two each): calls of as many are
+// not split, smaller ones to about twice as many. Both sides, 16 / 8 heads of 64:
+// with 148 in its place 20 rows of 8192 columns in e4m3 take 53.8 us against 39.0
+// (160 CTAs, then whole), but 8 rows of 2100 in bf16 10.3 against 16.4 and one of
+// 32,768 22.6 against 36.8 (fewer partial results to join); with 592 they take
+// 22.6 and 63.2.
+constexpr int kSlots = 296;
+// Keys of a split, at least. With 64 one row of 1089 columns takes 10.3 us against
+// 8.2; with 256 one of 2100 8.2 against 12.0, but 4 rows behind a prefix of 509 in
+// fp32 20.3 against 16.4.
+constexpr int64_t kMinKeys = 128;
 constexpr int kMaxCluster = 8;
 
 int splits_for(int64_t keys, int64_t ctas) {
@@ -1011,12 +1030,20 @@ int splits_for(int64_t keys, int64_t ctas) {
   return (int)(want < most ? want : most);
 }
 
+// Up to 8 rows transposed took 64 rows in e4m3 from 20.5 to 16.9 us, 16-bit
+// queries only: split tf32 operands have no transposed form here.
 Mode mode_for(int dtype, int64_t rows) {
   return rows <= 8 && dtype == MEP_BF16 ? kFewRows : rows <= 16 ? kByKeys : kByRows;
 }
 int rows_of(Mode m) { return m == kFewRows ? 8 : m == kByKeys ? 16 : 64; }
 
-constexpr int64_t kTcRows = 128;  // rows of a key/value head from which the prefix is tcgen05's
+// Rows of a key/value head from which the prefix is tcgen05's. Both sides at 128
+// rows on each of 8 heads of 64, tcgen05 against warp-level products: 4096 columns
+// 24.6 us against 31.3, 16,384 36.9 against 49.7, but 300 columns 25.0 against 18.5
+// and 1024 22.6 against 18.5 (too few units for the SMs); 6144 rows on each of 8
+// heads of 128 behind 4099, the whole call, 136 against 477. At 64 rows: 4096 columns 18.5 both, 16,384 28.7 against
+// 34.9, 1024 18.5 against 14.4.
+constexpr int64_t kTcRows = 128;
 
 Plan plan_for(int dtype, int64_t batch, int64_t tokens, int q_heads, int kv_heads, int head_dim,
               int64_t capacity, int64_t col, int64_t prefix_cols) {
@@ -1035,7 +1062,9 @@ Plan plan_for(int dtype, int64_t batch, int64_t tokens, int q_heads, int kv_head
     p.tc = plan_prefix_tc(pre_rows, kv_heads, prefix_cols);
     p.prefix_splits = p.tc.slots;
   }
-  // a split or two more than a cluster holds costs less than another launch
+  // up to twice as many splits as a cluster holds cost more, with another launch
+  // to join them, than the cluster's 8: one row of 1089 columns 10.3 us against
+  // 8.2, 8 rows of 2100 in e4m3 14.4 against 11.9
   if (p.own != kByRows && p.own_splits <= 2 * kMaxCluster && p.own_splits > kMaxCluster)
     p.own_splits = kMaxCluster;
   p.joined = p.own != kByRows ? p.own_splits <= kMaxCluster : p.own_splits == 1;

@@ -12,10 +12,11 @@
 // is the largest e4m3 value), quantised from the fp32 result: one rounding.
 //
 // Measured: 16 x 1021 tokens of 32 + 8 + 8 heads of 128, bf16, normalised, into
-// an e4m3 cache (370 MB): 96 us, 3.9 TB/s; instruction issue is 0.78 busy (two
-// reductions, a division and the conversions of each head). One token: 2.0 us,
-// 64 tokens of 32 heads of 64: 3.0 us. Reading the same columns back (101 MB):
-// 19 us, 5.4 TB/s.
+// an e4m3 cache (370 MB): 96 us, 3.9 TB/s; issue is 0.6 busy with 43 % of the warps
+// active, so what holds it is each head's chain (load, two reductions, a division,
+// conversions). The same into a bf16 cache (418 MB) 94 us, 4.4 TB/s, fp32 into fp32
+// (820 MB) 145 us, 5.7 TB/s. One token: 2.0 us, 64 tokens of 32 heads of 64: 3.0 us.
+// Reading the same columns back (101 MB): 19 us, 5.4 TB/s.
 #include <cstdint>
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
@@ -264,9 +265,12 @@ void launch_store_l(const StoreArgs& a, cudaStream_t st) {
   const int per_warp = 32 / (a.head_dim / 8);
   const int passes = (a.q_heads + per_warp - 1) / per_warp + 2 * ((a.kv_heads + per_warp - 1) / per_warp);
   const int64_t tokens = a.batch * a.tokens;
-  // few tokens: one pass a warp, for the latency; many (32 warps on each of
-  // 148 SMs, four passes each): all of a token's up to 12, else half of them,
-  // which share the table rows
+  // few tokens: one pass a warp, for the latency (64 tokens of 48 heads of 128,
+  // bf16: 4.1 us against 8.1); many (32 warps on each of 148 SMs, four passes
+  // each): all of a token's up to 12, else half of them, which share the table
+  // rows (16 x 1021 such tokens 96 us, 197 with one pass a warp). Half against all
+  // of 24 passes: 1024 tokens 8.2 us against 10.3, 8 x 1021 53.3 against 51.3; of 8
+  // passes: 8 x 1021 18.5 against 16.4.
   const int share = tokens * passes < (int64_t)148 * 32 * 4 ? 1 : passes <= 12 ? passes : (passes + 1) / 2;
   const int parts = (passes + share - 1) / share;
   const int warps = share == 1 ? 4 : 8;

@@ -12,9 +12,9 @@
 // less where the row's sum would pass 62 bits): integer sums do not depend on
 // their order, and a weight, computed in 64 bits, is off by half a unit.
 //
-// Measured, bf16 / fp32 logits: 256 rows of 100,003 with top_p 0.95 72 / 207
-// us, unfiltered 53 / 103 us, with top_k 50 71 / 86 us, greedy 21 / 35 us; one
-// row of 49,155 with top_k and top_p 16.5 us, greedy 6.3 us. Reading the logits
+// Measured, bf16 / fp32 logits: 256 rows of 100,003 with top_p 0.95 72 / 208
+// us, unfiltered 53 / 104 us, with top_k 50 70 / 86 us, greedy 21 / 36 us; one
+// row of 49,155 with top_k and top_p 16.4 us, greedy 6.2 us. Reading the logits
 // would take 8 / 16 us at 256 rows: what bounds it is the work on every token
 // (bf16, top_p: 51 warp instructions for 32 tokens, a shared-memory addition
 // and a read among them) and 256 CTAs on 148 SMs, for a few rows the chain of
@@ -582,8 +582,8 @@ __global__ void __launch_bounds__(kNT, 2) k_sample(const SampleArgs a, int cache
                       (W.lcut >= 0.f || cut_mag < kSmall + kHalf - 1);
     // a few tokens by top_k are sooner on one CTA's list (15 us against 20 for a
     // row of 49,155, 22 against 29 for 64; alike at 256 x 100003), short runs
-    // without a border by their exponentials (11.9 against 12.5 us at 2000 ids a
-    // CTA, 15.9 against 15.1 at 6000). The row's CTAs have to choose alike, as
+    // without a border by their exponentials (11.9 against 12.3 us at 2000 ids a
+    // CTA, 15.8 against 14.5 at 6000). The row's CTAs have to choose alike, as
     // the two ways meet at different barriers: `per` is the same in all of them,
     // the last one's own run may be shorter.
     const bool brief = by_k ? top_k <= 128 : !by_p && per * E < 4096;
@@ -803,8 +803,9 @@ __global__ void __launch_bounds__(kNT, 2) k_sample(const SampleArgs a, int cache
     const uint32_t n = S.r_cnt, n_bin = S.r_hi;
     const u64 above0 = S.r_above;
     // all candidates to the leading CTA if it finishes them sooner than all
-    // CTAs the row (behind one border; two borders cost much more), else the
-    // border's bin alone, if it can sort that
+    // CTAs the row, else the border's bin alone, if it can sort that. Behind one
+    // border 2048 candidates on one CTA cost more than 256 (one row of 49,155, fp32,
+    // top_p: 53 us against 22.6), behind two they save (64 mixed rows: 64 us with 256)
     const bool whole = n <= (by_k && by_p ? kList : kNT / 2);
     if (whole || n_bin <= kList) {
       Shared* lead = cluster.map_shared_rank(&S, 0);
@@ -1032,10 +1033,13 @@ constexpr int64_t kRunBytes = 52 << 10;
 template <typename T>
 int launch_sample(const SampleArgs& a, int64_t rows, cudaStream_t st) {
   // CTAs of a row: one from 148 rows on (a table of weights in each costs more
-  // than it saves), else up to 8 so that every SM has work, 512 ids each or more
+  // than it saves: 148 rows of 49,155, bf16, top_p 33 us, with four 70; fp32 rows of
+  // mixed filters would gain, 80 and 68), else up to 8 so that every SM has work
+  // (one row, top_p, 22.6 us, on one CTA 33; fp32 22.6 and 70), 512 ids each or more
   int nc = 1;
   while (nc < kMaxCtas && rows * nc < 148 && a.vocab >= nc * 1024) nc *= 2;
-  // a CTA's run in shared memory if two CTAs still fit an SM
+  // a CTA's run in shared memory if two CTAs still fit an SM (64 rows of 49,155,
+  // fp32, top_p: 43 us against 46 from L2; most others alike)
   const int64_t run = (a.vocab * (int64_t)sizeof(T) / 16 + 2 + nc) / nc * 16;
   const int cached = run <= kRunBytes;
   const int smem = (int)((sizeof(Shared) + 15) / 16 * 16 + (cached ? run : 0));

@@ -367,9 +367,12 @@ int mep_kv_read(int dtype, int64_t batch, int kv_heads, int head_dim, const void
  * columns [0, lengths[b]) of the padded prompt_cols, and what was decoded
  * behind them (lengths NULL: every c <= col + t). A query that sees nothing
  * gets zeros. scale: finite, |scale| <= 2^127. q: (batch, tokens, q_heads,
- * head_dim) strided; out the same,
- * contiguous. workspace: mep_cache_attention_workspace bytes, the caller's, in
- * use until the call's work on `stream` is done.
+ * head_dim) strided; out the same, contiguous. workspace:
+ * mep_cache_attention_workspace bytes, the caller's, in use until the call's
+ * work on `stream` is done. The kernel for a prefix behind 128 rows a head and
+ * more waits for its own copies and products, 2 s at the longest; rows that a
+ * wait which ran out leaves unfinished come out as NaN, and the context stays
+ * usable.
  */
 typedef struct mep_attention_args {
   int64_t dtype, cache_dtype, batch, tokens, q_heads, kv_heads, head_dim;
@@ -393,10 +396,8 @@ typedef struct mep_attention_args {
 } mep_attention_args;
 int mep_cache_attention(const mep_attention_args* args, void* stream);
 /*
- * Test hook: until it is called with -1, the loader of every CTA of the large
- * batches' prefix kernel stops behind its K load number `loads` (from 0) as if
- * a wait had run out. Waits are bounded (2 s); the rows that one leaves
- * unfinished come out as NaN, and the context stays usable.
+ * Test hook: until it is called with -1, the loader of every CTA of that kernel
+ * stops behind its K load number `loads` (from 0) as if a wait had run out.
  */
 int mep_debug_prefix_loads(int loads);
 /* Workspace of such a call (host arithmetic only). col: as given to the call,

@@ -390,8 +390,8 @@ __global__ void __launch_bounds__(kThreads, MODE == kByRows && sizeof(QT) == 2 ?
         }
     } else {
       // Codes are exact in fp16, so the products are fp16 ones. A query row is
-      // scaled by a power of two to a largest magnitude in [1, 2): its bf16
-      // values stay exact down to 2^-14 of it, and below that are off by 2^-25
+      // scaled by a power of two to a largest magnitude in [2^14, 2^15): its bf16
+      // values stay exact down to 2^-31 of it, and below that are off by 2^-39
       // of it at most.
       uint4 raw[QR][DP / 32];
 #pragma unroll
@@ -418,9 +418,8 @@ __global__ void __launch_bounds__(kThreads, MODE == kByRows && sizeof(QT) == 2 ?
         for (int i = 0; i < DP / 4; ++i) m = fmaxf(m, fabsf(qv[i]));
         m = quad_max(m);
         const int ex = (int)(__float_as_uint(m) >> 23) - 127;
-        const int e = m > 0.f && ex < 128 ? min(max(ex, -126), 126) : 0;
-        const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-        const float up = __uint_as_float((uint32_t)(127 + e) << 23);
+        const int e = m > 0.f && ex < 128 ? max(ex - 14, -126) : 0;
+        const float down = two_to(-e), up = two_to(e);
         if (kFew) {
           rscale[0] *= __shfl_sync(0xffffffffu, up, 8 * t4);
           rscale[1] *= __shfl_sync(0xffffffffu, up, 8 * t4 + 4);

@@ -373,6 +373,34 @@ def test_attention_weights_far_below_the_largest(gap, heads, T, dtype, quant):
     within(got, out, R.attention_tol(out, spread, size, m, dtype, D, quant))
 
 
+@pytest.mark.parametrize("dtype,quant", KINDS, ids=KIND_IDS)
+@pytest.mark.parametrize("heads,T", [((8, 2, 64), 1), ((8, 1, 128), 2), ((12, 1, 32), 1),
+                                     ((8, 2, 64), 24), ((4, 2, 80), 3)], ids=str)
+@pytest.mark.parametrize("by", [10, 16, 22, 28])
+def test_attention_queries_with_one_large_value(by, heads, T, dtype, quant):
+    """One value of a query 2^by times the others, where the keys are zero: the
+    others decide, with all their bits."""
+    Hq, Hk, D = heads
+    g = gen(by + T)
+    B, n = 3, 300
+    q = randn(g, B, T, Hq, D)
+    q[..., 5] = 2.0 ** by
+    q = q.to(dtype)
+    k, v = randn(g, 1, B, Hk, n, D), randn(g, 1, B, Hk, n, D)
+    k[..., 5] = 0
+    if quant:
+        (k, ks), (v, vs) = R.quantise(k), R.quantise(v)
+        cache = KVCache(k, v, ks, vs, dtype=dtype)
+        kd, vd = R.dequantised(k, ks), R.dequantised(v, vs)
+    else:
+        cache = KVCache(k.to(dtype), v.to(dtype))
+        kd, vd = cache.k.double(), cache.v.double()
+    got = cache_attention(q, cache, 0, n - T, 0.5)
+    keep = R.visible(T, n, n - T, None, 0, B, "cuda")
+    out, spread, size, m = R.attention(q, kd[0], vd[0], keep, 0.5)
+    within(got, out, R.attention_tol(out, spread, size, m, dtype, D, quant))
+
+
 @pytest.mark.parametrize("heads", [(16, 8, 64), (32, 8, 128), (4, 2, 16), (8, 8, 80)], ids=str)
 @pytest.mark.parametrize("scale", [0.1, -0.1])
 def test_attention_prefix_with_growing_scores(heads, scale):

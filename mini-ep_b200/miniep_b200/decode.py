@@ -140,18 +140,25 @@ class KVCache:
         """Columns [start, end) of one layer, (batch, kv_heads, end - start,
         head_dim) each, in the model dtype: a view of a cache that holds it,
         code * scale rounded once of a quantised one."""
+        return self._read(layer, 0, self.batch, start, end)
+
+    def _read(self, layer: int, first: int, rows: int, start: int, end: int):
+        """`read` of batch rows [first, first + rows)."""
         kp, vp, ksp, vsp = self.layer(layer)
         _need(0 <= start <= end <= self.capacity,
               f"columns [{start}, {end}) outside the cache's {self.capacity}")
         if not self.quantized:
-            return self.k[layer, :, :, start:end], self.v[layer, :, :, start:end]
-        shape = (2, self.batch, self.kv_heads, end - start, self.head_dim)
+            return tuple(t[layer, first:first + rows, :, start:end] for t in (self.k, self.v))
+        shape = (2, rows, self.kv_heads, end - start, self.head_dim)
         out = torch.empty(shape, dtype=self.dtype, device=self.device)
         k, v = out[0], out[1]
+        skip = first * self.kv_heads * self.capacity  # cached rows before them
+        at = skip * self.head_dim
         with _on(self.device) as stream:
-            check(_lib.lib().mep_kv_read(_DTYPES[self.dtype], self.batch, self.kv_heads,
-                                         self.head_dim, kp, vp, ksp, vsp, self.capacity, start,
-                                         end - start, k.data_ptr(), v.data_ptr(), stream),
+            check(_lib.lib().mep_kv_read(_DTYPES[self.dtype], rows, self.kv_heads,
+                                         self.head_dim, kp + at, vp + at, ksp + 4 * skip,
+                                         vsp + 4 * skip, self.capacity, start, end - start,
+                                         k.data_ptr(), v.data_ptr(), stream),
                   None, "KVCache.read")
         return k, v
 
@@ -180,9 +187,9 @@ class SharedPrefix:
         """A copy of the first `columns` columns of one row, of every layer
         (read back to the model dtype from a quantised cache)."""
         _need(0 <= row < cache.batch, f"row {row} outside [0, {cache.batch})")
-        got = [cache.read(l, 0, columns) for l in range(cache.layers)]
-        return cls(torch.stack([k[row] for k, _ in got]).contiguous(),
-                   torch.stack([v[row] for _, v in got]).contiguous())
+        got = [cache._read(l, row, 1, 0, columns) for l in range(cache.layers)]
+        return cls(torch.cat([k for k, _ in got]).contiguous(),
+                   torch.cat([v for _, v in got]).contiguous())
 
 
 def _column(col, device):

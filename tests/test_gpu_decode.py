@@ -206,6 +206,34 @@ def test_read_many_heads():
         within(got, want, R.HALF[F32] * want.abs())
 
 
+@pytest.mark.parametrize("quant", [False, True], ids=["plain", "e4m3"])
+def test_prefix_from_a_row_of_a_cache(quant):
+    """One row's columns of every layer, from a layout whose rows lie off the
+    16-byte grid of the scales; the other rows cost no memory."""
+    g = gen(41)
+    for L, B, Hk, cap, D, columns in ((3, 5, 3, 7, 48, 5), (1, 2, 1, 1, 16, 1), (2, 3, 2, 4, 64, 0),
+                                      (4, 64, 8, 1024, 64, 1000)):
+        k, v = randn(g, L, B, Hk, cap, D), randn(g, L, B, Hk, cap, D)
+        if quant:
+            (kc, ks), (vc, vs) = R.quantise(k), R.quantise(v)
+            cache = KVCache(kc, vc, ks, vs, dtype=BF)
+        else:
+            cache = KVCache(k.to(BF), v.to(BF))
+        del k, v
+        row = B - 1
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        torch.cuda.reset_peak_memory_stats()
+        prefix = SharedPrefix.from_cache(cache, row, columns)
+        # the result, and what it is gathered from
+        took = torch.cuda.max_memory_allocated() - before
+        assert took <= 3 * (2 * L * Hk * columns * D * 2) + L * 4096 + 4096
+        assert prefix.k.shape == (L, Hk, columns, D)
+        for l in range(L):
+            want = cache.read(l, 0, columns)
+            assert torch.equal(prefix.k[l], want[0][row]) and torch.equal(prefix.v[l], want[1][row])
+
+
 def test_store_and_read_of_nothing():
     cache = KVCache.empty(1, 0, 2, 4, 64, BF, quantized=True)
     q, k = torch.empty(0, 1, 4, 64, dtype=BF, device="cuda"), torch.empty(0, 1, 2, 64, dtype=BF, device="cuda")
